@@ -341,6 +341,145 @@ int prism_hip_sync(prism_hip_ctx *ctx, void *stream);
 /* The context's internal stream (a hipStream_t), for ordering caller work. */
 void *prism_hip_stream(prism_hip_ctx *ctx);
 
+/* ---- serving many requests: the paged 8-bit cache ----------------------------------
+ * What runs between the projections of a batch of requests.  All of it is device memory
+ * of the caller's and stream ordered, as the device-pointer calls above: the calls take
+ * the context stream, report at the next prism_hip_sync and can be captured once each has
+ * run uncaptured at the sizes of the capture.  Pointers are aligned to their element;
+ * the cache's to 16 bytes.  The reference pages its cache on the host in binary16 or with
+ * 3 and 4 bits a value (src/graph.rs, docs/quantized-kv.md); this is a design of its own. */
+#define PRISM_DTYPE_F32 0
+#define PRISM_DTYPE_F16 1
+#define PRISM_DTYPE_BF16 2
+/* 8-bit codes: two's complement -127..127, or OCP e4m3 (largest value 448). */
+#define PRISM_CACHE_INT8 0
+#define PRISM_CACHE_E4M3 1
+
+/* One layer's cache of `pages` pages of page_size positions (16, 32, 64, 128 or 256) for
+ * kv_heads heads of head_dim (64, 128 or 256) values.  Codes:
+ *   k[page][head][position][dimension], v[page][head][dimension][position]
+ * (values transposed, so that both products of the attention read runs of bytes); a value
+ * is its code times k_scale / v_scale[page][head].  pages * page_size < 2^31.  The memory
+ * may start as it is: a page's scales are set when its first position is written. */
+typedef struct prism_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    uint32_t format; /* PRISM_CACHE_* */
+    uint32_t pages, page_size, kv_heads, head_dim;
+} prism_kv_cache;
+
+/* One step of `requests` requests: pages, positions and slots of their new tokens.
+ *   lengths[r]  tokens of request r in the cache; added[r] its new tokens, or -1: the
+ *               request has ended and gives back the pages of its lengths[r] tokens.
+ *   block_table [requests][max_pages]: column j holds the page of positions
+ *               j * page_size ...; only the columns of new pages are written.
+ *   free_pages  a stack of free pages, *free_count of them, room for free_capacity.  Pages
+ *               given back go on top, in order of request and column; new ones are then
+ *               taken from the top in that order, so no result depends on timing.
+ *   new_lengths, offsets[requests + 1] (exclusive sums of the new tokens), and for every
+ *   token its position, its slot (page * page_size + place in the page) and its owner;
+ *   behind the last token, up to max_tokens, position 0, slot -1, owner -1.
+ *   counts[4]   free pages after the step, tokens, pages taken, pages short.
+ * new_lengths may be lengths, and counts may be free_count's memory, so that a captured
+ * step carries its own state on.  A step that has too few free pages, more tokens than
+ * max_tokens, a length past max_pages pages, a negative one, or no room for pages given
+ * back is refused as a whole: new_lengths = lengths, no tokens, the stack and table as
+ * they were, counts = {free pages, 0, 0, pages short}, and the next prism_hip_sync is
+ * PRISM_ERR_RESOURCE (pages short) or PRISM_ERR_INVALID_INPUT. */
+typedef struct prism_kv_plan {
+    uint32_t requests, max_pages, max_tokens, page_size, free_capacity;
+    const int32_t *lengths, *added;
+    int32_t *block_table, *free_pages;
+    const int32_t *free_count;
+    int32_t *new_lengths, *offsets, *positions, *slots, *owners, *counts;
+} prism_kv_plan;
+int prism_hip_kv_plan_device(prism_hip_ctx *ctx, const prism_kv_plan *plan, void *stream);
+
+/* Rotary positions.  The rotation keeps the frequencies (radians a position) of dims / 2
+ * pairs on the device; dims is even, 2 to 256.  Pairs are (i, i + dims/2), or (2i, 2i + 1)
+ * where interleaved; dimensions from dims on pass unrotated.  magnitude multiplies the
+ * cosines and sines (1 without scaling).  NULL on failure.  Destroy it before its context.
+ * prism_hip_rope_frequencies fills out[dims / 2] on the host: base^(-2i/dims), for long
+ * contexts divided by factor: each (original = 0), or by how often the pair turns in the
+ * `original` positions the model has seen, r = original * f / 2 pi: kept from beta turns,
+ * divided up to alpha turns, in between by ((r - alpha) / (beta - alpha)) of the way. */
+typedef struct prism_hip_rope prism_hip_rope;
+int prism_hip_rope_frequencies(uint32_t dims, double base, double factor, double original, double alpha, double beta,
+                               double *out);
+prism_hip_rope *prism_hip_rope_create(prism_hip_ctx *ctx, uint32_t dims, int interleaved, const double *frequencies,
+                                      double magnitude);
+void prism_hip_rope_destroy(prism_hip_rope *rope);
+/* out[t][h] = the rotation of x[t][h] (head_dim 64, 128 or 256 values of type dtype) by
+ * positions[t]; norm, if not NULL, first takes x to x / sqrt(mean(x^2) + eps) * norm[i]
+ * (binary32 norm[head_dim]).  Computed in binary64, rounded once to binary32 and from
+ * there to the type.  Strides are elements between tokens, at least heads * head_dim;
+ * out may be x with the same stride.  A non-finite x is PRISM_ERR_NONFINITE at sync. */
+int prism_hip_rope_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, int dtype, const void *x, uint64_t x_stride,
+                          const int32_t *positions, uint32_t tokens, uint32_t heads, uint32_t head_dim,
+                          const float *norm, float eps, void *out, uint64_t out_stride, void *stream);
+
+/* Writes tokens of k and v [tokens][kv_heads][head_dim] to the cache's slots.  For every
+ * page and head that receives tokens, M the largest magnitude among them:
+ *   s = max(the page's scale, or 0 where the page's first place is written now; 2^e),
+ *       e the least integer >= -100 with M <= qmax * 2^e (qmax 127 or 448);
+ *   tokens: code(x / s), ties to even; where s grew, the codes of the places before the
+ *   first new one become code(code * old scale / s).  Other places keep their bytes.
+ * Scales the append makes are powers of two, so a page is rescaled by whole bits and
+ * however often it grows loses less than one step of its last scale.
+ * Slots: -1 writes nothing (padding); the new tokens of one page stand together, in
+ * consecutive slots.  A slot outside the cache, or a page's token that does not follow the
+ * one before it, is not written and PRISM_ERR_INVALID_INPUT at sync; the same page in
+ * two places of the batch is the caller's error and leaves that page undefined.  A NaN
+ * is stored as 0, an infinity as the largest code, and either is PRISM_ERR_NONFINITE. */
+int prism_hip_kv_append_device(prism_hip_ctx *ctx, const prism_kv_cache *cache, int dtype, const void *k,
+                               uint64_t k_stride, const void *v, uint64_t v_stride, const int32_t *slots,
+                               uint32_t tokens, void *stream);
+/* The three of a layer in one call: q_out = rotated (and normed) q, the rotated (and
+ * normed) k rounded to the type and v into the cache; what prism_hip_rope_device of q and k
+ * and prism_hip_kv_append_device give, bit for bit.  q_out may be q with the same stride. */
+typedef struct prism_qkv_append {
+    int dtype;
+    uint32_t tokens, heads;
+    const void *q, *k, *v;
+    uint64_t q_stride, k_stride, v_stride;
+    const int32_t *positions, *slots;
+    const float *q_norm, *k_norm; /* NULL: none */
+    float eps;
+    void *q_out;
+    uint64_t q_out_stride;
+} prism_qkv_append;
+int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, const prism_kv_cache *cache,
+                                const prism_qkv_append *step, void *stream);
+
+/* Attention of q [tokens][heads][head_dim] over the cache.  Request r has the tokens
+ * offsets[r] .. offsets[r + 1] - 1 (offsets ascend from 0 to at most `tokens`; rows behind
+ * the last are not written) and the lengths[r] keys and values of its block table row, heads a multiple of
+ * kv_heads (head h reads kv head h / (heads / kv_heads)).
+ *   out = softmax(scale * q k^T) v over the allowed keys; a row without any is 0.
+ * causal: the request's tokens are its last, so token i of n sees the positions up to
+ * lengths[r] - n + i, with window > 0 only the last `window` of them; else (window = 0)
+ * every key, whatever their number: states of another length, an encoder's for instance.
+ * Table columns no row sees are not read.  A page outside the cache among those it does
+ * see is left out, and PRISM_ERR_INVALID_INPUT at sync, as are lengths past max_pages
+ * pages and offsets out of order; a non-finite output is PRISM_ERR_NONFINITE.
+ * max_length sizes the work split and should bound the lengths (any value is correct).
+ * Statistics and sums are binary32; codes are exact in the products' binary16 operands.  For F16 and BF16
+ * the probabilities are rounded to binary16, for F32 q and the probabilities enter in two binary16 parts. */
+typedef struct prism_attention {
+    int dtype;
+    uint32_t requests, tokens, heads, max_pages, max_length;
+    const void *q;
+    uint64_t q_stride;
+    void *out;
+    uint64_t out_stride;
+    const int32_t *offsets, *lengths, *block_table;
+    float scale;
+    int causal;
+    uint32_t window;
+} prism_attention;
+int prism_hip_attention_device(prism_hip_ctx *ctx, const prism_kv_cache *cache, const prism_attention *call,
+                               void *stream);
+
 /* ---- full-attention decode step ---------------------------------------------------
  * A resident decoder over a context: the layer loop of the reference's Qwen35 graph
  * for full-attention layers (src/graph.rs:3870-3995) in the source arithmetic, with

@@ -22,7 +22,7 @@ LIB = os.path.join(HERE, "libprism_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["quantize.hip", "matvec.hip", "mv_tiled.hip", "prefill.hip", "prefill_k.hip", "ffn.hip", "decode.hip", "static_scratch.hip",
-           "runtime.cpp", "decoder.cpp", "gguf.cpp"]
+           "kvcache.hip", "paged_attention.hip", "runtime.cpp", "decoder.cpp", "serving.cpp", "gguf.cpp"]
 
 FLAGS = [
     "--offload-arch=gfx950",

@@ -10,6 +10,8 @@ namespace prism {
 constexpr int kErrNonfinite = 1;   // non-finite output / scale (PRISM_ERR_NONFINITE)
 constexpr int kErrQuantRange = 2;  // activation quantizer overflow (PRISM_ERR_NONFINITE)
 constexpr int kErrInput = 4;       // non-finite activation input (PRISM_ERR_NONFINITE)
+constexpr int kErrIndex = 8;       // slot, page, length or offset out of range (PRISM_ERR_INVALID_INPUT)
+constexpr int kErrPages = 16;      // too few free cache pages (PRISM_ERR_RESOURCE)
 
 // Launcher status: 0 on success, kLaunchUnsupported for a geometry the kernels do not
 // cover, otherwise the hipError_t the launch left (positive).  hipGetLastError clears

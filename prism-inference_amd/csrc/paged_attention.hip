@@ -1,0 +1,546 @@
+// paged_attention.hip -- grouped-query attention over the paged 8-bit cache (gfx950), for
+// single tokens, chunks and prompts of many requests in one call.
+//
+// A request's queries of one kv head form rows (token, head of the group); a wavefront takes
+// 16 * NT of them through blocks of 64 keys with the running maximum and sum of the softmax:
+//   S^T = K Q^T   K codes (exact in binary16) as the A operand, 16 keys a matrix instruction
+//   z = S * (scale * k_scale) + log2 v_scale, p = 2^(z - max z), l = sum p / v_scale
+//   O^T += V^T P^T
+// so a page's two scales cost nothing per key: the keys' joins the softmax scale, the values'
+// the exponent, and p stays within the operand's range however the pages' scales differ.
+//
+// Keys are assigned to the rows of K's matrix instructions so that a lane's 16 scores of a
+// block are 16 consecutive keys, all of one page: they are the B operand of the second product
+// as they stand (no exchange between lanes), and one 16-byte load of the transposed values
+// is the A operand that meets them.  Neither codes nor probabilities pass through LDS.
+#include "serve_common.hpp"
+
+namespace prism {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+// Probabilities enter the second product as 2^14 p: contributions down to 2^-28 of the largest
+// keep binary16's full precision.
+constexpr float kHeadroom = 14.0f;
+constexpr float kNone = -__builtin_inff();
+
+struct AttendArgs {
+    prism_kv_cache c;
+    prism_attention a;
+    uint32_t group, page_log2;
+    uint32_t slots;     // row tiles, at most (tile_request)
+    uint32_t splits;    // key ranges a request's keys are split into, at most
+    float *part;        // [splits][tokens * heads][head_dim] unnormalised rows
+    float *part_ml;     // [splits][tokens * heads][2]: maximum (base 2), sum
+};
+
+// Key blocks of 64 a split takes at least: one for each of a workgroup's wavefronts, and one more round.
+constexpr uint32_t kLeastBlocks = 8;
+
+struct Request {
+    uint32_t first, n;      // its tokens
+    uint32_t length;        // its keys
+    bool bad;
+};
+__device__ __forceinline__ Request request_of(const AttendArgs &p, uint32_t r) {
+    const int32_t o0 = p.a.offsets[r], o1 = p.a.offsets[r + 1];
+    const int32_t len = p.a.lengths[r];
+    const int64_t room = static_cast<int64_t>(p.a.max_pages) << p.page_log2;
+    Request q;
+    q.bad = o0 < 0 || o1 < o0 || static_cast<uint32_t>(o1) > p.a.tokens || len < 0 || len > room;
+    q.first = q.bad ? 0 : o0;
+    q.n = q.bad ? 0 : o1 - o0;
+    q.length = q.bad ? 0 : len;
+    return q;
+}
+// Keys [lo, hi) that token i of the request sees.
+__device__ __forceinline__ void visible(const AttendArgs &p, const Request &q, uint32_t i, int32_t *lo, int32_t *hi) {
+    *lo = 0;
+    *hi = static_cast<int32_t>(q.length);
+    if (!p.a.causal) return;
+    const int32_t at = static_cast<int32_t>(q.length) - static_cast<int32_t>(q.n) + static_cast<int32_t>(i);
+    *hi = at + 1 > 0 ? at + 1 : 0;
+    if (p.a.window && at + 1 > static_cast<int64_t>(p.a.window)) *lo = at + 1 - static_cast<int32_t>(p.a.window);
+}
+// The 64-key blocks [b0, b1) any of the request's tokens i0 .. i1 sees, and how many of them a
+// split takes: the same for every tile of the request, so that the join knows the splits in use.
+__device__ __forceinline__ void blocks_of(const AttendArgs &p, const Request &q, uint32_t i0, uint32_t i1, uint32_t *b0,
+                                          uint32_t *b1) {
+    int32_t lo, hi, x;
+    visible(p, q, i0, &lo, &x);
+    visible(p, q, i1, &x, &hi);
+    *b0 = static_cast<uint32_t>(lo) / 64;
+    *b1 = hi > lo ? (static_cast<uint32_t>(hi) + 63) / 64 : *b0;
+}
+__device__ __forceinline__ uint32_t split_blocks(const AttendArgs &p, uint32_t blocks) {
+    const uint32_t each = (blocks + p.splits - 1) / p.splits;
+    return each < kLeastBlocks ? kLeastBlocks : each;
+}
+
+// Tiles of M rows: request r has the slots from offsets[r] * group / M + r on, at least as
+// many as it needs and in ascending order, so no sums over the requests are needed first.
+__device__ __forceinline__ uint32_t tile_start(const AttendArgs &p, uint32_t r, uint32_t M) {
+    const int32_t o = p.a.offsets[r];
+    const uint64_t tokens = o < 0 ? 0 : static_cast<uint32_t>(o) > p.a.tokens ? p.a.tokens : static_cast<uint32_t>(o);
+    return static_cast<uint32_t>(tokens * p.group / M) + r;
+}
+__device__ __forceinline__ uint32_t tile_request(const AttendArgs &p, uint32_t slot, uint32_t M) {
+    // The last r with tile_start(r) <= slot, 64 candidates at a time.
+    uint32_t lo = 0, n = p.a.requests;
+    const uint32_t lane = threadIdx.x & 63;
+    while (n > 1) {
+        const uint32_t step = (n + 63) / 64, k = lane * step;
+        const bool at = k < n && tile_start(p, lo + k, M) <= slot;
+        const uint64_t on = __ballot(at);
+        const uint32_t j = on ? 63 - __builtin_clzll(on) : 0;
+        n = min(step, n - j * step);
+        lo += j * step;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Eight codes of two dwords as binary16.
+template <int FMT>
+__device__ __forceinline__ f16x8 halves(uint32_t a, uint32_t b) {
+    union {
+        uint32_t u[4];
+        f16x2 h[4];
+        f16x8 v;
+    } r;
+    if constexpr (FMT == kInt8) {
+        // 0x6400 | (code + 128) is 1024 + code + 128.
+        a ^= 0x80808080u;
+        b ^= 0x80808080u;
+        r.u[0] = perm(0x64646464u, a, 0x04010400u);
+        r.u[1] = perm(0x64646464u, a, 0x04030402u);
+        r.u[2] = perm(0x64646464u, b, 0x04010400u);
+        r.u[3] = perm(0x64646464u, b, 0x04030402u);
+        const f16x2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.h[i] += off;
+    } else {
+        r.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(a), 1.0f, false);
+        r.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(a), 1.0f, true);
+        r.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(b), 1.0f, false);
+        r.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(b), 1.0f, true);
+    }
+    return r.v;
+}
+
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ float across_max(float v) {  // over the four lanes of a row
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float across_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+template <typename T>
+__device__ __forceinline__ void write_row(const AttendArgs &p, uint32_t token, uint32_t head, uint32_t dim, f32x4 v, bool *bad) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *bad |= !finite(v[i]);
+    store4(static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * p.c.head_dim + dim, v);
+}
+
+// T: type of q and out.  LIMBS: binary16 parts of q and of the probabilities (2 for binary32).
+// SHARED: the workgroup's four wavefronts share 16 * NT rows and split the keys (few rows);
+// otherwise each has 16 * NT rows of its own.
+template <typename T, int D, int FMT, int NT, bool SHARED>
+__global__ __launch_bounds__(256) void k_attend(AttendArgs p, int *err) {
+    constexpr int LIMBS = sizeof(T) == 4 ? 2 : 1;
+    constexpr int KS = D / 32, DT = D / 16;
+    constexpr uint32_t M = SHARED ? 16 * NT : 64 * NT;  // rows of a workgroup
+    __shared__ float join_ml[SHARED ? 4 : 1][SHARED ? 16 * NT : 1][2];
+    __shared__ f32x4 join_acc[SHARED ? 3 : 1][SHARED ? NT * DT : 1][SHARED ? 64 : 1];
+
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t n = lane & 15, g = lane / 16;
+    // Heavy tiles first: a prompt's last rows see the most keys.
+    const uint32_t slot = gridDim.x - 1 - blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
+    const uint32_t r = tile_request(p, slot, M);
+    const Request q = request_of(p, r);
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0)  // offsets out of order may leave a request without a tile
+        for (uint32_t i = threadIdx.x; i < p.a.requests; i += 256)
+            if (request_of(p, i).bad) raise_error(err, kErrIndex);
+    const uint32_t rows = q.n * p.group, start = tile_start(p, r, M), row0 = (slot - start) * M;
+    if (slot < start || row0 >= rows) return;
+    const uint32_t last = min(rows, row0 + M) - 1;
+    if (!SHARED && row0 + wave * 16 * NT >= rows) return;
+
+    // The tile's key blocks, this split's part of them, and this wavefront's.
+    uint32_t b0, b1;
+    blocks_of(p, q, row0 / p.group, last / p.group, &b0, &b1);
+    const uint32_t each = split_blocks(p, b1 - b0);
+    const uint32_t parts = b1 > b0 ? (b1 - b0 + each - 1) / each : 1;
+    if (split >= parts) return;
+    b0 += split * each;
+    b1 = min(b1, b0 + each);
+
+    const uint32_t base_row = SHARED ? row0 : row0 + wave * 16 * NT;
+    uint32_t token[NT], head[NT];  // of this lane's rows
+    bool live[NT];
+    int32_t lo[NT], hi[NT];
+    float kf[NT];
+    f16x8 qv[LIMBS][NT][KS];
+    int32_t all_lo = 0, all_hi = 0x7fffffff;  // keys every row of the wavefront sees
+    int32_t any_lo = 0x7fffffff, any_hi = 0;  // keys any row sees
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const uint32_t row = base_row + 16 * t + n;
+        live[t] = row < rows;
+        const uint32_t rr = live[t] ? row : last, i = rr / p.group;
+        token[t] = q.first + i;
+        head[t] = kvh * p.group + rr % p.group;
+        visible(p, q, i, &lo[t], &hi[t]);
+        all_lo = max(all_lo, lo[t]);
+        all_hi = min(all_hi, hi[t]);
+        any_lo = min(any_lo, lo[t]);
+        any_hi = max(any_hi, hi[t]);
+        // Lane group g has the dimensions [g D/4, (g + 1) D/4) of the row.
+        const T *src = static_cast<const T *>(p.a.q) + token[t] * p.a.q_stride + static_cast<uint64_t>(head[t]) * D + g * (D / 4);
+        f32x4 x[D / 16];
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+            x[j] = load4(src + 4 * j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(x[j][k]));
+        }
+        most = across_max(most);
+        // A power of two takes the row's largest value to [2^13, 2^14).
+        int e = static_cast<int>(__float_as_uint(most) >> 23 & 255) - 127;
+        e = !finite(most) || e < -100 ? 0 : e;
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+        kf[t] = p.a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = x[2 * s + j / 4][j % 4] * up;
+                const _Float16 h = static_cast<_Float16>(v);
+                qv[0][t][s][j] = h;
+                if constexpr (LIMBS == 2) qv[LIMBS - 1][t][s][j] = static_cast<_Float16>(v - static_cast<float>(h));
+            }
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+        all_lo = max(all_lo, __shfl_xor(all_lo, d));
+        all_hi = min(all_hi, __shfl_xor(all_hi, d));
+        any_lo = min(any_lo, __shfl_xor(any_lo, d));
+        any_hi = max(any_hi, __shfl_xor(any_hi, d));
+    }
+
+    float m[NT], l[NT];
+    f32x4 acc[NT][DT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = kNone;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0, 0, 0, 0};
+    }
+
+    const uint32_t page_mask = p.c.page_size - 1;
+    const int32_t *table = p.a.block_table + static_cast<uint64_t>(r) * p.a.max_pages;
+    const uint8_t *kc = static_cast<const uint8_t *>(p.c.k), *vc = static_cast<const uint8_t *>(p.c.v);
+    const uint32_t kgroup = (lane >> 2) & 3;  // 16-key group whose keys this lane loads for the first product
+    bool missing = false;
+
+    for (uint32_t b = SHARED ? b0 + wave : b0; b < b1; b += SHARED ? 4 : 1) {
+        const int32_t base = static_cast<int32_t>(64 * b);
+        if (base >= any_hi || base + 64 <= any_lo) continue;
+        // The pages of the two 16-key groups this lane reads; a group without a page, or behind the
+        // keys, reads page 0 and counts as masked.
+        const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
+        int32_t page_k = 0, page_v = 0;
+        bool there = false;
+        if (key_k < any_hi) {
+            const int32_t id = table[key_k >> p.page_log2];
+            page_k = id >= 0 && static_cast<uint32_t>(id) < p.c.pages ? id : 0;
+        }
+        if (key_v < any_hi) {
+            const int32_t id = table[key_v >> p.page_log2];
+            there = id >= 0 && static_cast<uint32_t>(id) < p.c.pages;
+            page_v = there ? id : 0;
+            missing |= !there && key_v + 16 > any_lo;
+        }
+        const uint64_t unit_k = static_cast<uint64_t>(page_k) * p.c.kv_heads + kvh;
+        const uint64_t unit_v = static_cast<uint64_t>(page_v) * p.c.kv_heads + kvh;
+        const float ks = there ? p.c.k_scale[unit_v] : 0.0f;
+        float vs = there ? p.c.v_scale[unit_v] : 1.0f;
+        if (vs < 0x1p-100f) vs = 0x1p-100f;  // log2 and 1 / vs stay finite; NaN stays NaN
+
+        u32x4 kraw[4][D / 64], vraw[DT];
+        const uint8_t *kp = kc + ((unit_k << p.page_log2) + (static_cast<uint32_t>(key_k) & page_mask) + (lane & 3)) * D + g * (D / 4);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) kraw[t][j] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * D + 16 * j);
+        const uint8_t *vp = vc + ((unit_v * D + n) << p.page_log2) + (static_cast<uint32_t>(key_v) & page_mask);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vraw[d] = *reinterpret_cast<const u32x4 *>(vp + (static_cast<uint64_t>(16 * d) << p.page_log2));
+
+        const bool edge = base < all_lo || base + 64 > all_hi || __ballot(there) != ~0ull;
+        if (edge && FMT == kE4m3) {
+            // Bytes behind the keys may hold NaN codes, which zero probabilities do not silence.
+            const int32_t keep = there ? any_hi - key_v : 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int32_t left = keep - 4 * w;
+                const uint32_t mask = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) vraw[d][w] &= mask;
+            }
+        }
+
+        f16x8 pv[LIMBS][NT][2];
+        {
+            f32x4 s[NT][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int u = 0; u < NT; ++u) s[u][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    const f16x8 kv = halves<FMT>(kraw[t][k / 2][2 * (k % 2)], kraw[t][k / 2][2 * (k % 2) + 1]);
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) {
+                        s[u][t] = mfma(kv, qv[0][u][k], s[u][t]);
+                        if constexpr (LIMBS == 2) s[u][t] = mfma(kv, qv[LIMBS - 1][u][k], s[u][t]);
+                    }
+                }
+            }
+            const float lv = __builtin_amdgcn_logf(vs), iv = 1.0f / vs;
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const float f = kf[u] * ks;
+                float top = kNone;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float z = __builtin_fmaf(s[u][t][i], f, lv);
+                        if (edge) {
+                            const int32_t key = key_v + 4 * t + i;
+                            z = there && key >= lo[u] && key < hi[u] ? z : kNone;
+                        }
+                        s[u][t][i] = z;
+                        top = fmaxf(top, z);
+                    }
+                const float next = fmaxf(m[u], across_max(top));
+                const float ref = next == kNone ? 0.0f : next;  // a row that has seen no key yet
+                const float alpha = __builtin_amdgcn_exp2f(m[u] - ref);
+                m[u] = next;
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(s[u][t][i] - (ref - kHeadroom));
+                        sum += e;
+                        const _Float16 h = static_cast<_Float16>(e);
+                        pv[0][u][t / 2][4 * (t % 2) + i] = h;
+                        if constexpr (LIMBS == 2) pv[LIMBS - 1][u][t / 2][4 * (t % 2) + i] = static_cast<_Float16>(e - static_cast<float>(h));
+                    }
+                l[u] = __builtin_fmaf(l[u], alpha, sum == 0.0f ? 0.0f : sum * iv);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[u][d] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const f16x8 vv = halves<FMT>(vraw[d][2 * c], vraw[d][2 * c + 1]);
+#pragma unroll
+                for (int u = 0; u < NT; ++u) {
+                    acc[u][d] = mfma(vv, pv[0][u][c], acc[u][d]);
+                    if constexpr (LIMBS == 2) acc[u][d] = mfma(vv, pv[LIMBS - 1][u][c], acc[u][d]);
+                }
+            }
+    }
+    if (missing) raise_error(err, kErrIndex);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) l[t] = across_sum(l[t]);
+
+    if constexpr (SHARED) {
+        // The four wavefronts' rows join in the first.
+        if (g == 0)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                join_ml[wave][16 * t + n][0] = m[t];
+                join_ml[wave][16 * t + n][1] = l[t];
+            }
+        if (wave)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) join_acc[wave - 1][t * DT + d][lane] = acc[t][d];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float top = m[t];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) top = fmaxf(top, join_ml[w][16 * t + n][0]);
+            const float ref = top == kNone ? 0.0f : top;
+            const float mine = __builtin_amdgcn_exp2f(m[t] - ref);
+            l[t] *= mine;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[t][d] *= mine;
+#pragma unroll
+            for (int w = 1; w < 4; ++w) {
+                const float other = __builtin_amdgcn_exp2f(join_ml[w][16 * t + n][0] - ref);
+                l[t] += other * join_ml[w][16 * t + n][1];
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const f32x4 v = join_acc[w - 1][t * DT + d][lane];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t][d][i] = __builtin_fmaf(v[i], other, acc[t][d][i]);
+                }
+            }
+            m[t] = top;
+        }
+    }
+
+    // Lane (n, g) has dimensions 16 d + 4 g .. + 3 of row n.
+    bool bad = false;
+    const uint64_t all_rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        if (!live[t]) continue;
+        if (parts == 1) {
+            const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) write_row<T>(p, token[t], head[t], 16 * d + 4 * g, acc[t][d] * inv, &bad);
+        } else {
+            const uint64_t row = split * all_rows + static_cast<uint64_t>(token[t]) * p.a.heads + head[t];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + row * D + 16 * d + 4 * g) = acc[t][d];
+            if (g == 0) {
+                p.part_ml[2 * row] = m[t];
+                p.part_ml[2 * row + 1] = l[t];
+            }
+        }
+    }
+    if (bad) raise_error(err, kErrNonfinite);
+}
+
+// Joins the splits of the rows that have more than one: a wavefront a row, a lane D / 64 dimensions.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, int *err) {
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + threadIdx.x / 64, all_rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
+    const uint32_t lane = threadIdx.x & 63;
+    if (row >= all_rows) return;
+    const uint32_t token = static_cast<uint32_t>(row / p.a.heads), head = static_cast<uint32_t>(row % p.a.heads);
+    // The request of the token, 64 candidates at a time.
+    uint32_t lo = 0, n = p.a.requests;
+    while (n > 1) {
+        const uint32_t step = (n + 63) / 64, k = lane * step;
+        const uint64_t on = __ballot(k < n && p.a.offsets[lo + k] <= static_cast<int32_t>(token));
+        const uint32_t j = on ? 63 - __builtin_clzll(on) : 0;
+        n = min(step, n - j * step);
+        lo += j * step;
+    }
+    const uint32_t r = __builtin_amdgcn_readfirstlane(lo);
+    const Request q = request_of(p, r);
+    if (token < q.first || token >= q.first + q.n) return;
+    const uint32_t rows = q.n * p.group, row0 = ((token - q.first) * p.group + head % p.group) / M * M, last = min(rows, row0 + M) - 1;
+    uint32_t b0, b1;
+    blocks_of(p, q, row0 / p.group, last / p.group, &b0, &b1);
+    const uint32_t each = split_blocks(p, b1 - b0), parts = (b1 - b0 + each - 1) / each;
+    if (parts <= 1) return;
+    float top = kNone;
+    for (uint32_t s = 0; s < parts; ++s) top = fmaxf(top, p.part_ml[2 * (s * all_rows + row)]);
+    const float ref = top == kNone ? 0.0f : top;
+    float l = 0.0f, acc[D / 64] = {};
+    for (uint32_t s = 0; s < parts; ++s) {
+        const uint64_t at = s * all_rows + row;
+        const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - ref);
+        l = __builtin_fmaf(p.part_ml[2 * at + 1], f, l);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) acc[i] = __builtin_fmaf(p.part[at * D + lane + 64 * i], f, acc[i]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bool bad = false;
+    T *out = static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * D;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        const float v = acc[i] * inv;
+        bad |= !finite(v);
+        out[lane + 64 * i] = static_cast<T>(v);
+    }
+    if (bad) raise_error(err, kErrNonfinite);
+}
+
+// How a call runs: rows a workgroup takes, whether its wavefronts share them, and the most splits.
+struct Plan {
+    uint32_t nt, M, slots, splits;
+    bool shared;
+};
+Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus) {
+    const uint32_t group = a.heads / c.kv_heads;
+    const uint64_t typical = (static_cast<uint64_t>(a.tokens) * group + a.requests - 1) / a.requests;  // rows of a request
+    Plan p;
+    p.shared = typical <= 32;
+    p.nt = c.head_dim == 256 || (p.shared && typical <= 16) ? 1 : 2;
+    p.M = p.shared ? 16 * p.nt : 64 * p.nt;
+    p.slots = static_cast<uint32_t>(static_cast<uint64_t>(a.tokens) * group / p.M) + a.requests;
+    // Keys are split until some 1024 workgroups share them.
+    const uint64_t tiles = static_cast<uint64_t>(p.slots) * c.kv_heads, want = 4ull * cus;
+    const uint32_t most = (a.max_length / 64 + kLeastBlocks) / kLeastBlocks;
+    uint64_t splits = tiles >= want ? 1 : want / tiles;
+    if (splits > most) splits = most;
+    p.splits = splits < 1 ? 1 : static_cast<uint32_t>(splits);
+    return p;
+}
+
+template <typename T, int D, int FMT>
+int attend_launch(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s) {
+    const dim3 grid(p.slots, p.c.kv_heads, p.splits);
+    constexpr int most = D == 256 ? 1 : 2;
+    if (!plan.shared) k_attend<T, D, FMT, most, false><<<grid, 256, 0, s>>>(p, err);
+    else if (plan.nt == 1) k_attend<T, D, FMT, 1, true><<<grid, 256, 0, s>>>(p, err);
+    else k_attend<T, D, FMT, most, true><<<grid, 256, 0, s>>>(p, err);
+    int rc = launch_status();
+    if (rc || p.splits == 1) return rc;
+    const uint64_t rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
+    k_attend_join<T, D><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, s>>>(p, plan.M, err);
+    return launch_status();
+}
+template <typename T, int D>
+int attend_format(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s) {
+    return p.c.format == PRISM_CACHE_INT8 ? attend_launch<T, D, kInt8>(p, plan, err, s) : attend_launch<T, D, kE4m3>(p, plan, err, s);
+}
+template <typename T>
+int attend_headed(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s) {
+    switch (p.c.head_dim) {
+    case 64: return attend_format<T, 64>(p, plan, err, s);
+    case 128: return attend_format<T, 128>(p, plan, err, s);
+    case 256: return attend_format<T, 256>(p, plan, err, s);
+    default: return kLaunchUnsupported;
+    }
+}
+
+}  // namespace
+
+size_t attention_scratch_bytes(const prism_kv_cache &c, const prism_attention &a, uint32_t cus) {
+    const Plan p = attend_plan(c, a, cus);
+    return p.splits == 1 ? 0 : sizeof(float) * p.splits * (static_cast<size_t>(a.tokens) * a.heads) * (c.head_dim + 2);
+}
+
+int launch_attention_paged(const prism_kv_cache &c, const prism_attention &a, void *scratch, uint32_t cus, int *err, hipStream_t s) {
+    const Plan plan = attend_plan(c, a, cus);
+    AttendArgs p{c, a, a.heads / c.kv_heads, 0, plan.slots, plan.splits, static_cast<float *>(scratch), nullptr};
+    p.page_log2 = static_cast<uint32_t>(__builtin_ctz(c.page_size));
+    p.part_ml = p.part + static_cast<size_t>(plan.splits) * a.tokens * a.heads * c.head_dim;
+    if (a.dtype == PRISM_DTYPE_F32) return attend_headed<float>(p, plan, err, s);
+    if (a.dtype == PRISM_DTYPE_F16) return attend_headed<_Float16>(p, plan, err, s);
+    return attend_headed<__bf16>(p, plan, err, s);
+}
+
+}  // namespace prism

@@ -85,6 +85,7 @@ struct prism_hip_ctx {
     int64_t next_id = 1;
     int *err = nullptr;  // device error flag
     prism::rt::DevBuf x, act, act2, out, gate, up, h, hr, res, pre, sk, lora;
+    prism::rt::DevBuf plan, rope, att;  // serving.cpp
     // Whether the current device call took one of them, whether a captured one ever did (a graph
     // may hold any of them from then on), and those outgrown since, kept for such graphs.
     bool scratch_used = false, scratch_captured = false;
@@ -418,6 +419,8 @@ inline int drain(prism_hip_ctx *c, hipStream_t s) {
     if (flag) {
         if (const int e = launch_fill_i32(c->err, 0, 1, s)) return launch_result(c, e, "reset error flag");
         HIP_OR_FAIL(c, hipStreamSynchronize(s));
+        if (flag & kErrIndex) return fail(c, PRISM_ERR_INVALID_INPUT, "cache slot, page, length or offset out of range");
+        if (flag & kErrPages) return fail(c, PRISM_ERR_RESOURCE, "too few free cache pages");
         if (flag & kErrInput) return fail(c, PRISM_ERR_NONFINITE, "non-finite activation input");
         if (flag & kErrQuantRange) return fail(c, PRISM_ERR_NONFINITE, "activation quantization scale overflow");
         return fail(c, PRISM_ERR_NONFINITE, "non-finite value in projection output");

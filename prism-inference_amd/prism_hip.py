@@ -43,6 +43,13 @@ Q8_SOURCE = 0
 Q8_PINNED = 1
 Q8_PINNED_NATIVE = 2
 
+DTYPE_F32 = 0
+DTYPE_F16 = 1
+DTYPE_BF16 = 2
+
+CACHE_INT8 = 0
+CACHE_E4M3 = 1
+
 Q8K_DTYPE = np.dtype([("scale", "<f4"), ("values", "i1", (256,)), ("sums", "<i2", (16,))])
 Q8_DTYPE = np.dtype([("scale", "<f4"), ("sum", "<f4"), ("values", "i1", (32,))])
 
@@ -73,6 +80,7 @@ def lib() -> ctypes.CDLL:
         raise RuntimeError(f"{LIB_PATH} is missing: build it with prism-inference_amd/build.py")
     L = ctypes.CDLL(LIB_PATH)
     P, U64, U32, I, I64 = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int, ctypes.c_int64
+    F, D = ctypes.c_float, ctypes.c_double
     sig = {
         "prism_hip_create": (P, [I, U64, U32]),
         "prism_hip_destroy": (None, [P]),
@@ -121,6 +129,14 @@ def lib() -> ctypes.CDLL:
         "prism_hip_ffn_chain_device": (I, [P, I64, I64, I64, P, P, U32, I, P, P, P]),
         "prism_hip_sync": (I, [P, P]),
         "prism_hip_stream": (P, [P]),
+        "prism_hip_kv_plan_device": (I, [P, P, P]),
+        "prism_hip_rope_frequencies": (I, [U32, D, D, D, D, D, P]),
+        "prism_hip_rope_create": (P, [P, U32, I, P, D]),
+        "prism_hip_rope_destroy": (None, [P]),
+        "prism_hip_rope_device": (I, [P, P, I, P, U64, P, U32, U32, U32, P, F, P, U64, P]),
+        "prism_hip_kv_append_device": (I, [P, P, I, P, U64, P, U64, P, U32, P]),
+        "prism_hip_qkv_append_device": (I, [P, P, P, P, P]),
+        "prism_hip_attention_device": (I, [P, P, P, P]),
         "prism_hip_decoder_create": (P, [P, P, U32]),
         "prism_hip_decoder_destroy": (None, [P]),
         "prism_hip_decoder_set_layer": (I, [P, U32, P, P, P, P, P, P, P, P, P]),
@@ -317,6 +333,69 @@ def _ptr(a):
         return ctypes.c_void_p(a.data_ptr())
     assert a.flags["C_CONTIGUOUS"], "arrays must be C contiguous"
     return a.ctypes.data_as(ctypes.c_void_p)
+
+
+def _address(a) -> int:
+    """Address of a device array: a torch tensor of any strides, a buffer of hiprt, or an integer."""
+    return a if isinstance(a, int) else a.data_ptr()
+
+
+class _Described(ctypes.Structure):
+    """A struct of the C ABI built by keyword: device arrays (torch tensors or buffers) give their
+    addresses and are kept alive, everything else its value."""
+
+    def __init__(self, **fields):
+        super().__init__()
+        names = [n for n, _ in self._fields_]
+        missing = sorted(set(names) - set(fields)), sorted(set(fields) - set(names))
+        if missing[0] or missing[1]:
+            raise TypeError(f"{type(self).__name__}: missing {missing[0]}, unknown {missing[1]}")
+        self._kept = []
+        for name, kind in self._fields_:
+            value = fields[name]
+            if kind is ctypes.c_void_p and value is not None:
+                self._kept.append(value)
+                value = _address(value)
+            setattr(self, name, value)
+
+
+class KvCache(_Described):
+    """prism_kv_cache: one layer's paged 8-bit cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, ctypes.c_uint32) for n in ("format", "pages", "page_size", "kv_heads", "head_dim")]
+
+
+class KvPlan(_Described):
+    """prism_kv_plan: one step's lengths in, its pages, positions and slots out."""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("requests", "max_pages", "max_tokens", "page_size", "free_capacity")] + [
+        (n, ctypes.c_void_p) for n in ("lengths", "added", "block_table", "free_pages", "free_count", "new_lengths", "offsets",
+                                       "positions", "slots", "owners", "counts")]
+
+
+class QkvAppend(_Described):
+    """prism_qkv_append: one layer's q, k and v of a step."""
+    _fields_ = [("dtype", ctypes.c_int), ("tokens", ctypes.c_uint32), ("heads", ctypes.c_uint32)] + [
+        (n, ctypes.c_void_p) for n in ("q", "k", "v")] + [(n, ctypes.c_uint64) for n in ("q_stride", "k_stride", "v_stride")] + [
+        (n, ctypes.c_void_p) for n in ("positions", "slots", "q_norm", "k_norm")] + [
+        ("eps", ctypes.c_float), ("q_out", ctypes.c_void_p), ("q_out_stride", ctypes.c_uint64)]
+
+
+class Attention(_Described):
+    """prism_attention: the queries of a step's requests over the cache."""
+    _fields_ = [("dtype", ctypes.c_int)] + [(n, ctypes.c_uint32) for n in ("requests", "tokens", "heads", "max_pages", "max_length")] + [
+        ("q", ctypes.c_void_p), ("q_stride", ctypes.c_uint64), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_uint64)] + [
+        (n, ctypes.c_void_p) for n in ("offsets", "lengths", "block_table")] + [
+        ("scale", ctypes.c_float), ("causal", ctypes.c_int), ("window", ctypes.c_uint32)]
+
+
+def rope_frequencies(dims: int, base: float, factor: float = 1.0, original: float = 0.0, alpha: float = 1.0,
+                     beta: float = 32.0) -> np.ndarray:
+    """Radians a position of dims / 2 pairs, scaled for long contexts (prism_hip_rope_frequencies)."""
+    out = np.zeros(max(dims, 0) // 2, np.float64)
+    rc = lib().prism_hip_rope_frequencies(dims, base, factor, original, alpha, beta, _ptr(out))
+    if rc:
+        raise PrismError(rc, "bad rotary frequencies")
+    return out
 
 
 class Context:
@@ -597,8 +676,57 @@ class Context:
         self._check(lib().prism_hip_ffn_chain_device(self._h, g, u, d, _ptr(x), _ptr(residual), hadamard_block,
                                                      int(pinned), _ptr(out), _ptr(h), stream))
 
+    # -- serving many requests (torch tensors; strides in elements) --
+    def kv_plan_device(self, plan: KvPlan, stream=None):
+        self._check(lib().prism_hip_kv_plan_device(self._h, ctypes.byref(plan), stream))
+
+    def rope_device(self, rope: "Rope", dtype: int, x, x_stride: int, positions, tokens: int, heads: int, head_dim: int, out,
+                    out_stride: int, norm=None, eps: float = 0.0, stream=None):
+        self._check(lib().prism_hip_rope_device(self._h, rope.handle, dtype, _ptr(x), x_stride, _ptr(positions), tokens, heads,
+                                                head_dim, _ptr(norm), eps, _ptr(out), out_stride, stream))
+
+    def kv_append_device(self, cache: KvCache, dtype: int, k, k_stride: int, v, v_stride: int, slots, tokens: int, stream=None):
+        self._check(lib().prism_hip_kv_append_device(self._h, ctypes.byref(cache), dtype, _ptr(k), k_stride, _ptr(v), v_stride,
+                                                     _ptr(slots), tokens, stream))
+
+    def qkv_append_device(self, rope: "Rope", cache: KvCache, step: QkvAppend, stream=None):
+        self._check(lib().prism_hip_qkv_append_device(self._h, rope.handle, ctypes.byref(cache), ctypes.byref(step), stream))
+
+    def attention_device(self, cache: KvCache, call: Attention, stream=None):
+        self._check(lib().prism_hip_attention_device(self._h, ctypes.byref(cache), ctypes.byref(call), stream))
+
     def sync(self, stream=None) -> int:
         return lib().prism_hip_sync(self._h, stream)
+
+
+class Rope:
+    """Rotary positions of `dims` dimensions (prism_hip_rope_*); frequencies as rope_frequencies gives them."""
+
+    def __init__(self, ctx: Context, dims: int, frequencies, interleaved: bool = False, magnitude: float = 1.0):
+        self._h = None
+        self.ctx = ctx
+        f = np.ascontiguousarray(frequencies, np.float64)
+        if f.shape != (dims // 2,):
+            raise ValueError("a rotation of `dims` dimensions has dims / 2 frequencies")
+        self._h = lib().prism_hip_rope_create(ctx.handle, dims, int(interleaved), _ptr(f), magnitude)
+        if not self._h:
+            raise PrismError(ERR_DEVICE_FAULT if ctx.faulted else ERR_INVALID_INPUT, ctx.last_error)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def close(self):
+        # A context that went first has ended the process's use of its rotations.
+        if self._h and self.ctx.handle:
+            lib().prism_hip_rope_destroy(self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class DecoderLaunchTime(ctypes.Structure):
