@@ -8,20 +8,21 @@ namespace {
 
 // ---- plan -------------------------------------------------------------------------------
 // Exclusive sums over the requests of their new tokens, of the pages they need and of those
-// they give back; everything else follows from these per token.  One workgroup makes the
-// sums (a few thousand requests are a few loads a thread); the tokens are filled by the same
-// workgroup, or by a grid where they are many.
+// they give back; every token's position, page and slot follows from these by itself.  One
+// workgroup makes the sums (a few thousand requests are a few loads a thread).  Few requests stay in
+// its LDS and it fills their tokens too; else a grid does, whose wavefronts look the request of
+// their first token up 64 offsets at a time and the others' in the 64 offsets behind it.
 
 constexpr uint32_t kPlanThreads = 1024;
-constexpr uint32_t kPlanOwnFill = 4096;  // tokens the summing workgroup fills by itself
+constexpr uint32_t kPlanOwnTokens = 4096, kPlanOwnRequests = 1024;
 
 struct PlanScratch {
     int32_t *need_base, *back_base;  // [requests + 1]
-    int32_t *head;                   // {tokens, stack height before pages are taken, refused}
+    int32_t *head;                   // {tokens, free pages, pages given back}
 };
 PlanScratch plan_scratch(void *p, uint32_t requests) {
     int32_t *i = static_cast<int32_t *>(p);
-    return PlanScratch{i, i + requests + 1, i + 2 * (requests + 1)};
+    return PlanScratch{i, i + requests + 1, i + 2 * (static_cast<size_t>(requests) + 1)};
 }
 
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, uint32_t page) { return (tokens + page - 1) / page; }
@@ -36,32 +37,56 @@ __device__ __forceinline__ uint32_t last_at_most(const int32_t *base, uint32_t n
     }
     return lo;
 }
-
-__device__ __forceinline__ void plan_fill(const prism_kv_plan &p, const PlanScratch &sc, uint32_t t, int32_t tokens,
-                                          int32_t height) {
-    int32_t position = 0, slot = -1, owner = -1;
-    if (static_cast<int32_t>(t) < tokens) {
-        // Requests without new tokens share their offset with the next: the last of equals has it.
-        const uint32_t r = last_at_most(p.offsets, p.requests, static_cast<int32_t>(t));
-        const int32_t old = p.new_lengths[r] - p.added[r];
-        const int32_t page = static_cast<int32_t>(p.page_size);
-        position = old + static_cast<int32_t>(t) - p.offsets[r];
-        owner = static_cast<int32_t>(r);
-        const int32_t held = static_cast<int32_t>(pages_of(old, p.page_size)), j = position / page, place = position % page;
-        int32_t *entry = p.block_table + static_cast<uint64_t>(r) * p.max_pages + j;
-        int32_t id;
-        if (j < held) {
-            id = *entry;
-        } else {
-            id = p.free_pages[height - 1 - (sc.need_base[r] + j - held)];
-            if (place == 0) *entry = id;  // a new page begins with a new token
-        }
-        const int64_t s = static_cast<int64_t>(id) * page + place;
-        slot = id >= 0 && s <= 0x7fffffff ? static_cast<int32_t>(s) : -1;
+// The same for a wavefront whose lanes have ascending x.
+__device__ __forceinline__ uint32_t last_at_most_wave(const int32_t *base, uint32_t n, int32_t x) {
+    const uint32_t lane = threadIdx.x & 63;
+    const int32_t x0 = __shfl(x, 0);
+    uint32_t lo = 0, left = n;
+    while (left > 1) {
+        const uint32_t step = (left + 63) / 64, k = lane * step;
+        const uint64_t on = __ballot(k < left && base[lo + k] <= x0);
+        const uint32_t j = on ? 63 - __builtin_clzll(on) : 0;
+        left = min(step, left - j * step);
+        lo += j * step;
     }
+    const int32_t next = lo + 1 + lane < n ? base[lo + 1 + lane] : 0x7fffffff;
+    uint32_t c = 0;  // of the 64 entries behind lo, those at most x
+#pragma unroll
+    for (uint32_t d = 32; d; d /= 2)
+        if (__shfl(next, c + d - 1) <= x) c += d;
+    if (c == 63 && __shfl(next, 63) <= x) c = 64;
+    return c < 64 ? lo + c : lo + 64 + last_at_most(base + lo + 64, n - lo - 64, x);
+}
+
+// Pages given back, on top of the stack: the b-th of them.
+__device__ __forceinline__ int32_t page_given_back(const prism_kv_plan &p, const int32_t *back_base, int32_t b) {
+    const uint32_t r = last_at_most(back_base, p.requests, b);
+    return p.block_table[static_cast<uint64_t>(r) * p.max_pages + (b - back_base[r])];
+}
+
+__device__ __forceinline__ void plan_token(const prism_kv_plan &p, const int32_t *back_base, uint32_t t, uint32_t r, int32_t old,
+                                           int32_t offset, int32_t need_base, int32_t count, int32_t back) {
+    const int32_t page = static_cast<int32_t>(p.page_size);
+    const int32_t position = old + static_cast<int32_t>(t) - offset;
+    const int32_t held = static_cast<int32_t>(pages_of(old, p.page_size)), j = position / page, place = position % page;
+    int32_t *entry = p.block_table + static_cast<uint64_t>(r) * p.max_pages + j;
+    int32_t id;
+    if (j < held) {
+        id = *entry;
+    } else {
+        const int32_t k = count + back - 1 - (need_base + j - held);
+        id = k < count ? p.free_pages[k] : page_given_back(p, back_base, k - count);
+        if (place == 0) *entry = id;  // a new page begins with a new token
+    }
+    const int64_t s = static_cast<int64_t>(id) * page + place;
     p.positions[t] = position;
-    p.slots[t] = slot;
-    p.owners[t] = owner;
+    p.slots[t] = id >= 0 && s <= 0x7fffffff ? static_cast<int32_t>(s) : -1;
+    p.owners[t] = static_cast<int32_t>(r);
+}
+__device__ __forceinline__ void plan_no_token(const prism_kv_plan &p, uint32_t t) {
+    p.positions[t] = 0;
+    p.slots[t] = -1;
+    p.owners[t] = -1;
 }
 
 __device__ __forceinline__ int64_t wave_inclusive(int64_t v) {
@@ -74,9 +99,12 @@ __device__ __forceinline__ int64_t wave_inclusive(int64_t v) {
     return v;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void k_plan(prism_kv_plan p, PlanScratch sc, int fill, int *err) {
+template <bool OWN>
+__global__ __launch_bounds__(kPlanThreads) void k_plan(prism_kv_plan p, PlanScratch sc, int *err) {
     __shared__ int64_t part[3][kPlanThreads / 64];
     __shared__ int bad_any;
+    constexpr uint32_t kOwn = OWN ? kPlanOwnRequests : 1;
+    __shared__ int32_t own_offset[kOwn], own_old[kOwn], own_need[kOwn], own_back[kOwn];
     const uint32_t tid = threadIdx.x, wave = tid / 64, waves = blockDim.x / 64;
     if (tid == 0) bad_any = 0;
     __syncthreads();
@@ -118,82 +146,205 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(prism_kv_plan p, PlanScra
     const bool refused = wrong || missing > 0;
     for (uint32_t r = r0; r < r1; ++r) {
         const int32_t n = p.lengths[r], a = p.added[r];
-        p.offsets[r] = refused ? 0 : static_cast<int32_t>(before[0]);
+        const int32_t offset = refused ? 0 : static_cast<int32_t>(before[0]);
+        p.offsets[r] = offset;
         if (refused) {
             p.new_lengths[r] = n;
             continue;
         }
-        sc.need_base[r] = static_cast<int32_t>(before[1]);
-        sc.back_base[r] = static_cast<int32_t>(before[2]);
+        if constexpr (OWN) {
+            own_offset[r] = offset;
+            own_old[r] = n;
+            own_need[r] = static_cast<int32_t>(before[1]);
+            own_back[r] = static_cast<int32_t>(before[2]);
+        } else {
+            sc.need_base[r] = static_cast<int32_t>(before[1]);
+            sc.back_base[r] = static_cast<int32_t>(before[2]);
+        }
         p.new_lengths[r] = a == -1 ? 0 : n + a;
         const int64_t held = pages_of(n, p.page_size);
         before[0] += a == -1 ? 0 : a;
         before[1] += a == -1 ? 0 : pages_of(static_cast<int64_t>(n) + a, p.page_size) - held;
         before[2] += a == -1 ? held : 0;
     }
-    const int32_t tokens = refused ? 0 : static_cast<int32_t>(total[0]);
+    const int32_t tokens = refused ? 0 : static_cast<int32_t>(total[0]), back = refused ? 0 : static_cast<int32_t>(total[2]);
     if (tid == 0) {
         p.offsets[p.requests] = tokens;
         p.counts[0] = static_cast<int32_t>(refused ? count : height - total[1]);
         p.counts[1] = tokens;
         p.counts[2] = static_cast<int32_t>(refused ? 0 : total[1]);
         p.counts[3] = static_cast<int32_t>(missing < 0x7fffffff ? missing : 0x7fffffff);
-        sc.head[0] = tokens;
-        sc.head[1] = static_cast<int32_t>(refused ? 0 : height);
+        if constexpr (!OWN) {
+            sc.head[0] = tokens;
+            sc.head[1] = count;
+            sc.head[2] = back;
+        }
         if (wrong) raise_error(err, kErrIndex);
         if (missing) raise_error(err, kErrPages);
     }
-    __syncthreads();
-    if (!refused)
-        for (int32_t b = static_cast<int32_t>(tid); b < total[2]; b += static_cast<int32_t>(blockDim.x)) {
-            const uint32_t r = last_at_most(sc.back_base, p.requests, b);
-            p.free_pages[count + b] = p.block_table[static_cast<uint64_t>(r) * p.max_pages + (b - sc.back_base[r])];
+    if constexpr (OWN) {
+        __syncthreads();
+        for (int32_t b = static_cast<int32_t>(tid); b < back; b += static_cast<int32_t>(blockDim.x))
+            p.free_pages[count + b] = page_given_back(p, own_back, b);
+        for (uint32_t t = tid; t < p.max_tokens; t += blockDim.x) {
+            if (static_cast<int32_t>(t) >= tokens) {
+                plan_no_token(p, t);
+                continue;
+            }
+            const uint32_t r = last_at_most(own_offset, p.requests, static_cast<int32_t>(t));
+            plan_token(p, own_back, t, r, own_old[r], own_offset[r], own_need[r], count, back);
         }
-    if (!fill) return;
-    __syncthreads();
-    for (uint32_t t = tid; t < p.max_tokens; t += blockDim.x) plan_fill(p, sc, t, tokens, static_cast<int32_t>(height));
+    }
 }
 
 __global__ __launch_bounds__(256) void k_plan_fill(prism_kv_plan p, PlanScratch sc) {
     const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-    if (t < p.max_tokens) plan_fill(p, sc, t, sc.head[0], sc.head[1]);
+    const int32_t tokens = sc.head[0], count = sc.head[1], back = sc.head[2];
+    for (int32_t b = static_cast<int32_t>(t); b < back; b += static_cast<int32_t>(gridDim.x * 256))
+        p.free_pages[count + b] = page_given_back(p, sc.back_base, b);
+    if (static_cast<int32_t>(t & ~63u) < tokens) {
+        const uint32_t r = last_at_most_wave(p.offsets, p.requests, static_cast<int32_t>(t));
+        if (static_cast<int32_t>(t) < tokens) {
+            plan_token(p, sc.back_base, t, r, p.new_lengths[r] - p.added[r], p.offsets[r], sc.need_base[r], count, back);
+            return;
+        }
+    }
+    if (t < p.max_tokens) plan_no_token(p, t);
 }
 
 // ---- rotary positions -------------------------------------------------------------------
-// One workgroup rotates kRopeTokens tokens of some heads: it first makes their cosines and
-// sines in binary64 (one pair of them serves every head), then a lane takes four consecutive
-// elements of a row and their partners.  binary64 FMAs run at the binary32 rate here, so
-// the exact rotation costs no more than a rounded one; memory bounds it.
+// A workgroup rotates kRopeTokens tokens of some heads, a wavefront one token: the workgroup makes
+// their cosines and sines in binary64 first (one pair of them serves every head), then each lane
+// keeps those of its four pairs and takes the heads, several rows in flight.  binary64 FMAs
+// run at the binary32 rate here, so the exact rotation costs no more than a rounded one; memory
+// bounds it.
 
 constexpr uint32_t kRopeTokens = 4;
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation rot, const int32_t *positions, uint32_t tokens,
-                                              uint32_t heads_each, double eps, int *err) {
-    constexpr uint32_t kLanes = D / 4, kRows = 64 / kLanes;  // lanes of a row, rows of a wavefront
-    __shared__ double cs[kRopeTokens][D / 2], sn[kRopeTokens][D / 2];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, half = rot.dims / 2;
-    const uint32_t t0 = blockIdx.x * kRopeTokens, nt = min(kRopeTokens, tokens - t0);
-    for (uint32_t i = tid; i < nt * half; i += 256) {
+__device__ __forceinline__ void rope_table(double (*cs)[128], double (*sn)[128], const Rotation &rot, const int32_t *positions,
+                                           uint32_t nt) {
+    const uint32_t half = rot.dims / 2;
+    for (uint32_t i = threadIdx.x; i < nt * half; i += 256) {
         const uint32_t t = i / half, k = i % half;
         double s, c;
-        sincos(static_cast<double>(positions[t0 + t]) * rot.freq[k], &s, &c);
+        sincos(static_cast<double>(positions[t]) * rot.freq[k], &s, &c);
         cs[t][k] = c * rot.magnitude;
         sn[t][k] = s * rot.magnitude;
     }
     __syncthreads();
-    const uint32_t all = a.heads + b.heads, h0 = blockIdx.y * heads_each, h1 = min(all, h0 + heads_each);
+}
+
+// dims a multiple of 8: a lane has four pairs of a row (four elements of each half, or eight
+// neighbours where interleaved), or eight elements behind the rotated ones.
+template <typename T, int D, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation rot, const int32_t *positions, uint32_t tokens,
+                                              uint32_t heads_each, double eps, int *err) {
+    constexpr uint32_t kLanes = D / 8, kRows = 64 / kLanes;  // lanes of a row, rows of a wavefront
+    constexpr uint32_t kFlight = 4;                          // row groups whose loads are in flight together
+    __shared__ double cs[kRopeTokens][128], sn[kRopeTokens][128];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, half = rot.dims / 2;
+    const uint32_t t0 = blockIdx.x * kRopeTokens, nt = min(kRopeTokens, tokens - t0);
+    rope_table(cs, sn, rot, positions + t0, nt);
+    if (wave >= nt) return;
+    const uint32_t li = lane % kLanes, t = t0 + wave;
+    const bool turns = 8 * li < rot.dims;
+    // This lane's two runs of four elements.
+    const uint32_t e0 = INTERLEAVED || !turns ? 8 * li : 4 * li, e1 = INTERLEAVED || !turns ? e0 + 4 : e0 + half;
+    double c[4], s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        c[j] = turns ? cs[wave][4 * li + j] : 1.0;
+        s[j] = turns ? sn[wave][4 * li + j] : 0.0;
+    }
+    const uint32_t h0 = blockIdx.y * heads_each, h1 = min(a.heads + b.heads, h0 + heads_each);
+    bool bad = false;
+    // The heads of a, then those of b.
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        const RopeRows &m = which ? b : a;
+        const uint32_t from = which ? max(h0, a.heads) - a.heads : h0;
+        const uint32_t to = which ? (h1 > a.heads ? h1 - a.heads : 0) : min(h1, a.heads);
+        if (from >= to) continue;
+        f32x4 w0{1, 1, 1, 1}, w1{1, 1, 1, 1};
+        if (m.norm) w0 = load4(m.norm + e0), w1 = load4(m.norm + e1);
+        const T *x = static_cast<const T *>(m.x) + t * m.x_stride;
+        T *out = static_cast<T *>(m.out) + t * m.out_stride;
+        for (uint32_t h = from + lane / kLanes; h - lane / kLanes < to; h += kRows * kFlight) {
+            f32x4 v0[kFlight], v1[kFlight];
+#pragma unroll
+            for (uint32_t u = 0; u < kFlight; ++u) {
+                const uint32_t hh = min(h + u * kRows, to - 1);
+                v0[u] = load4(x + hh * D + e0);
+                v1[u] = load4(x + hh * D + e1);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kFlight; ++u) {
+                double y[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    bad |= !finite(v0[u][j]) || !finite(v1[u][j]);
+                    y[j] = v0[u][j];
+                    y[4 + j] = v1[u][j];
+                }
+                if (m.norm) {
+                    double q = 0.0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q = __builtin_fma(y[j], y[j], q);
+#pragma unroll
+                    for (uint32_t d = 1; d < kLanes; d *= 2) q += __shfl_xor(q, d);
+                    const double scale = 1.0 / sqrt(q / D + eps);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        y[j] = y[j] * scale * static_cast<double>(w0[j]);
+                        y[4 + j] = y[4 + j] * scale * static_cast<double>(w1[j]);
+                    }
+                }
+                f32x4 o0, o1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double p = INTERLEAVED ? y[2 * j] : y[j], q = INTERLEAVED ? y[2 * j + 1] : y[4 + j];
+                    const float f = static_cast<float>(__builtin_fma(p, c[j], -(q * s[j])));
+                    const float g = static_cast<float>(__builtin_fma(q, c[j], p * s[j]));
+                    if constexpr (INTERLEAVED) (j < 2 ? o0 : o1)[2 * (j & 1)] = f, (j < 2 ? o0 : o1)[2 * (j & 1) + 1] = g;
+                    else o0[j] = f, o1[j] = g;
+                }
+                if (h + u * kRows < to) {
+                    store4(out + (h + u * kRows) * D + e0, o0);
+                    store4(out + (h + u * kRows) * D + e1, o1);
+                }
+            }
+        }
+    }
+    if (bad) raise_error(err, kErrInput);
+}
+
+// Any dims: a lane has four consecutive elements and looks their partners up.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_rope_any(RopeRows a, RopeRows b, Rotation rot, const int32_t *positions, uint32_t tokens,
+                                                  uint32_t heads_each, double eps, int *err) {
+    constexpr uint32_t kLanes = D / 4, kRows = 64 / kLanes;
+    __shared__ double cs[kRopeTokens][128], sn[kRopeTokens][128];
+    const uint32_t lane = threadIdx.x & 63, half = rot.dims / 2;
+    const uint32_t t0 = blockIdx.x * kRopeTokens, nt = min(kRopeTokens, tokens - t0);
+    rope_table(cs, sn, rot, positions + t0, nt);
+    const uint32_t h0 = blockIdx.y * heads_each, h1 = min(a.heads + b.heads, h0 + heads_each);
     const uint32_t groups = (h1 - h0 + kRows - 1) / kRows;
     const uint32_t e0 = 4 * (lane % kLanes);
     bool bad = false;
-    for (uint32_t it = tid / 64; it < nt * groups; it += 4) {
+    for (uint32_t it = threadIdx.x / 64; it < nt * groups; it += 4) {
         const uint32_t t = it / groups, h = h0 + it % groups * kRows + lane / kLanes;
-        const bool live = h < h1;
-        const RopeRows &m = h < a.heads ? a : b;
-        const uint32_t hh = min(h, h1 - 1) - (h < a.heads ? 0 : a.heads);
-        const T *x = static_cast<const T *>(m.x) + (t0 + t) * m.x_stride + static_cast<uint64_t>(hh) * D;
-        f32x4 v{0, 0, 0, 0};
-        if (live) v = load4(x + e0);
+        const uint32_t hc = min(h, h1 - 1);
+        const RopeRows &m = hc < a.heads ? a : b;
+        const uint64_t row = static_cast<uint64_t>(hc < a.heads ? hc : hc - a.heads) * D;
+        const T *x = static_cast<const T *>(m.x) + (t0 + t) * m.x_stride + row;
+        const f32x4 v = load4(x + e0);
+        f32x4 partner;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t e = e0 + j;
+            const uint32_t o = e >= rot.dims ? e : rot.interleaved ? e ^ 1 : e < half ? e + half : e - half;
+            partner[j] = static_cast<float>(x[o]);
+        }
         double scale = 1.0;
         if (m.norm) {
             double q = 0.0;
@@ -203,35 +354,33 @@ __global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation r
             for (uint32_t d = 1; d < kLanes; d *= 2) q += __shfl_xor(q, d);
             scale = 1.0 / sqrt(q / D + eps);
         }
-        if (!live) continue;
         f32x4 out;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (uint32_t j = 0; j < 4; ++j) {
             const uint32_t e = e0 + j;
             bad |= !finite(v[j]);
-            double y = v[j];
+            double y = v[j], z = partner[j];
             if (m.norm) y = y * scale * m.norm[e];
             if (e < rot.dims) {
                 const bool first = rot.interleaved ? !(e & 1) : e < half;
                 const uint32_t o = rot.interleaved ? e ^ 1 : first ? e + half : e - half;
                 const uint32_t k = rot.interleaved ? e / 2 : first ? e : o;
-                double z = rot.interleaved ? v[j ^ 1] : static_cast<float>(x[o]);
                 if (m.norm) z = z * scale * m.norm[o];
-                y = y * cs[t][k] + (first ? -z : z) * sn[t][k];
+                y = first ? __builtin_fma(y, cs[t][k], -(z * sn[t][k])) : __builtin_fma(y, cs[t][k], z * sn[t][k]);
             }
             out[j] = static_cast<float>(y);
         }
-        store4(static_cast<T *>(m.out) + (t0 + t) * m.out_stride + static_cast<uint64_t>(hh) * D + e0, out);
+        if (h < h1) store4(static_cast<T *>(m.out) + (t0 + t) * m.out_stride + row + e0, out);
     }
     if (bad) raise_error(err, kErrInput);
 }
 
 // ---- append -----------------------------------------------------------------------------
-// A run is the new tokens of one page: consecutive tokens on consecutive slots.  One
-// wavefront takes one run's keys or values of one head, so a page's scale and codes have
-// one writer and no result depends on timing.  It reads the run twice (the magnitudes, then
-// the codes; the second time from cache), and rewrites the page's earlier codes where the
-// scale grew.
+// A run is the new tokens of one page: consecutive tokens on consecutive slots.  One workgroup
+// takes the keys or values of one head of the runs that begin among its tokens, so a page's
+// scale and codes have one writer and no result depends on timing.  Runs that a wavefront's
+// registers hold (single tokens above all) go to one wavefront each, longer ones to all four, which
+// exchange their magnitudes.  Earlier codes of the page are rewritten only where the scale grew.
 
 template <int FMT>
 __device__ __forceinline__ float least_scale(float most) {  // 2^e, most <= qmax 2^e
@@ -245,7 +394,11 @@ __device__ __forceinline__ float least_scale(float most) {  // 2^e, most <= qmax
 
 template <int FMT>
 __device__ __forceinline__ uint32_t rescale4(uint32_t c, float by) {
-    return code4<FMT>(value4<FMT>(c) * by);
+    f32x4 v = value4<FMT>(c);
+    if constexpr (FMT == kE4m3)  // memory never written may hold NaN codes
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = v[i] == v[i] ? v[i] : 0.0f;
+    return code4<FMT>(v * by);
 }
 
 struct AppendArgs {
@@ -256,75 +409,142 @@ struct AppendArgs {
     uint32_t tokens;
 };
 
-template <typename T, int FMT, int D>
-__device__ void append_run(const prism_kv_cache &c, const T *x, uint64_t stride, bool is_v, uint32_t head, uint32_t page,
-                           uint32_t first, uint32_t n, int *err) {
-    constexpr uint32_t kLanes = D / 4, kRows = 64 / kLanes;
-    const uint32_t lane = threadIdx.x & 63, e0 = 4 * (lane % kLanes), ps = c.page_size;
-    float most = 0.0f;
-    bool bad = false;
-    for (uint32_t i = lane / kLanes; i < n; i += kRows) {
-        const f32x4 v = load4(x + i * stride + e0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            bad |= !finite(v[j]);
-            most = fmaxf(most, finite(v[j]) ? fabsf(v[j]) : 0.0f);
-        }
-    }
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    if (bad) raise_error(err, kErrInput);
-    const uint64_t unit = static_cast<uint64_t>(page) * c.kv_heads + head;
-    float *scale = (is_v ? c.v_scale : c.k_scale) + unit;
-    const float old = first ? *scale : 0.0f, s = fmaxf(old, least_scale<FMT>(most));
-    const float inv = 1.0f / s, by = old * inv;
-    const bool grew = first && s != old;
-    uint8_t *codes = static_cast<uint8_t *>(is_v ? c.v : c.k) + unit * ps * D;
-    if (!is_v) {
-        if (grew)
-            for (uint32_t i = 4 * lane; i < first * D; i += 256) {
-                uint32_t *w = reinterpret_cast<uint32_t *>(codes + i);
-                *w = rescale4<FMT>(*w, by);
-            }
-        for (uint32_t i = lane / kLanes; i < n; i += kRows)
-            *reinterpret_cast<uint32_t *>(codes + (first + i) * D + e0) = code4<FMT>(load4(x + i * stride + e0) * inv);
-    } else {
-        // Four places of a dimension at a time.
-        const uint32_t end = first + n;
-        for (uint32_t g = grew ? 0 : first & ~3u; g < end; g += 4)
-            for (uint32_t d = lane; d < D; d += 64) {
-                f32x4 v{0, 0, 0, 0};
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j)
-                    if (g + j >= first && g + j < end) v[j] = static_cast<float>(x[(g + j - first) * stride + d]);
-                uint32_t *w = reinterpret_cast<uint32_t *>(codes + d * ps + g);
-                uint32_t r = code4<FMT>(v * inv);
-                if (g < first || g + 4 > end) {  // keep, or rescale, what the page held beside the run
-                    const uint32_t had = *w, again = grew ? rescale4<FMT>(had, by) : had;
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        const uint32_t mask = 255u << (8 * j);
-                        if (g + j < first) r = (r & ~mask) | (again & mask);
-                        else if (g + j >= end) r = (r & ~mask) | (had & mask);
-                    }
-                }
-                *w = r;
-            }
-    }
-    if (lane == 0) *scale = s;
+// The bytes of places below `end` among the four from `place` on.
+__device__ __forceinline__ uint32_t bytes_below(uint32_t place, uint32_t end) {
+    return end >= place + 4 ? ~0u : end <= place ? 0u : (1u << (8 * (end - place))) - 1;
 }
 
-// A wavefront looks for the runs that begin among `each` (at most 32) tokens.
+// A lane has four dimensions of sixteen places (an aligned group of the page), their loads in
+// flight together (places beside the run load its nearest token: no branches, and the same largest
+// magnitude); a step is as many groups as the lanes of a wavefront, or of all four, cover.  The
+// last step stays in registers; only runs of more than one are read twice.
+template <typename T, int FMT, int D>
+__device__ __forceinline__ void append_run(const prism_kv_cache &c, const T *x, uint64_t stride, bool is_v, uint32_t head, uint32_t page,
+                                           uint32_t first, uint32_t n, bool all, float *shared, int *err) {
+    constexpr uint32_t kLanes = D / 4;
+    const uint32_t lanes = all ? 256 : 64, lane = threadIdx.x & (lanes - 1), groups = lanes / kLanes;
+    const uint32_t e0 = 4 * (lane % kLanes), ps = c.page_size, end = first + n;
+    const uint32_t g0 = first / 16, steps = ((end + 15) / 16 - g0 + groups - 1) / groups;
+    const uint64_t unit = static_cast<uint64_t>(page) * c.kv_heads + head;
+    float *scale = (is_v ? c.v_scale : c.k_scale) + unit;
+    uint8_t *codes = static_cast<uint8_t *>(is_v ? c.v : c.k) + unit * ps * D;
+    const float before = *scale;
+    typename Four<T>::type held[16];
+    uint32_t at = 0;  // the lane's group in the step that is held
+    auto load = [&](uint32_t step) {
+        at = 16 * (g0 + step * groups + lane / kLanes);
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j)
+            held[j] = load_any<typename Four<T>::type>(x + (min(max(at + j, first), end - 1) - first) * stride + e0);
+    };
+    uint32_t most = 0;  // magnitudes compare as integers, NaN and infinities above all others
+    for (uint32_t step = 0; step < steps; ++step) {
+        load(step);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = max(most, __float_as_uint(static_cast<float>(held[j][i])) & 0x7fffffffu);
+    }
+    // What a group of values holds beside the run's places.
+    u32x4 had[4];
+    const bool whole = at >= first && at + 16 <= end, partial = is_v && !whole && at < end;
+    if (partial)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) had[i] = *reinterpret_cast<const u32x4 *>(codes + (e0 + i) * ps + at);
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+    if (all) {  // also: every wavefront has read the scale before it is written
+        if ((threadIdx.x & 63) == 0) shared[threadIdx.x / 64] = __uint_as_float(most);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = max(most, __float_as_uint(shared[w]));
+        __syncthreads();
+    }
+    const bool bad = most >= 0x7f800000u;
+    if (bad) {  // the largest finite magnitude; each wavefront for itself
+        raise_error(err, kErrInput);
+        most = 0;
+        const uint32_t l = threadIdx.x & 63;
+        for (uint32_t i = l / kLanes; i < n; i += 64 / kLanes) {
+            const f32x4 v = load4(x + i * stride + 4 * (l % kLanes));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) most = finite(v[k]) ? max(most, __float_as_uint(v[k]) & 0x7fffffffu) : most;
+        }
+#pragma unroll
+        for (uint32_t d = 1; d < 64; d *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+    }
+    const float old = first ? before : 0.0f, s = fmaxf(old, least_scale<FMT>(__uint_as_float(most)));
+    const float inv = 1.0f / s, by = old * inv;
+    const bool grew = first && s != old;
+    if (lane == 0) *scale = s;
+    if (grew) {  // the codes before the run, at the new scale; a group of values the run shares is done below
+        const uint32_t pieces = is_v ? g0 * D : first * D / 16;  // of sixteen bytes
+        for (uint32_t i = lane; i < pieces; i += 4 * lanes) {    // four in flight
+            u32x4 r[4];
+            u32x4 *w[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+                const uint32_t k = min(i + lanes * u, pieces - 1);
+                w[u] = reinterpret_cast<u32x4 *>(codes + (is_v ? k % D * ps + 16 * (k / D) : 16 * k));
+                r[u] = *w[u];
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) r[u][k] = rescale4<FMT>(r[u][k], by);
+                if (i + lanes * u < pieces) *w[u] = r[u];
+            }
+        }
+    }
+    for (uint32_t step = steps; step-- > 0;) {
+        if (step + 1 < steps) load(step);
+        if (bad)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) held[j][i] = held[j][i] == held[j][i] ? held[j][i] : static_cast<T>(0.0f);
+        if (at >= end) continue;
+        if (!is_v) {
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j)
+                if (at + j >= first && at + j < end)
+                    *reinterpret_cast<uint32_t *>(codes + (at + j) * D + e0) = code4<FMT>(__builtin_convertvector(held[j], f32x4) * inv);
+            continue;
+        }
+        const bool kept = at < first || at + 16 > end;  // the group has places beside the run
+        if (kept && step + 1 < steps)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) had[i] = *reinterpret_cast<const u32x4 *>(codes + (e0 + i) * ps + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u32x4 r;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                r[k] = code4<FMT>(f32x4{static_cast<float>(held[4 * k][i]), static_cast<float>(held[4 * k + 1][i]),
+                                        static_cast<float>(held[4 * k + 2][i]), static_cast<float>(held[4 * k + 3][i])} * inv);
+            if (kept)
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t low = bytes_below(at + 4 * k, first), below = bytes_below(at + 4 * k, end);
+                    const uint32_t again = grew ? rescale4<FMT>(had[i][k], by) : had[i][k];
+                    r[k] = (again & low) | (r[k] & below & ~low) | (had[i][k] & ~below);
+                }
+            *reinterpret_cast<u32x4 *>(codes + (e0 + i) * ps + at) = r;
+        }
+    }
+}
+
+// The runs that begin among `each` (at most 32) tokens.
 template <typename T, int FMT, int D>
 __global__ __launch_bounds__(256) void k_append(AppendArgs a, uint32_t each, int *err) {
-    const uint32_t lane = threadIdx.x & 63, task = blockIdx.y * 4 + threadIdx.x / 64;
-    if (task >= 2 * a.c.kv_heads) return;
+    __shared__ float shared[4];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), task = blockIdx.y;
     const uint32_t t0 = blockIdx.x * each, ps = a.c.page_size;
     const int32_t slots = static_cast<int32_t>(a.c.pages * ps);
     // Lane l holds the slot of token t0 - 1 + l.
     const int64_t mine = static_cast<int64_t>(t0) + lane - 1;
     int32_t s = -1;
-    if (lane <= each && mine >= 0 && mine < a.tokens) s = a.slots[mine];
+    if (mine >= 0 && mine < a.tokens) s = a.slots[mine];
     const bool here = lane >= 1 && lane <= each;
     bool bad = here && (s < -1 || s >= slots);
     if (s < 0 || s >= slots) s = -1;
@@ -335,26 +555,32 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs a, uint32_t each, int
         bad = true;  // a second run in the page
         leads = false;
     }
-    if (bad && task == 0) raise_error(err, kErrIndex);
+    if (bad && task == 0 && wave == 0) raise_error(err, kErrIndex);
     const bool is_v = task >= a.c.kv_heads;
     const uint32_t head = is_v ? task - a.c.kv_heads : task;
     const uint64_t stride = is_v ? a.v_stride : a.k_stride;
-    uint64_t left = __ballot(leads);
-    while (left) {
+    // All four wavefronts see the same runs.
+    uint32_t turn = 0;
+    for (uint64_t left = __ballot(leads); left; left &= left - 1) {
         const int l = __builtin_ctzll(left);
-        left &= left - 1;
         const uint32_t t = t0 + l - 1, slot = static_cast<uint32_t>(__shfl(s, l));
         const uint32_t page = slot / ps, first = slot % ps, most = min(ps - first, a.tokens - t);
-        uint32_t n = 0;
-        for (uint32_t base = 0; base < most; base += 64) {  // how many tokens follow
-            const uint32_t i = base + lane;
-            const uint64_t on = __ballot(i < most && static_cast<uint32_t>(a.slots[t + i]) == slot + i);
-            const uint32_t run = ~on ? __builtin_ctzll(~on) : 64;
-            n += run;
-            if (run < 64) break;
-        }
+        // How many tokens follow: among the lanes', and further on.
+        const uint64_t off = __ballot(static_cast<int>(lane) >= l && static_cast<uint32_t>(s) != slot + lane - l) >> l;
+        uint32_t n = off ? __builtin_ctzll(off) : 64 - l;
+        if (n == 64u - l)
+            for (uint32_t i0 = n; i0 < most; i0 += 64) {
+                const uint32_t i = i0 + lane;
+                const uint64_t no = ~__ballot(i < most && static_cast<uint32_t>(a.slots[t + i]) == slot + i);
+                const uint32_t more = no ? __builtin_ctzll(no) : 64;
+                n += more;
+                if (more < 64) break;
+            }
+        n = min(n, most);
         const T *x = static_cast<const T *>(is_v ? a.v : a.k) + t * stride + static_cast<uint64_t>(head) * D;
-        append_run<T, FMT, D>(a.c, x, stride, is_v, head, page, first, n, err);
+        constexpr uint32_t kWaveGroups = 64 / (D / 4);
+        const bool all = (first + n + 15) / 16 - first / 16 > kWaveGroups;
+        if (all || turn++ % 4 == wave) append_run<T, FMT, D>(a.c, x, stride, is_v, head, page, first, n, all, shared, err);
     }
 }
 
@@ -362,12 +588,16 @@ template <typename T, int D>
 int rope_typed(const Rotation &rot, const RopeRows &a, const RopeRows &b, const int32_t *positions, uint32_t tokens, float eps,
                int *err, hipStream_t s) {
     const uint32_t tiles = (tokens + kRopeTokens - 1) / kRopeTokens, heads = a.heads + b.heads;
-    // Heads are split over workgroups until some 1024 of them share the rows.
+    const bool eights = rot.dims % 8 == 0;
+    // Heads are split over workgroups until some 1024 of them share the rows, whole row groups each.
+    const uint32_t least = eights ? 64 / (D / 8) : 4 * 64 / (D / 4);
     uint32_t parts = (1024 + tiles - 1) / tiles;
-    constexpr uint32_t least = 4 * 64 / (D / 4);  // rows of a workgroup's four wavefronts
     if (parts > (heads + least - 1) / least) parts = (heads + least - 1) / least;
-    const uint32_t each = (heads + parts - 1) / parts;
-    k_rope<T, D><<<dim3(tiles, (heads + each - 1) / each), 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, err);
+    const uint32_t each = ((heads + parts - 1) / parts + least - 1) / least * least;
+    const dim3 grid(tiles, (heads + each - 1) / each);
+    if (!eights) k_rope_any<T, D><<<grid, 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, err);
+    else if (rot.interleaved) k_rope<T, D, true><<<grid, 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, err);
+    else k_rope<T, D, false><<<grid, 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, err);
     return launch_status();
 }
 template <typename T>
@@ -403,10 +633,15 @@ size_t plan_scratch_bytes(uint32_t requests) { return sizeof(int32_t) * (2 * (st
 
 int launch_kv_plan(const prism_kv_plan &p, void *scratch, int *err, hipStream_t s) {
     const PlanScratch sc = plan_scratch(scratch, p.requests);
-    const bool own = p.max_tokens <= kPlanOwnFill;
-    k_plan<<<1, kPlanThreads, 0, s>>>(p, sc, own, err);
+    const uint32_t wide = p.requests > p.max_tokens ? p.requests : p.max_tokens;
+    const uint32_t threads = wide >= kPlanThreads ? kPlanThreads : (wide + 63) / 64 * 64;
+    if (p.max_tokens <= kPlanOwnTokens && p.requests <= kPlanOwnRequests) {
+        k_plan<true><<<1, threads, 0, s>>>(p, sc, err);
+        return launch_status();
+    }
+    k_plan<false><<<1, threads, 0, s>>>(p, sc, err);
     const int rc = launch_status();
-    if (rc || own) return rc;
+    if (rc) return rc;
     k_plan_fill<<<(p.max_tokens + 255) / 256, 256, 0, s>>>(p, sc);
     return launch_status();
 }
@@ -421,8 +656,8 @@ int launch_rope(int dtype, const Rotation &rot, const RopeRows &a, const RopeRow
 int launch_kv_append(const prism_kv_cache &cache, int dtype, const void *k, uint64_t k_stride, const void *v,
                      uint64_t v_stride, const int32_t *slots, uint32_t tokens, int *err, hipStream_t s) {
     const AppendArgs a{cache, k, v, k_stride, v_stride, slots, tokens};
-    const uint32_t each = tokens <= 512 ? 1 : tokens <= 4096 ? 4 : 16;
-    const dim3 grid((tokens + each - 1) / each, (2 * cache.kv_heads + 3) / 4);
+    const uint32_t each = tokens <= 1024 ? 4 : tokens <= 4096 ? 16 : 32;
+    const dim3 grid((tokens + each - 1) / each, 2 * cache.kv_heads);
     if (dtype == PRISM_DTYPE_F32) return append_typed<float>(a, each, grid, err, s);
     if (dtype == PRISM_DTYPE_F16) return append_typed<_Float16>(a, each, grid, err, s);
     return append_typed<__bf16>(a, each, grid, err, s);

@@ -49,20 +49,21 @@ __device__ __forceinline__ void store4(T *p, f32x4 v) {  // ties to even
 
 constexpr int kInt8 = PRISM_CACHE_INT8, kE4m3 = PRISM_CACHE_E4M3;
 
-// The code of v, whose magnitude is at most the format's largest value but for infinities
-// and rounding of the scale; ties to even.  NaN is 0.
+// The codes of four values, ties to even, magnitudes past the format's largest at it.  Not for NaN.
 template <int FMT>
 __device__ __forceinline__ uint32_t code4(f32x4 v) {
     constexpr float top = FMT == kInt8 ? 127.0f : 448.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = v[i] == v[i] ? fminf(fmaxf(v[i], -top), top) : 0.0f;
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_fmed3f(v[i], -top, top);
     if constexpr (FMT == kInt8) {
-        uint32_t r = 0;
+        // 1.5 * 2^23 + v rounds v to an integer, whose two's complement the sum's low byte is.
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r |= (static_cast<uint32_t>(static_cast<int>(rintf(v[i]))) & 255u) << (8 * i);
-        return r;
+        for (int i = 0; i < 4; ++i) v[i] += 12582912.0f;
+        const uint32_t low = perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x0c0c0400u);
+        const uint32_t high = perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x04000c0cu);
+        return low | high;
     } else {
-        int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        const int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
         return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], r, true));
     }
 }
