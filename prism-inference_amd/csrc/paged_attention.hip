@@ -4,7 +4,7 @@
 // A request's queries of one kv head form rows (token, head of the group); a wavefront takes
 // 16 * NT of them through blocks of 64 keys with the running maximum and sum of the softmax:
 //   S^T = K Q^T   K codes (exact in binary16) as the A operand, 16 keys a matrix instruction
-//   z = S * (scale * k_scale) + log2 v_scale, p = 2^(z - max z), l = sum p / v_scale
+//   z = S * (scale * k_scale) + log2 v_scale, p = 2^(z - m), l = sum p / v_scale
 //   O^T += V^T P^T
 // so a page's two scales cost nothing per key: the keys' joins the softmax scale, the values'
 // the exponent, and p stays within the operand's range however the pages' scales differ.
@@ -12,7 +12,7 @@
 // Keys are assigned to the rows of K's matrix instructions so that a lane's 16 scores of a
 // block are 16 consecutive keys, all of one page: they are the B operand of the second product
 // as they stand (no exchange between lanes), and one 16-byte load of the transposed values
-// is the A operand that meets them.  Neither codes nor probabilities pass through LDS.
+// is the A operand that meets them.
 #include "serve_common.hpp"
 
 namespace prism {
@@ -20,9 +20,10 @@ namespace prism {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Probabilities enter the second product as 2^14 p: contributions down to 2^-28 of the largest
-// keep binary16's full precision.
-constexpr float kHeadroom = 14.0f;
+// Probabilities enter the second product as 2^11 2^(z - m), with m at most kSlack below the largest z
+// (rows are rescaled only where it grew by more): at most 2^15, and full binary16 precision for
+// contributions down to 2^-25 of the largest.
+constexpr float kHeadroom = 11.0f, kSlack = 4.0f;
 constexpr float kNone = -__builtin_inff();
 
 struct AttendArgs {
@@ -146,134 +147,241 @@ __device__ __forceinline__ void write_row(const AttendArgs &p, uint32_t token, u
     store4(static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * p.c.head_dim + dim, v);
 }
 
-// T: type of q and out.  LIMBS: binary16 parts of q and of the probabilities (2 for binary32).
-// SHARED: the workgroup's four wavefronts share 16 * NT rows and split the keys (few rows);
-// otherwise each has 16 * NT rows of its own.
-template <typename T, int D, int FMT, int NT, bool SHARED>
-__global__ __launch_bounds__(256) void k_attend(AttendArgs p, int *err) {
-    constexpr int LIMBS = sizeof(T) == 4 ? 2 : 1;
-    constexpr int KS = D / 32, DT = D / 16;
-    constexpr uint32_t M = SHARED ? 16 * NT : 64 * NT;  // rows of a workgroup
-    __shared__ float join_ml[SHARED ? 4 : 1][SHARED ? 16 * NT : 1][2];
-    __shared__ f32x4 join_acc[SHARED ? 3 : 1][SHARED ? NT * DT : 1][SHARED ? 64 : 1];
-
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t n = lane & 15, g = lane / 16;
-    // Heavy tiles first: a prompt's last rows see the most keys.
-    const uint32_t slot = gridDim.x - 1 - blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
-    const uint32_t r = tile_request(p, slot, M);
-    const Request q = request_of(p, r);
-    if (blockIdx.x + blockIdx.y + blockIdx.z == 0)  // offsets out of order may leave a request without a tile
-        for (uint32_t i = threadIdx.x; i < p.a.requests; i += 256)
-            if (request_of(p, i).bad) raise_error(err, kErrIndex);
-    const uint32_t rows = q.n * p.group, start = tile_start(p, r, M), row0 = (slot - start) * M;
-    if (slot < start || row0 >= rows) return;
-    const uint32_t last = min(rows, row0 + M) - 1;
-    if (!SHARED && row0 + wave * 16 * NT >= rows) return;
-
-    // The tile's key blocks, this split's part of them, and this wavefront's.
-    uint32_t b0, b1;
-    blocks_of(p, q, row0 / p.group, last / p.group, &b0, &b1);
-    const uint32_t each = split_blocks(p, b1 - b0);
-    const uint32_t parts = b1 > b0 ? (b1 - b0 + each - 1) / each : 1;
-    if (split >= parts) return;
-    b0 += split * each;
-    b1 = min(b1, b0 + each);
-
-    const uint32_t base_row = SHARED ? row0 : row0 + wave * 16 * NT;
+// What both kernels below share: a wavefront's 16 * NT rows, their queries, statistics and sums.
+// T: type of q and out; LIMBS: binary16 parts of q and of the probabilities (2 for binary32).
+template <typename T, int D, int FMT, int NT>
+struct Rows {
+    static constexpr int LIMBS = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int KS = D / 32, DT = D / 16;
     uint32_t token[NT], head[NT];  // of this lane's rows
     bool live[NT];
-    int32_t lo[NT], hi[NT];
-    float kf[NT];
+    int32_t lo[NT], hi[NT];        // the keys they see
+    int32_t all_lo, all_hi;        // keys every row of the wavefront sees
+    int32_t any_lo, any_hi;        // keys any row sees
+    float kf[NT];                  // base-2 softmax scale of the row's integer-like queries, not negative
     f16x8 qv[LIMBS][NT][KS];
-    int32_t all_lo = 0, all_hi = 0x7fffffff;  // keys every row of the wavefront sees
-    int32_t any_lo = 0x7fffffff, any_hi = 0;  // keys any row sees
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const uint32_t row = base_row + 16 * t + n;
-        live[t] = row < rows;
-        const uint32_t rr = live[t] ? row : last, i = rr / p.group;
-        token[t] = q.first + i;
-        head[t] = kvh * p.group + rr % p.group;
-        visible(p, q, i, &lo[t], &hi[t]);
-        all_lo = max(all_lo, lo[t]);
-        all_hi = min(all_hi, hi[t]);
-        any_lo = min(any_lo, lo[t]);
-        any_hi = max(any_hi, hi[t]);
-        // Lane group g has the dimensions [g D/4, (g + 1) D/4) of the row.
-        const T *src = static_cast<const T *>(p.a.q) + token[t] * p.a.q_stride + static_cast<uint64_t>(head[t]) * D + g * (D / 4);
-        f32x4 x[D / 16];
-        float most = 0.0f;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-            x[j] = load4(src + 4 * j);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(x[j][k]));
-        }
-        most = across_max(most);
-        // A power of two takes the row's largest value to [2^13, 2^14).
-        int e = static_cast<int>(__float_as_uint(most) >> 23 & 255) - 127;
-        e = !finite(most) || e < -100 ? 0 : e;
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
-        kf[t] = p.a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = x[2 * s + j / 4][j % 4] * up;
-                const _Float16 h = static_cast<_Float16>(v);
-                qv[0][t][s][j] = h;
-                if constexpr (LIMBS == 2) qv[LIMBS - 1][t][s][j] = static_cast<_Float16>(v - static_cast<float>(h));
-            }
-    }
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) {
-        all_lo = max(all_lo, __shfl_xor(all_lo, d));
-        all_hi = min(all_hi, __shfl_xor(all_hi, d));
-        any_lo = min(any_lo, __shfl_xor(any_lo, d));
-        any_hi = max(any_hi, __shfl_xor(any_hi, d));
-    }
-
     float m[NT], l[NT];
     f32x4 acc[NT][DT];
+
+    __device__ __forceinline__ void load(const AttendArgs &p, const Request &q, uint32_t base_row, uint32_t last, uint32_t kvh) {
+        const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane / 16;
+        all_lo = 0, all_hi = 0x7fffffff, any_lo = 0x7fffffff, any_hi = 0;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        m[t] = kNone;
-        l[t] = 0.0f;
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t row = base_row + 16 * t + n;
+            live[t] = row <= last;
+            const uint32_t rr = live[t] ? row : last, i = rr / p.group;
+            token[t] = q.first + i;
+            head[t] = kvh * p.group + rr % p.group;
+            visible(p, q, i, &lo[t], &hi[t]);
+            all_lo = max(all_lo, lo[t]);
+            all_hi = min(all_hi, hi[t]);
+            any_lo = min(any_lo, lo[t]);
+            any_hi = max(any_hi, hi[t]);
+            // Lane group g has the dimensions [g D/4, (g + 1) D/4) of the row.
+            const T *src = static_cast<const T *>(p.a.q) + token[t] * p.a.q_stride + static_cast<uint64_t>(head[t]) * D + g * (D / 4);
+            f32x4 x[D / 16];
+            float most = 0.0f;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0, 0, 0, 0};
+            for (int j = 0; j < D / 16; ++j) {
+                x[j] = load4(src + 4 * j);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(x[j][k]));
+            }
+            most = across_max(most);
+            // A power of two takes the row's largest value to [2^13, 2^14); the sign of the scale goes along.
+            int e = static_cast<int>(__float_as_uint(most) >> 23 & 255) - 127;
+            e = !finite(most) || e < -100 ? 0 : e;
+            float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+            if (p.a.scale < 0.0f) up = -up;
+            kf[t] = fabsf(p.a.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = x[2 * s + j / 4][j % 4] * up;
+                    const _Float16 h = static_cast<_Float16>(v);
+                    qv[0][t][s][j] = h;
+                    if constexpr (LIMBS == 2) qv[LIMBS - 1][t][s][j] = static_cast<_Float16>(v - static_cast<float>(h));
+                }
+            m[t] = kNone;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[t][d] = f32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) {
+            all_lo = max(all_lo, __shfl_xor(all_lo, d));
+            all_hi = min(all_hi, __shfl_xor(all_hi, d));
+            any_lo = min(any_lo, __shfl_xor(any_lo, d));
+            any_hi = max(any_hi, __shfl_xor(any_hi, d));
+        }
     }
 
+    // Scores s of the lane's 16 keys from `key` on -> probabilities, the operand of the second product.
+    // ks, vs: the scales of their page; edge: some row does not see some key of the block.
+    __device__ __forceinline__ void softmax(f32x4 (&s)[NT][4], f16x8 (&pv)[LIMBS][NT][2], float ks, float vs, bool there, bool edge,
+                                            int32_t key) {
+        const float lv = __builtin_amdgcn_logf(vs), iv = 1.0f / vs;
+        float f[NT], top[NT];
+        bool grows = false;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            if (edge)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int32_t k = key + 4 * t + i;
+                        s[u][t][i] = there && k >= lo[u] && k < hi[u] ? s[u][t][i] : kNone;
+                    }
+            f[u] = kf[u] * ks;
+            // z = s f + lv rises with s, so the largest s gives the largest z.
+            float most = kNone;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, s[u][t][i]);
+            top[u] = across_max(most == kNone ? kNone : __builtin_fmaf(most, f[u], lv));
+            grows |= top[u] > m[u] + kSlack || m[u] == kNone;
+        }
+        if (__ballot(grows)) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const float next = fmaxf(m[u], top[u]);
+                const float alpha = next == kNone ? 1.0f : __builtin_amdgcn_exp2f(m[u] - next);
+                m[u] = next;
+                l[u] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[u][d] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            // A row that has seen no key yet has m = -inf, and scores of -inf.
+            const float off = lv + kHeadroom - (m[u] == kNone ? 0.0f : m[u]);
+            // 0 * -inf would be NaN where a page's keys are all zero and a key is masked.
+            const float ff = f[u] < 0x1p-120f ? 0x1p-120f : f[u];
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][t][i], ff, off));
+                    sum += e;
+                    const _Float16 h = static_cast<_Float16>(e);
+                    pv[0][u][t / 2][4 * (t % 2) + i] = h;
+                    if constexpr (LIMBS == 2) pv[LIMBS - 1][u][t / 2][4 * (t % 2) + i] = static_cast<_Float16>(e - static_cast<float>(h));
+                }
+            l[u] += sum == 0.0f ? 0.0f : sum * iv;
+        }
+    }
+
+    // The rows, or with more than one part their unnormalised sums: lane (n, g) has the dimensions
+    // 16 d + 4 g .. + 3 of row n.
+    __device__ __forceinline__ void write(const AttendArgs &p, uint32_t parts, uint32_t split, int *err) const {
+        const uint32_t g = (threadIdx.x & 63) / 16;
+        bool bad = false;
+        const uint64_t all_rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (!live[t]) continue;
+            if (parts == 1) {
+                const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+#pragma unroll
+                for (int d = 0; d < DT; ++d) write_row<T>(p, token[t], head[t], 16 * d + 4 * g, acc[t][d] * inv, &bad);
+            } else {
+                const uint64_t row = split * all_rows + static_cast<uint64_t>(token[t]) * p.a.heads + head[t];
+#pragma unroll
+                for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + row * D + 16 * d + 4 * g) = acc[t][d];
+                if (g == 0) {
+                    p.part_ml[2 * row] = m[t];
+                    p.part_ml[2 * row + 1] = l[t];
+                }
+            }
+        }
+        if (bad) raise_error(err, kErrNonfinite);
+    }
+};
+
+// A workgroup's tile: its request, rows and part of the key blocks; false: nothing to do.
+struct Tile {
+    Request q;
+    uint32_t r, row0, last, b0, b1, parts;
+};
+__device__ __forceinline__ bool tile_of(const AttendArgs &p, uint32_t M, uint32_t split, int *err, Tile *t) {
+    // Heavy tiles first: a prompt's last rows see the most keys.
+    const uint32_t slot = gridDim.x - 1 - blockIdx.x;
+    t->r = tile_request(p, slot, M);
+    t->q = request_of(p, t->r);
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0)  // offsets out of order may leave a request without a tile
+        for (uint32_t i = threadIdx.x; i < p.a.requests; i += blockDim.x)
+            if (request_of(p, i).bad) raise_error(err, kErrIndex);
+    const uint32_t rows = t->q.n * p.group, start = tile_start(p, t->r, M);
+    t->row0 = (slot - start) * M;
+    if (slot < start || t->row0 >= rows) return false;
+    t->last = min(rows, t->row0 + M) - 1;
+    uint32_t b0, b1;
+    blocks_of(p, t->q, t->row0 / p.group, t->last / p.group, &b0, &b1);
+    const uint32_t each = split_blocks(p, b1 - b0);
+    t->parts = b1 > b0 ? (b1 - b0 + each - 1) / each : 1;
+    t->b0 = b0 + split * each;
+    t->b1 = min(b1, t->b0 + each);
+    return split < t->parts;
+}
+
+// The page of 16 keys from `key` on, for a lane that reads them: 0, and not `there`, where the table has
+// none or no row sees them.
+__device__ __forceinline__ int32_t page_at(const AttendArgs &p, const int32_t *table, int32_t key, int32_t end, bool *there) {
+    int32_t id = -1;
+    if (key < end) id = table[key >> p.page_log2];
+    *there = id >= 0 && static_cast<uint32_t>(id) < p.c.pages;
+    return *there ? id : 0;
+}
+__device__ __forceinline__ void page_scales(const AttendArgs &p, uint64_t unit, bool there, float *ks, float *vs) {
+    *ks = there ? p.c.k_scale[unit] : 0.0f;
+    float v = there ? p.c.v_scale[unit] : 1.0f;
+    if (v < 0x1p-100f) v = 0x1p-100f;  // log2 and 1 / v stay finite; NaN stays NaN
+    *vs = v;
+}
+// Bytes behind the keys may hold NaN codes, which zero probabilities do not silence: the first `keep` of 16 stay.
+__device__ __forceinline__ void keep_bytes(u32x4 &v, int32_t keep) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int32_t left = keep - 4 * w;
+        v[w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+    }
+}
+
+// Few rows (single tokens, drafts): the workgroup's four wavefronts share 16 * NT rows and split the
+// keys.  Every code is used once, so they go from memory to registers; the cache's bytes bound it.
+template <typename T, int D, int FMT, int NT>
+__global__ __launch_bounds__(256) void k_attend_rows(AttendArgs p, int *err) {
+    typedef Rows<T, D, FMT, NT> R;
+    constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT;
+    __shared__ float join_ml[4][16 * NT][2];
+    __shared__ f32x4 join_acc[3][NT * DT][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t n = lane & 15, g = lane / 16, kvh = blockIdx.y;
+    Tile tile;
+    if (!tile_of(p, 16 * NT, blockIdx.z, err, &tile)) return;
+    R rows;
+    rows.load(p, tile.q, tile.row0, tile.last, kvh);
+
     const uint32_t page_mask = p.c.page_size - 1;
-    const int32_t *table = p.a.block_table + static_cast<uint64_t>(r) * p.a.max_pages;
+    const int32_t *table = p.a.block_table + static_cast<uint64_t>(tile.r) * p.a.max_pages;
     const uint8_t *kc = static_cast<const uint8_t *>(p.c.k), *vc = static_cast<const uint8_t *>(p.c.v);
     const uint32_t kgroup = (lane >> 2) & 3;  // 16-key group whose keys this lane loads for the first product
     bool missing = false;
-
-    for (uint32_t b = SHARED ? b0 + wave : b0; b < b1; b += SHARED ? 4 : 1) {
+    for (uint32_t b = tile.b0 + wave; b < tile.b1; b += 4) {
         const int32_t base = static_cast<int32_t>(64 * b);
-        if (base >= any_hi || base + 64 <= any_lo) continue;
-        // The pages of the two 16-key groups this lane reads; a group without a page, or behind the
-        // keys, reads page 0 and counts as masked.
         const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
-        int32_t page_k = 0, page_v = 0;
-        bool there = false;
-        if (key_k < any_hi) {
-            const int32_t id = table[key_k >> p.page_log2];
-            page_k = id >= 0 && static_cast<uint32_t>(id) < p.c.pages ? id : 0;
-        }
-        if (key_v < any_hi) {
-            const int32_t id = table[key_v >> p.page_log2];
-            there = id >= 0 && static_cast<uint32_t>(id) < p.c.pages;
-            page_v = there ? id : 0;
-            missing |= !there && key_v + 16 > any_lo;
-        }
-        const uint64_t unit_k = static_cast<uint64_t>(page_k) * p.c.kv_heads + kvh;
-        const uint64_t unit_v = static_cast<uint64_t>(page_v) * p.c.kv_heads + kvh;
-        const float ks = there ? p.c.k_scale[unit_v] : 0.0f;
-        float vs = there ? p.c.v_scale[unit_v] : 1.0f;
-        if (vs < 0x1p-100f) vs = 0x1p-100f;  // log2 and 1 / vs stay finite; NaN stays NaN
-
+        bool there, there_k;
+        const uint64_t unit_k = static_cast<uint64_t>(page_at(p, table, key_k, rows.any_hi, &there_k)) * p.c.kv_heads + kvh;
+        const uint64_t unit_v = static_cast<uint64_t>(page_at(p, table, key_v, rows.any_hi, &there)) * p.c.kv_heads + kvh;
+        missing |= !there && key_v < rows.any_hi && key_v + 16 > rows.any_lo;
+        float ks, vs;
+        page_scales(p, unit_v, there, &ks, &vs);
         u32x4 kraw[4][D / 64], vraw[DT];
         const uint8_t *kp = kc + ((unit_k << p.page_log2) + (static_cast<uint32_t>(key_k) & page_mask) + (lane & 3)) * D + g * (D / 4);
 #pragma unroll
@@ -283,19 +391,10 @@ __global__ __launch_bounds__(256) void k_attend(AttendArgs p, int *err) {
         const uint8_t *vp = vc + ((unit_v * D + n) << p.page_log2) + (static_cast<uint32_t>(key_v) & page_mask);
 #pragma unroll
         for (int d = 0; d < DT; ++d) vraw[d] = *reinterpret_cast<const u32x4 *>(vp + (static_cast<uint64_t>(16 * d) << p.page_log2));
-
-        const bool edge = base < all_lo || base + 64 > all_hi || __ballot(there) != ~0ull;
-        if (edge && FMT == kE4m3) {
-            // Bytes behind the keys may hold NaN codes, which zero probabilities do not silence.
-            const int32_t keep = there ? any_hi - key_v : 0;
+        const bool edge = base < rows.all_lo || base + 64 > rows.all_hi || __ballot(there) != ~0ull;
+        if (edge && FMT == kE4m3)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int32_t left = keep - 4 * w;
-                const uint32_t mask = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) vraw[d][w] &= mask;
-            }
-        }
+            for (int d = 0; d < DT; ++d) keep_bytes(vraw[d], there ? rows.any_hi - key_v : 0);
 
         f16x8 pv[LIMBS][NT][2];
         {
@@ -308,48 +407,12 @@ __global__ __launch_bounds__(256) void k_attend(AttendArgs p, int *err) {
                 for (int k = 0; k < KS; ++k) {
                     const f16x8 kv = halves<FMT>(kraw[t][k / 2][2 * (k % 2)], kraw[t][k / 2][2 * (k % 2) + 1]);
 #pragma unroll
-                    for (int u = 0; u < NT; ++u) {
-                        s[u][t] = mfma(kv, qv[0][u][k], s[u][t]);
-                        if constexpr (LIMBS == 2) s[u][t] = mfma(kv, qv[LIMBS - 1][u][k], s[u][t]);
-                    }
+                    for (int u = 0; u < NT; ++u)
+#pragma unroll
+                        for (int i = 0; i < LIMBS; ++i) s[u][t] = mfma(kv, rows.qv[i][u][k], s[u][t]);
                 }
             }
-            const float lv = __builtin_amdgcn_logf(vs), iv = 1.0f / vs;
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const float f = kf[u] * ks;
-                float top = kNone;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float z = __builtin_fmaf(s[u][t][i], f, lv);
-                        if (edge) {
-                            const int32_t key = key_v + 4 * t + i;
-                            z = there && key >= lo[u] && key < hi[u] ? z : kNone;
-                        }
-                        s[u][t][i] = z;
-                        top = fmaxf(top, z);
-                    }
-                const float next = fmaxf(m[u], across_max(top));
-                const float ref = next == kNone ? 0.0f : next;  // a row that has seen no key yet
-                const float alpha = __builtin_amdgcn_exp2f(m[u] - ref);
-                m[u] = next;
-                float sum = 0.0f;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(s[u][t][i] - (ref - kHeadroom));
-                        sum += e;
-                        const _Float16 h = static_cast<_Float16>(e);
-                        pv[0][u][t / 2][4 * (t % 2) + i] = h;
-                        if constexpr (LIMBS == 2) pv[LIMBS - 1][u][t / 2][4 * (t % 2) + i] = static_cast<_Float16>(e - static_cast<float>(h));
-                    }
-                l[u] = __builtin_fmaf(l[u], alpha, sum == 0.0f ? 0.0f : sum * iv);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) acc[u][d] *= alpha;
-            }
+            rows.softmax(s, pv, ks, vs, there, edge, key_v);
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -357,77 +420,176 @@ __global__ __launch_bounds__(256) void k_attend(AttendArgs p, int *err) {
             for (int c = 0; c < 2; ++c) {
                 const f16x8 vv = halves<FMT>(vraw[d][2 * c], vraw[d][2 * c + 1]);
 #pragma unroll
-                for (int u = 0; u < NT; ++u) {
-                    acc[u][d] = mfma(vv, pv[0][u][c], acc[u][d]);
-                    if constexpr (LIMBS == 2) acc[u][d] = mfma(vv, pv[LIMBS - 1][u][c], acc[u][d]);
-                }
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < LIMBS; ++i) rows.acc[u][d] = mfma(vv, pv[i][u][c], rows.acc[u][d]);
             }
     }
     if (missing) raise_error(err, kErrIndex);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) l[t] = across_sum(l[t]);
 
-    if constexpr (SHARED) {
-        // The four wavefronts' rows join in the first.
-        if (g == 0)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                join_ml[wave][16 * t + n][0] = m[t];
-                join_ml[wave][16 * t + n][1] = l[t];
-            }
-        if (wave)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int d = 0; d < DT; ++d) join_acc[wave - 1][t * DT + d][lane] = acc[t][d];
-        __syncthreads();
-        if (wave) return;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float top = m[t];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) top = fmaxf(top, join_ml[w][16 * t + n][0]);
-            const float ref = top == kNone ? 0.0f : top;
-            const float mine = __builtin_amdgcn_exp2f(m[t] - ref);
-            l[t] *= mine;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) acc[t][d] *= mine;
-#pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                const float other = __builtin_amdgcn_exp2f(join_ml[w][16 * t + n][0] - ref);
-                l[t] += other * join_ml[w][16 * t + n][1];
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const f32x4 v = join_acc[w - 1][t * DT + d][lane];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t][d][i] = __builtin_fmaf(v[i], other, acc[t][d][i]);
-                }
-            }
-            m[t] = top;
-        }
-    }
-
-    // Lane (n, g) has dimensions 16 d + 4 g .. + 3 of row n.
-    bool bad = false;
-    const uint64_t all_rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
+    // The four wavefronts' rows join in the first.
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        if (!live[t]) continue;
-        if (parts == 1) {
-            const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+        rows.l[t] = across_sum(rows.l[t]);
+        if (g == 0) {
+            join_ml[wave][16 * t + n][0] = rows.m[t];
+            join_ml[wave][16 * t + n][1] = rows.l[t];
+        }
+        if (wave)
 #pragma unroll
-            for (int d = 0; d < DT; ++d) write_row<T>(p, token[t], head[t], 16 * d + 4 * g, acc[t][d] * inv, &bad);
-        } else {
-            const uint64_t row = split * all_rows + static_cast<uint64_t>(token[t]) * p.a.heads + head[t];
+            for (int d = 0; d < DT; ++d) join_acc[wave - 1][t * DT + d][lane] = rows.acc[t][d];
+    }
+    __syncthreads();
+    if (wave) return;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(p.part + row * D + 16 * d + 4 * g) = acc[t][d];
-            if (g == 0) {
-                p.part_ml[2 * row] = m[t];
-                p.part_ml[2 * row + 1] = l[t];
+    for (int t = 0; t < NT; ++t) {
+        float top = rows.m[t];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, join_ml[w][16 * t + n][0]);
+        const float ref = top == kNone ? 0.0f : top;
+        const float mine = __builtin_amdgcn_exp2f(rows.m[t] - ref);
+        rows.l[t] *= mine;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) rows.acc[t][d] *= mine;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+            const float other = __builtin_amdgcn_exp2f(join_ml[w][16 * t + n][0] - ref);
+            rows.l[t] += other * join_ml[w][16 * t + n][1];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const f32x4 v = join_acc[w - 1][t * DT + d][lane];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rows.acc[t][d][i] = __builtin_fmaf(v[i], other, rows.acc[t][d][i]);
             }
         }
+        rows.m[t] = top;
     }
-    if (bad) raise_error(err, kErrNonfinite);
+    rows.write(p, tile.parts, blockIdx.z, err);
+}
+
+// Many rows (prompts, chunks): each wavefront has 16 * NT rows of its own and all keys.  A block's codes are
+// converted to binary16 once by the workgroup, a quarter by each wavefront, into LDS in the order of the
+// operands (a fragment is 16 consecutive bytes a lane: no bank conflicts); the next block's codes
+// come from memory meanwhile and are converted behind the products, so a block costs one barrier.
+// Converting in every wavefront instead took 1240 us for a prompt of 8192 tokens.
+template <typename T, int D, int FMT, int NT>
+__global__ __launch_bounds__(256) void k_attend_tile(AttendArgs p, int *err) {
+    typedef Rows<T, D, FMT, NT> R;
+    constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT;
+    __shared__ f16x8 kf[2][4][KS][64], vf[2][DT][2][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t n = lane & 15, g = lane / 16, kvh = blockIdx.y;
+    Tile tile;
+    if (!tile_of(p, 64 * NT, blockIdx.z, err, &tile)) return;
+    R rows;
+    rows.load(p, tile.q, min(tile.row0 + wave * 16 * NT, tile.last), tile.last, kvh);
+    const bool idle = tile.row0 + wave * 16 * NT > tile.last;  // converts only
+
+    const uint32_t page_mask = p.c.page_size - 1;
+    const int32_t *table = p.a.block_table + static_cast<uint64_t>(tile.r) * p.a.max_pages;
+    const uint8_t *kc = static_cast<const uint8_t *>(p.c.k), *vc = static_cast<const uint8_t *>(p.c.v);
+    int32_t seen_lo, seen_hi, x;  // keys any row of the tile sees
+    visible(p, tile.q, tile.row0 / p.group, &seen_lo, &x);
+    visible(p, tile.q, tile.last / p.group, &x, &seen_hi);
+    const uint32_t kgroup = (lane >> 2) & 3;
+    bool missing = false;
+
+    // Codes of block b: K's 16-key tile `wave`, and V's dimension tiles wave DT/4 ...
+    u32x4 kraw[D / 64], vraw[DT / 4];
+    float ks = 0.0f, vs = 1.0f, ks_next = 0.0f, vs_next = 1.0f;
+    bool there = false, there_next = false;
+    int32_t id_k = 0, id_v = 0;
+    bool has_v = false;
+    auto look = [&](uint32_t b) {  // the pages of block b
+        const int32_t base = static_cast<int32_t>(64 * b);
+        bool has_k;
+        id_k = page_at(p, table, base + 16 * static_cast<int32_t>(kgroup), seen_hi, &has_k);
+        id_v = page_at(p, table, base + 16 * static_cast<int32_t>(g), seen_hi, &has_v);
+    };
+    auto fetch = [&](uint32_t b) {  // its codes and scales, from the pages that look found
+        const int32_t base = static_cast<int32_t>(64 * b);
+        const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
+        const uint64_t unit_k = static_cast<uint64_t>(id_k) * p.c.kv_heads + kvh, unit_v = static_cast<uint64_t>(id_v) * p.c.kv_heads + kvh;
+        missing |= !has_v && key_v < seen_hi && key_v + 16 > seen_lo;
+        there_next = has_v;
+        page_scales(p, unit_v, has_v, &ks_next, &vs_next);
+        const uint8_t *kp = kc + ((unit_k << p.page_log2) + (static_cast<uint32_t>(key_k) & page_mask) + 4 * wave + (lane & 3)) * D + g * (D / 4);
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) kraw[j] = *reinterpret_cast<const u32x4 *>(kp + 16 * j);
+        const uint8_t *vp = vc + ((unit_v * D + 16 * (DT / 4) * wave + n) << p.page_log2) + (static_cast<uint32_t>(key_v) & page_mask);
+#pragma unroll
+        for (int d = 0; d < DT / 4; ++d) vraw[d] = *reinterpret_cast<const u32x4 *>(vp + (static_cast<uint64_t>(16 * d) << p.page_log2));
+    };
+    auto convert = [&](uint32_t b) {  // into buffer b & 1
+        const uint32_t at = b & 1;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) kf[at][wave][k][lane] = halves<FMT>(kraw[k / 2][2 * (k % 2)], kraw[k / 2][2 * (k % 2) + 1]);
+        if (FMT == kE4m3) {
+            const int32_t left = seen_hi - static_cast<int32_t>(64 * b + 16 * g);
+            if (__ballot(!there_next || left < 16))
+#pragma unroll
+                for (int d = 0; d < DT / 4; ++d) keep_bytes(vraw[d], there_next ? left : 0);
+        }
+#pragma unroll
+        for (int d = 0; d < DT / 4; ++d)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) vf[at][DT / 4 * wave + d][c][lane] = halves<FMT>(vraw[d][2 * c], vraw[d][2 * c + 1]);
+    };
+
+    if (tile.b0 < tile.b1) {
+        look(tile.b0);
+        fetch(tile.b0);
+        if (tile.b0 + 1 < tile.b1) look(tile.b0 + 1);
+        convert(tile.b0);
+    }
+    for (uint32_t b = tile.b0; b < tile.b1; ++b) {
+        __syncthreads();  // block b is in LDS, and every wavefront is done with block b - 1
+        ks = ks_next;
+        vs = vs_next;
+        there = there_next;
+        if (b + 1 < tile.b1) {
+            fetch(b + 1);
+            if (b + 2 < tile.b1) look(b + 2);
+        }
+        const int32_t base = static_cast<int32_t>(64 * b);
+        if (!idle && base < rows.any_hi && base + 64 > rows.any_lo) {
+            const bool edge = base < rows.all_lo || base + 64 > rows.all_hi || __ballot(there) != ~0ull;
+            f16x8 pv[LIMBS][NT][2];
+            {
+                f32x4 s[NT][4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) s[u][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const f16x8 kv = kf[b & 1][t][k][lane];
+#pragma unroll
+                        for (int u = 0; u < NT; ++u)
+#pragma unroll
+                            for (int i = 0; i < LIMBS; ++i) s[u][t] = mfma(kv, rows.qv[i][u][k], s[u][t]);
+                    }
+                }
+                rows.softmax(s, pv, ks, vs, there, edge, base + 16 * static_cast<int32_t>(g));
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const f16x8 vv = vf[b & 1][d][c][lane];
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+#pragma unroll
+                        for (int i = 0; i < LIMBS; ++i) rows.acc[u][d] = mfma(vv, pv[i][u][c], rows.acc[u][d]);
+                }
+        }
+        if (b + 1 < tile.b1) convert(b + 1);
+    }
+    if (missing) raise_error(err, kErrIndex);
+    if (idle) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) rows.l[t] = across_sum(rows.l[t]);
+    rows.write(p, tile.parts, blockIdx.z, err);
 }
 
 // Joins the splits of the rows that have more than one: a wavefront a row, a lane D / 64 dimensions.
@@ -487,7 +649,7 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     const uint64_t typical = (static_cast<uint64_t>(a.tokens) * group + a.requests - 1) / a.requests;  // rows of a request
     Plan p;
     p.shared = typical <= 32;
-    p.nt = c.head_dim == 256 || (p.shared && typical <= 16) ? 1 : 2;
+    p.nt = p.shared && (c.head_dim == 256 || typical <= 16) ? 1 : 2;
     p.M = p.shared ? 16 * p.nt : 64 * p.nt;
     p.slots = static_cast<uint32_t>(static_cast<uint64_t>(a.tokens) * group / p.M) + a.requests;
     // Keys are split until some 1024 workgroups share them.
@@ -502,10 +664,10 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
 template <typename T, int D, int FMT>
 int attend_launch(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s) {
     const dim3 grid(p.slots, p.c.kv_heads, p.splits);
-    constexpr int most = D == 256 ? 1 : 2;
-    if (!plan.shared) k_attend<T, D, FMT, most, false><<<grid, 256, 0, s>>>(p, err);
-    else if (plan.nt == 1) k_attend<T, D, FMT, 1, true><<<grid, 256, 0, s>>>(p, err);
-    else k_attend<T, D, FMT, most, true><<<grid, 256, 0, s>>>(p, err);
+    constexpr int most = D == 256 ? 1 : 2;  // row tiles of the first kernel
+    if (!plan.shared) k_attend_tile<T, D, FMT, 2><<<grid, 256, 0, s>>>(p, err);
+    else if (plan.nt == 1) k_attend_rows<T, D, FMT, 1><<<grid, 256, 0, s>>>(p, err);
+    else k_attend_rows<T, D, FMT, most><<<grid, 256, 0, s>>>(p, err);
     int rc = launch_status();
     if (rc || p.splits == 1) return rc;
     const uint64_t rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;

@@ -171,9 +171,9 @@ def attention(cache, q, offsets, lengths, table, page, scale, causal=True, windo
       p = 2^z: ln 2 * dz, one step of exp (2^-23), and its parts: 2^-22 for two, half a step 2^-11 for one
       sums over n keys: n roundings each, in the numerator and the denominator; six more for joins and the division
     each relative to the term, so against sum p |v| / sum p; and the result's own rounding.
-      The probabilities times their page's value scale are held in binary16 with their largest at 2^14, where the smallest
-      step is 2^-24: a term far below the largest is off by up to half of it, 2^-25 / 2^14 = 2^-39 of the largest p * v_scale
-      for each unit of its code (twice that is allowed), however small the term itself is.
+      The probabilities times their page's value scale are held in binary16 with their largest at 2^11 to 2^15, where the
+      smallest step is 2^-24: a term far below the largest is off by up to half of it, 2^-25 / 2^11 = 2^-36 of the largest
+      p * v_scale for each unit of its code (twice that is allowed), however small the term itself is.
     """
     q = np.asarray(q, np.float64)
     t, heads, d = q.shape
@@ -215,6 +215,6 @@ def attention(cache, q, offsets, lengths, table, page, scale, causal=True, windo
                 got = out[o0 + i, h * g:(h + 1) * g]
                 vs = np.repeat(cache["v_scale"][np.clip(table[r], 0, None), h].astype(np.float64), page)[lo:hi][keep]
                 code = np.abs(vv) / vs[:, None]
-                floor = 2.0 ** -38 * (p * vs).max(1, keepdims=True) * code.sum(0)[None]
+                floor = 2.0 ** -35 * (p * vs).max(1, keepdims=True) * code.sum(0)[None]
                 tol[o0 + i, h * g:(h + 1) * g] = (rel * (p @ np.abs(vv)) + floor) / l + HALF[dtype] * np.abs(got) + TINY[dtype]
     return out, tol * 1.01 + 1e-30
