@@ -13,6 +13,8 @@
 // block are 16 consecutive keys, all of one page: they are the B operand of the second product
 // as they stand (no exchange between lanes), and one 16-byte load of the transposed values
 // is the A operand that meets them.
+#include <type_traits>
+
 #include "serve_common.hpp"
 
 namespace prism {
@@ -31,13 +33,11 @@ struct AttendArgs {
     prism_attention a;
     uint32_t group, page_log2;
     uint32_t slots;     // row tiles, at most (tile_request)
-    uint32_t splits;    // key ranges a request's keys are split into, at most
+    uint32_t each;      // key blocks of 64 a part of a tile's keys has, at least
+    uint32_t splits;    // parts, at most
     float *part;        // [splits][tokens * heads][head_dim] unnormalised rows
     float *part_ml;     // [splits][tokens * heads][2]: maximum (base 2), sum
 };
-
-// Key blocks of 64 a split takes at least: one for each of a workgroup's wavefronts, and one more round.
-constexpr uint32_t kLeastBlocks = 8;
 
 struct Request {
     uint32_t first, n;      // its tokens
@@ -64,8 +64,7 @@ __device__ __forceinline__ void visible(const AttendArgs &p, const Request &q, u
     *hi = at + 1 > 0 ? at + 1 : 0;
     if (p.a.window && at + 1 > static_cast<int64_t>(p.a.window)) *lo = at + 1 - static_cast<int32_t>(p.a.window);
 }
-// The 64-key blocks [b0, b1) any of the request's tokens i0 .. i1 sees, and how many of them a
-// split takes: the same for every tile of the request, so that the join knows the splits in use.
+// The 64-key blocks [b0, b1) any of the request's tokens i0 .. i1 sees, and the parts they are split into.
 __device__ __forceinline__ void blocks_of(const AttendArgs &p, const Request &q, uint32_t i0, uint32_t i1, uint32_t *b0,
                                           uint32_t *b1) {
     int32_t lo, hi, x;
@@ -74,9 +73,12 @@ __device__ __forceinline__ void blocks_of(const AttendArgs &p, const Request &q,
     *b0 = static_cast<uint32_t>(lo) / 64;
     *b1 = hi > lo ? (static_cast<uint32_t>(hi) + 63) / 64 : *b0;
 }
-__device__ __forceinline__ uint32_t split_blocks(const AttendArgs &p, uint32_t blocks) {
-    const uint32_t each = (blocks + p.splits - 1) / p.splits;
-    return each < kLeastBlocks ? kLeastBlocks : each;
+__device__ __forceinline__ uint32_t part_blocks(const AttendArgs &p, uint32_t blocks) {
+    return max(p.each, (blocks + p.splits - 1) / p.splits);
+}
+__device__ __forceinline__ uint32_t parts_of(const AttendArgs &p, uint32_t blocks) {
+    const uint32_t each = part_blocks(p, blocks);
+    return blocks <= each ? 1 : (blocks + each - 1) / each;
 }
 
 // Tiles of M rows: request r has the slots from offsets[r] * group / M + r on, at least as
@@ -131,14 +133,21 @@ __device__ __forceinline__ f16x8 halves(uint32_t a, uint32_t b) {
 
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-__device__ __forceinline__ float across_max(float v) {  // over the four lanes of a row
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+// Over the four lanes of a row: lane groups 0 and 1, 2 and 3 exchange, then the halves of the wavefront.
+__device__ __forceinline__ float across_max(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float across_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
 template <typename T>
 __device__ __forceinline__ void write_row(const AttendArgs &p, uint32_t token, uint32_t head, uint32_t dim, f32x4 v, bool *bad) {
@@ -216,6 +225,7 @@ struct Rows {
             any_lo = min(any_lo, __shfl_xor(any_lo, d));
             any_hi = max(any_hi, __shfl_xor(any_hi, d));
         }
+        all_lo = uniform(all_lo), all_hi = uniform(all_hi), any_lo = uniform(any_lo), any_hi = uniform(any_hi);
     }
 
     // Scores s of the lane's 16 keys from `key` on -> probabilities, the operand of the second product.
@@ -308,12 +318,14 @@ struct Rows {
 struct Tile {
     Request q;
     uint32_t r, row0, last, b0, b1, parts;
+    int32_t seen_lo, seen_hi;  // keys some row sees
 };
 __device__ __forceinline__ bool tile_of(const AttendArgs &p, uint32_t M, uint32_t split, int *err, Tile *t) {
     // Heavy tiles first: a prompt's last rows see the most keys.
     const uint32_t slot = gridDim.x - 1 - blockIdx.x;
     t->r = tile_request(p, slot, M);
     t->q = request_of(p, t->r);
+    t->q.first = uniform(t->q.first), t->q.n = uniform(t->q.n), t->q.length = uniform(t->q.length);
     if (blockIdx.x + blockIdx.y + blockIdx.z == 0)  // offsets out of order may leave a request without a tile
         for (uint32_t i = threadIdx.x; i < p.a.requests; i += blockDim.x)
             if (request_of(p, i).bad) raise_error(err, kErrIndex);
@@ -321,28 +333,30 @@ __device__ __forceinline__ bool tile_of(const AttendArgs &p, uint32_t M, uint32_
     t->row0 = (slot - start) * M;
     if (slot < start || t->row0 >= rows) return false;
     t->last = min(rows, t->row0 + M) - 1;
+    int32_t x;
+    visible(p, t->q, t->row0 / p.group, &t->seen_lo, &x);
+    visible(p, t->q, t->last / p.group, &x, &t->seen_hi);
+    t->seen_lo = uniform(t->seen_lo), t->seen_hi = uniform(t->seen_hi);
     uint32_t b0, b1;
     blocks_of(p, t->q, t->row0 / p.group, t->last / p.group, &b0, &b1);
-    const uint32_t each = split_blocks(p, b1 - b0);
-    t->parts = b1 > b0 ? (b1 - b0 + each - 1) / each : 1;
-    t->b0 = b0 + split * each;
-    t->b1 = min(b1, t->b0 + each);
+    const uint32_t each = part_blocks(p, b1 - b0);
+    t->parts = uniform(parts_of(p, b1 - b0));
+    t->b0 = uniform(b0 + split * each);
+    t->b1 = uniform(min(b1, b0 + (split + 1) * each));
     return split < t->parts;
 }
 
-// The page of 16 keys from `key` on, for a lane that reads them: 0, and not `there`, where the table has
-// none or no row sees them.
-__device__ __forceinline__ int32_t page_at(const AttendArgs &p, const int32_t *table, int32_t key, int32_t end, bool *there) {
-    int32_t id = -1;
-    if (key < end) id = table[key >> p.page_log2];
-    *there = id >= 0 && static_cast<uint32_t>(id) < p.c.pages;
-    return *there ? id : 0;
+// The table's entry for 16 keys from `key` on: their page, where some row sees one of them (key < end) and
+// the entry is a page; else page 0 stands in and they count as masked.  Entries and scales are taken as
+// loaded and looked at where they are used, blocks later.
+__device__ __forceinline__ int32_t entry_at(const AttendArgs &p, const int32_t *table, int32_t key, int32_t end) {
+    return table[min(key, end - 1) >> p.page_log2];
 }
-__device__ __forceinline__ void page_scales(const AttendArgs &p, uint64_t unit, bool there, float *ks, float *vs) {
-    *ks = there ? p.c.k_scale[unit] : 0.0f;
-    float v = there ? p.c.v_scale[unit] : 1.0f;
-    if (v < 0x1p-100f) v = 0x1p-100f;  // log2 and 1 / v stay finite; NaN stays NaN
-    *vs = v;
+__device__ __forceinline__ bool is_page(const AttendArgs &p, int32_t id, int32_t key, int32_t end) {
+    return key < end && static_cast<uint32_t>(id) < p.c.pages;
+}
+__device__ __forceinline__ float value_scale(float v, bool there) {  // log2 and 1 / v stay finite; NaN stays NaN
+    return !there ? 1.0f : v < 0x1p-100f ? 0x1p-100f : v;
 }
 // Bytes behind the keys may hold NaN codes, which zero probabilities do not silence: the first `keep` of 16 stay.
 __device__ __forceinline__ void keep_bytes(u32x4 &v, int32_t keep) {
@@ -355,8 +369,10 @@ __device__ __forceinline__ void keep_bytes(u32x4 &v, int32_t keep) {
 
 // Few rows (single tokens, drafts): the workgroup's four wavefronts share 16 * NT rows and split the
 // keys.  Every code is used once, so they go from memory to registers; the cache's bytes bound it.
-template <typename T, int D, int FMT, int NT>
-__global__ __launch_bounds__(256) void k_attend_rows(AttendArgs p, int *err) {
+// WIDE: byte offsets into the keys or values pass 32 bits; else a lane's address is one register
+// beside a scalar base.
+template <typename T, int D, int FMT, int NT, bool WIDE>
+__global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_attend_rows(AttendArgs p, int *err) {
     typedef Rows<T, D, FMT, NT> R;
     constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT;
     __shared__ float join_ml[4][16 * NT][2];
@@ -365,55 +381,87 @@ __global__ __launch_bounds__(256) void k_attend_rows(AttendArgs p, int *err) {
     const uint32_t n = lane & 15, g = lane / 16, kvh = blockIdx.y;
     Tile tile;
     if (!tile_of(p, 16 * NT, blockIdx.z, err, &tile)) return;
-    R rows;
-    rows.load(p, tile.q, tile.row0, tile.last, kvh);
-
     const uint32_t page_mask = p.c.page_size - 1;
     const int32_t *table = p.a.block_table + static_cast<uint64_t>(tile.r) * p.a.max_pages;
     const uint8_t *kc = static_cast<const uint8_t *>(p.c.k), *vc = static_cast<const uint8_t *>(p.c.v);
     const uint32_t kgroup = (lane >> 2) & 3;  // 16-key group whose keys this lane loads for the first product
-    bool missing = false;
-    for (uint32_t b = tile.b0 + wave; b < tile.b1; b += 4) {
+    // Registers of codes are filled again as soon as a product has used them, the next block's keys behind the
+    // first product and its values behind the second; its table entries are a block further ahead.
+    // Heads of 256 have no registers for that (spilled, 205 us instead of 153 for eight long requests):
+    // their codes are loaded at the block's start, two wavefronts a SIMD covering each other.
+    constexpr bool kAhead = D < 256;
+    int32_t id_k = 0, id_v = 0;
+    u32x4 kraw[4][D / 64], vraw[DT];
+    typedef std::conditional_t<WIDE, uint64_t, uint32_t> Offset;
+    Offset v_at = 0;
+    float ks_next = 0.0f, vs_next = 1.0f;
+    bool there_next = false, missing = false;
+    auto look = [&](uint32_t b) {
+        const int32_t base = static_cast<int32_t>(64 * b);
+        id_k = entry_at(p, table, base + 16 * static_cast<int32_t>(kgroup), tile.seen_hi);
+        id_v = entry_at(p, table, base + 16 * static_cast<int32_t>(g), tile.seen_hi);
+    };
+    auto fetch_keys = [&](uint32_t b) {
         const int32_t base = static_cast<int32_t>(64 * b);
         const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
-        bool there, there_k;
-        const uint64_t unit_k = static_cast<uint64_t>(page_at(p, table, key_k, rows.any_hi, &there_k)) * p.c.kv_heads + kvh;
-        const uint64_t unit_v = static_cast<uint64_t>(page_at(p, table, key_v, rows.any_hi, &there)) * p.c.kv_heads + kvh;
-        missing |= !there && key_v < rows.any_hi && key_v + 16 > rows.any_lo;
-        float ks, vs;
-        page_scales(p, unit_v, there, &ks, &vs);
-        u32x4 kraw[4][D / 64], vraw[DT];
-        const uint8_t *kp = kc + ((unit_k << p.page_log2) + (static_cast<uint32_t>(key_k) & page_mask) + (lane & 3)) * D + g * (D / 4);
+        there_next = is_page(p, id_v, key_v, tile.seen_hi);
+        missing |= !there_next && key_v < tile.seen_hi && key_v + 16 > tile.seen_lo;
+        const Offset unit_k = static_cast<Offset>(is_page(p, id_k, key_k, tile.seen_hi) ? id_k : 0) * p.c.kv_heads + kvh;
+        const Offset unit_v = static_cast<Offset>(there_next ? id_v : 0) * p.c.kv_heads + kvh;
+        ks_next = p.c.k_scale[unit_v];
+        vs_next = p.c.v_scale[unit_v];
+        const Offset k_at = ((unit_k << p.page_log2) + (static_cast<uint32_t>(key_k) & page_mask) + (lane & 3)) * D + g * (D / 4);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j) kraw[t][j] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * D + 16 * j);
-        const uint8_t *vp = vc + ((unit_v * D + n) << p.page_log2) + (static_cast<uint32_t>(key_v) & page_mask);
+            for (int j = 0; j < D / 64; ++j) kraw[t][j] = *reinterpret_cast<const u32x4 *>(kc + k_at + (4 * t * D + 16 * j));
+        v_at = ((unit_v * D + n) << p.page_log2) + (static_cast<uint32_t>(key_v) & page_mask);
+    };
+    auto fetch_values = [&] {
 #pragma unroll
-        for (int d = 0; d < DT; ++d) vraw[d] = *reinterpret_cast<const u32x4 *>(vp + (static_cast<uint64_t>(16 * d) << p.page_log2));
+        for (int d = 0; d < DT; ++d)
+            vraw[d] = *reinterpret_cast<const u32x4 *>(vc + (static_cast<uint64_t>(16 * d) << p.page_log2) + v_at);
+    };
+    const uint32_t first = tile.b0 + wave;
+    if (first < tile.b1) look(first);
+    R rows;
+    rows.load(p, tile.q, tile.row0, tile.last, kvh);
+    if (kAhead && first < tile.b1) {
+        fetch_keys(first);
+        fetch_values();
+        if (first + 4 < tile.b1) look(first + 4);
+    }
+    for (uint32_t b = first; b < tile.b1; b += 4) {
+        if constexpr (!kAhead) {
+            fetch_keys(b);
+            fetch_values();
+            if (b + 4 < tile.b1) look(b + 4);
+        }
+        const int32_t base = static_cast<int32_t>(64 * b), key = base + 16 * static_cast<int32_t>(g);
+        const bool there = there_next;
+        const float ks = there ? ks_next : 0.0f, vs = value_scale(vs_next, there);
         const bool edge = base < rows.all_lo || base + 64 > rows.all_hi || __ballot(there) != ~0ull;
+        f32x4 s[NT][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u) s[u][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const f16x8 kv = halves<FMT>(kraw[t][k / 2][2 * (k % 2)], kraw[t][k / 2][2 * (k % 2) + 1]);
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < LIMBS; ++i) s[u][t] = mfma(kv, rows.qv[i][u][k], s[u][t]);
+            }
+        }
+        const bool more = kAhead && b + 4 < tile.b1;
+        if (more) fetch_keys(b + 4);
+        f16x8 pv[LIMBS][NT][2];
+        rows.softmax(s, pv, ks, vs, there, edge, key);
         if (edge && FMT == kE4m3)
 #pragma unroll
-            for (int d = 0; d < DT; ++d) keep_bytes(vraw[d], there ? rows.any_hi - key_v : 0);
-
-        f16x8 pv[LIMBS][NT][2];
-        {
-            f32x4 s[NT][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                for (int u = 0; u < NT; ++u) s[u][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const f16x8 kv = halves<FMT>(kraw[t][k / 2][2 * (k % 2)], kraw[t][k / 2][2 * (k % 2) + 1]);
-#pragma unroll
-                    for (int u = 0; u < NT; ++u)
-#pragma unroll
-                        for (int i = 0; i < LIMBS; ++i) s[u][t] = mfma(kv, rows.qv[i][u][k], s[u][t]);
-                }
-            }
-            rows.softmax(s, pv, ks, vs, there, edge, key_v);
-        }
+            for (int d = 0; d < DT; ++d) keep_bytes(vraw[d], there ? tile.seen_hi - key : 0);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -424,6 +472,10 @@ __global__ __launch_bounds__(256) void k_attend_rows(AttendArgs p, int *err) {
 #pragma unroll
                     for (int i = 0; i < LIMBS; ++i) rows.acc[u][d] = mfma(vv, pv[i][u][c], rows.acc[u][d]);
             }
+        if (more) {
+            fetch_values();
+            if (b + 8 < tile.b1) look(b + 8);
+        }
     }
     if (missing) raise_error(err, kErrIndex);
 
@@ -473,7 +525,7 @@ __global__ __launch_bounds__(256) void k_attend_rows(AttendArgs p, int *err) {
 // come from memory meanwhile and are converted behind the products, so a block costs one barrier.
 // Converting in every wavefront instead took 1240 us for a prompt of 8192 tokens.
 template <typename T, int D, int FMT, int NT>
-__global__ __launch_bounds__(256) void k_attend_tile(AttendArgs p, int *err) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArgs p, int *err) {
     typedef Rows<T, D, FMT, NT> R;
     constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT;
     __shared__ f16x8 kf[2][4][KS][64], vf[2][DT][2][64];
@@ -488,31 +540,29 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs p, int *err) {
     const uint32_t page_mask = p.c.page_size - 1;
     const int32_t *table = p.a.block_table + static_cast<uint64_t>(tile.r) * p.a.max_pages;
     const uint8_t *kc = static_cast<const uint8_t *>(p.c.k), *vc = static_cast<const uint8_t *>(p.c.v);
-    int32_t seen_lo, seen_hi, x;  // keys any row of the tile sees
-    visible(p, tile.q, tile.row0 / p.group, &seen_lo, &x);
-    visible(p, tile.q, tile.last / p.group, &x, &seen_hi);
+    const int32_t seen_lo = tile.seen_lo, seen_hi = tile.seen_hi;
     const uint32_t kgroup = (lane >> 2) & 3;
     bool missing = false;
 
     // Codes of block b: K's 16-key tile `wave`, and V's dimension tiles wave DT/4 ...
     u32x4 kraw[D / 64], vraw[DT / 4];
-    float ks = 0.0f, vs = 1.0f, ks_next = 0.0f, vs_next = 1.0f;
-    bool there = false, there_next = false;
+    float ks_next = 0.0f, vs_next = 1.0f;
+    bool there_next = false;
     int32_t id_k = 0, id_v = 0;
-    bool has_v = false;
-    auto look = [&](uint32_t b) {  // the pages of block b
+    auto look = [&](uint32_t b) {  // the table's entries of block b
         const int32_t base = static_cast<int32_t>(64 * b);
-        bool has_k;
-        id_k = page_at(p, table, base + 16 * static_cast<int32_t>(kgroup), seen_hi, &has_k);
-        id_v = page_at(p, table, base + 16 * static_cast<int32_t>(g), seen_hi, &has_v);
+        id_k = entry_at(p, table, base + 16 * static_cast<int32_t>(kgroup), seen_hi);
+        id_v = entry_at(p, table, base + 16 * static_cast<int32_t>(g), seen_hi);
     };
     auto fetch = [&](uint32_t b) {  // its codes and scales, from the pages that look found
         const int32_t base = static_cast<int32_t>(64 * b);
         const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
-        const uint64_t unit_k = static_cast<uint64_t>(id_k) * p.c.kv_heads + kvh, unit_v = static_cast<uint64_t>(id_v) * p.c.kv_heads + kvh;
-        missing |= !has_v && key_v < seen_hi && key_v + 16 > seen_lo;
-        there_next = has_v;
-        page_scales(p, unit_v, has_v, &ks_next, &vs_next);
+        there_next = is_page(p, id_v, key_v, seen_hi);
+        missing |= !there_next && key_v < seen_hi && key_v + 16 > seen_lo;
+        const uint64_t unit_k = static_cast<uint64_t>(is_page(p, id_k, key_k, seen_hi) ? id_k : 0) * p.c.kv_heads + kvh;
+        const uint64_t unit_v = static_cast<uint64_t>(there_next ? id_v : 0) * p.c.kv_heads + kvh;
+        ks_next = p.c.k_scale[unit_v];
+        vs_next = p.c.v_scale[unit_v];
         const uint8_t *kp = kc + ((unit_k << p.page_log2) + (static_cast<uint32_t>(key_k) & page_mask) + 4 * wave + (lane & 3)) * D + g * (D / 4);
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) kraw[j] = *reinterpret_cast<const u32x4 *>(kp + 16 * j);
@@ -544,9 +594,8 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs p, int *err) {
     }
     for (uint32_t b = tile.b0; b < tile.b1; ++b) {
         __syncthreads();  // block b is in LDS, and every wavefront is done with block b - 1
-        ks = ks_next;
-        vs = vs_next;
-        there = there_next;
+        const bool there = there_next;
+        const float ks = there ? ks_next : 0.0f, vs = value_scale(vs_next, there);
         if (b + 1 < tile.b1) {
             fetch(b + 1);
             if (b + 2 < tile.b1) look(b + 2);
@@ -556,31 +605,30 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs p, int *err) {
             const bool edge = base < rows.all_lo || base + 64 > rows.all_hi || __ballot(there) != ~0ull;
             f16x8 pv[LIMBS][NT][2];
             {
+                // Products of one step of dimensions, four key tiles by NT row tiles, do not wait for each other.
                 f32x4 s[NT][4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
+                for (int k = 0; k < KS; ++k)
 #pragma unroll
-                    for (int u = 0; u < NT; ++u) s[u][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int k = 0; k < KS; ++k) {
+                    for (int t = 0; t < 4; ++t) {
                         const f16x8 kv = kf[b & 1][t][k][lane];
 #pragma unroll
-                        for (int u = 0; u < NT; ++u)
+                        for (int i = 0; i < LIMBS; ++i)
 #pragma unroll
-                            for (int i = 0; i < LIMBS; ++i) s[u][t] = mfma(kv, rows.qv[i][u][k], s[u][t]);
+                            for (int u = 0; u < NT; ++u)
+                                s[u][t] = mfma(kv, rows.qv[i][u][k], k || i ? s[u][t] : f32x4{0, 0, 0, 0});
                     }
-                }
                 rows.softmax(s, pv, ks, vs, there, edge, base + 16 * static_cast<int32_t>(g));
             }
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int d = 0; d < DT; ++d) {
                     const f16x8 vv = vf[b & 1][d][c][lane];
 #pragma unroll
-                    for (int u = 0; u < NT; ++u)
+                    for (int i = 0; i < LIMBS; ++i)
 #pragma unroll
-                        for (int i = 0; i < LIMBS; ++i) rows.acc[u][d] = mfma(vv, pv[i][u][c], rows.acc[u][d]);
+                        for (int u = 0; u < NT; ++u) rows.acc[u][d] = mfma(vv, pv[i][u][c], rows.acc[u][d]);
                 }
         }
         if (b + 1 < tile.b1) convert(b + 1);
@@ -592,11 +640,14 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs p, int *err) {
     rows.write(p, tile.parts, blockIdx.z, err);
 }
 
-// Joins the splits of the rows that have more than one: a wavefront a row, a lane D / 64 dimensions.
-template <typename T, int D>
+// Joins the parts of the rows that have more than one: WAVES wavefronts a row, which share its parts, a lane
+// with D / 64 dimensions; four parts in flight each.
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, int *err) {
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + threadIdx.x / 64, all_rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
-    const uint32_t lane = threadIdx.x & 63;
+    constexpr int E = D / 64;
+    __shared__ float join[WAVES > 1 ? 4 : 1][D + 1];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, mine = wave % WAVES;
+    const uint64_t row = uniform(blockIdx.x * (4 / WAVES) + wave / WAVES), all_rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
     if (row >= all_rows) return;
     const uint32_t token = static_cast<uint32_t>(row / p.a.heads), head = static_cast<uint32_t>(row % p.a.heads);
     // The request of the token, 64 candidates at a time.
@@ -608,40 +659,74 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
         n = min(step, n - j * step);
         lo += j * step;
     }
-    const uint32_t r = __builtin_amdgcn_readfirstlane(lo);
+    const uint32_t r = uniform(lo);
     const Request q = request_of(p, r);
     if (token < q.first || token >= q.first + q.n) return;
     const uint32_t rows = q.n * p.group, row0 = ((token - q.first) * p.group + head % p.group) / M * M, last = min(rows, row0 + M) - 1;
     uint32_t b0, b1;
     blocks_of(p, q, row0 / p.group, last / p.group, &b0, &b1);
-    const uint32_t each = split_blocks(p, b1 - b0), parts = (b1 - b0 + each - 1) / each;
+    const uint32_t parts = uniform(parts_of(p, b1 - b0));
     if (parts <= 1) return;
     float top = kNone;
-    for (uint32_t s = 0; s < parts; ++s) top = fmaxf(top, p.part_ml[2 * (s * all_rows + row)]);
-    const float ref = top == kNone ? 0.0f : top;
-    float l = 0.0f, acc[D / 64] = {};
-    for (uint32_t s = 0; s < parts; ++s) {
-        const uint64_t at = s * all_rows + row;
-        const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - ref);
-        l = __builtin_fmaf(p.part_ml[2 * at + 1], f, l);
+    for (uint32_t s = lane; s < parts; s += 64) top = fmaxf(top, p.part_ml[2 * (s * all_rows + row)]);
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) acc[i] = __builtin_fmaf(p.part[at * D + lane + 64 * i], f, acc[i]);
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float ref = top == kNone ? 0.0f : top;
+    float l = 0.0f, acc[E] = {};
+    for (uint32_t s0 = 4 * mine; s0 < parts; s0 += 4 * WAVES) {
+        float f[4], pl[4], v[4][E];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            const uint64_t at = min(s0 + u, parts - 1) * all_rows + row;
+            f[u] = p.part_ml[2 * at];
+            pl[u] = p.part_ml[2 * at + 1];
+            __builtin_memcpy(v[u], p.part + at * D + E * lane, sizeof v[u]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            const float w = s0 + u < parts ? __builtin_amdgcn_exp2f(f[u] - ref) : 0.0f;
+            // A part no key of which the row sees has sums of zero; those of a duplicate count for nothing.
+            if (s0 + u < parts) {
+                l = __builtin_fmaf(pl[u], w, l);
+#pragma unroll
+                for (int i = 0; i < E; ++i) acc[i] = __builtin_fmaf(v[u][i], w, acc[i]);
+            }
+        }
+    }
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) join[wave][E * lane + i] = acc[i];
+        if (lane == 0) join[wave][D] = l;
+        __syncthreads();
+        if (mine) return;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            l += join[w][D];
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[i] += join[w][E * lane + i];
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     bool bad = false;
-    T *out = static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * D;
+    T *out = static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * D + E * lane;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
+    for (int i = 0; i < E; ++i) {
         const float v = acc[i] * inv;
         bad |= !finite(v);
-        out[lane + 64 * i] = static_cast<T>(v);
+        out[i] = static_cast<T>(v);
     }
     if (bad) raise_error(err, kErrNonfinite);
 }
 
+// Workgroups a CU gets at most, and key blocks a part has at least, in the kernels for few and for many rows.
+constexpr uint32_t kWantedRows = 8, kLeastRows = 8, kWantedTiles = 4, kLeastTiles = 8;
+
 // How a call runs: rows a workgroup takes, whether its wavefronts share them, and the most splits.
 struct Plan {
-    uint32_t nt, M, slots, splits;
+    uint32_t nt, M, slots, each, splits;
     bool shared;
 };
 Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus) {
@@ -652,26 +737,32 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     p.nt = p.shared && (c.head_dim == 256 || typical <= 16) ? 1 : 2;
     p.M = p.shared ? 16 * p.nt : 64 * p.nt;
     p.slots = static_cast<uint32_t>(static_cast<uint64_t>(a.tokens) * group / p.M) + a.requests;
-    // Keys are split until some 1024 workgroups share them.
-    const uint64_t tiles = static_cast<uint64_t>(p.slots) * c.kv_heads, want = 4ull * cus;
-    const uint32_t most = (a.max_length / 64 + kLeastBlocks) / kLeastBlocks;
-    uint64_t splits = tiles >= want ? 1 : want / tiles;
-    if (splits > most) splits = most;
-    p.splits = splits < 1 ? 1 : static_cast<uint32_t>(splits);
+    // Parts of equal size, so that long requests among short ones do not finish last: as many as
+    // would make `wanted` workgroups a CU were every request as long as max_length.
+    const uint64_t tiles = static_cast<uint64_t>(p.slots) * c.kv_heads, blocks = a.max_length / 64 + 1;
+    const uint32_t wanted = p.shared ? kWantedRows : kWantedTiles, least = p.shared ? kLeastRows : kLeastTiles;
+    uint64_t each = tiles * blocks / (static_cast<uint64_t>(wanted) * cus);
+    each = each < least ? least : each > blocks ? blocks : each;
+    p.each = static_cast<uint32_t>(each + 3) / 4 * 4;
+    p.splits = static_cast<uint32_t>((blocks + p.each - 1) / p.each);
     return p;
 }
 
 template <typename T, int D, int FMT>
 int attend_launch(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s) {
     const dim3 grid(p.slots, p.c.kv_heads, p.splits);
-    constexpr int most = D == 256 ? 1 : 2;  // row tiles of the first kernel
+    constexpr int most = D == 256 ? 1 : 2;  // row tiles of the kernel for few rows
+    const bool wide = static_cast<uint64_t>(p.c.pages) * p.c.page_size * p.c.kv_heads * D > 0xffffffffull;
     if (!plan.shared) k_attend_tile<T, D, FMT, 2><<<grid, 256, 0, s>>>(p, err);
-    else if (plan.nt == 1) k_attend_rows<T, D, FMT, 1><<<grid, 256, 0, s>>>(p, err);
-    else k_attend_rows<T, D, FMT, most><<<grid, 256, 0, s>>>(p, err);
+    else if (wide && plan.nt == 1) k_attend_rows<T, D, FMT, 1, true><<<grid, 256, 0, s>>>(p, err);
+    else if (wide) k_attend_rows<T, D, FMT, most, true><<<grid, 256, 0, s>>>(p, err);
+    else if (plan.nt == 1) k_attend_rows<T, D, FMT, 1, false><<<grid, 256, 0, s>>>(p, err);
+    else k_attend_rows<T, D, FMT, most, false><<<grid, 256, 0, s>>>(p, err);
     int rc = launch_status();
     if (rc || p.splits == 1) return rc;
     const uint64_t rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
-    k_attend_join<T, D><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, s>>>(p, plan.M, err);
+    if (p.splits > 8) k_attend_join<T, D, 4><<<static_cast<uint32_t>(rows), 256, 0, s>>>(p, plan.M, err);
+    else k_attend_join<T, D, 1><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, s>>>(p, plan.M, err);
     return launch_status();
 }
 template <typename T, int D>
@@ -697,7 +788,7 @@ size_t attention_scratch_bytes(const prism_kv_cache &c, const prism_attention &a
 
 int launch_attention_paged(const prism_kv_cache &c, const prism_attention &a, void *scratch, uint32_t cus, int *err, hipStream_t s) {
     const Plan plan = attend_plan(c, a, cus);
-    AttendArgs p{c, a, a.heads / c.kv_heads, 0, plan.slots, plan.splits, static_cast<float *>(scratch), nullptr};
+    AttendArgs p{c, a, a.heads / c.kv_heads, 0, plan.slots, plan.each, plan.splits, static_cast<float *>(scratch), nullptr};
     p.page_log2 = static_cast<uint32_t>(__builtin_ctz(c.page_size));
     p.part_ml = p.part + static_cast<size_t>(plan.splits) * a.tokens * a.heads * c.head_dim;
     if (a.dtype == PRISM_DTYPE_F32) return attend_headed<float>(p, plan, err, s);
