@@ -721,9 +721,6 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
     if (bad) raise_error(err, kErrNonfinite);
 }
 
-// Workgroups a CU gets at most, and key blocks a part has at least, in the kernels for few and for many rows.
-constexpr uint32_t kWantedRows = 8, kLeastRows = 8, kWantedTiles = 4, kLeastTiles = 8;
-
 // How a call runs: rows a workgroup takes, whether its wavefronts share them, and the most splits.
 struct Plan {
     uint32_t nt, M, slots, each, splits;
@@ -737,13 +734,30 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     p.nt = p.shared && (c.head_dim == 256 || typical <= 16) ? 1 : 2;
     p.M = p.shared ? 16 * p.nt : 64 * p.nt;
     p.slots = static_cast<uint32_t>(static_cast<uint64_t>(a.tokens) * group / p.M) + a.requests;
-    // Parts of equal size, so that long requests among short ones do not finish last: as many as
-    // would make `wanted` workgroups a CU were every request as long as max_length.
-    const uint64_t tiles = static_cast<uint64_t>(p.slots) * c.kv_heads, blocks = a.max_length / 64 + 1;
-    const uint32_t wanted = p.shared ? kWantedRows : kWantedTiles, least = p.shared ? kLeastRows : kLeastTiles;
-    uint64_t each = tiles * blocks / (static_cast<uint64_t>(wanted) * cus);
-    each = each < least ? least : each > blocks ? blocks : each;
-    p.each = static_cast<uint32_t>(each + 3) / 4 * 4;
+    uint64_t longest = a.max_length;
+    if (a.window && longest > a.window + p.M / group) longest = a.window + p.M / group;  // what a tile sees of it
+    const uint64_t tiles = static_cast<uint64_t>(p.slots) * c.kv_heads, blocks = longest / 64 + 1;
+    uint64_t parts;
+    if (p.shared) {
+        // Some eight workgroups a CU were every request as long as max_length, so that long requests among
+        // short ones do not finish last; eight blocks a part at least, two for each wavefront.  A batch of 64
+        // requests up to 8192 keys took 171 us unsplit, with 4 / 8 / 16 / 32 workgroups 140 / 135 / 134 / 140;
+        // eight requests up to 65536 keys 168 / 153 / 163 / 173.
+        parts = (blocks + 7) / 8;
+        if (parts > 8ull * cus / tiles) parts = 8ull * cus / tiles;
+    } else {
+        // A part writes and reads its rows' sums, as long as five blocks take, so parts have 24 blocks or more
+        // (32 blocks a tile: 89 us whole, 111 in parts of 16) until the chip is full, and then up to eight
+        // workgroups a CU (79 blocks on 480 tiles: 267 / 241 / 210 us in parts of 76 / 40 / 20), eight
+        // blocks where the tiles leave CUs idle.
+        parts = blocks / 24;
+        if (parts > 8ull * cus / tiles) parts = 8ull * cus / tiles;
+        uint64_t fill = 2ull * cus / tiles;
+        if (fill > blocks / 8) fill = blocks / 8;
+        if (parts < fill) parts = fill;
+    }
+    if (parts < 1) parts = 1;
+    p.each = static_cast<uint32_t>((blocks + parts - 1) / parts);
     p.splits = static_cast<uint32_t>((blocks + p.each - 1) / p.each);
     return p;
 }
