@@ -228,11 +228,11 @@ struct Rows {
         all_lo = uniform(all_lo), all_hi = uniform(all_hi), any_lo = uniform(any_lo), any_hi = uniform(any_hi);
     }
 
-    // Scores s of the lane's 16 keys from `key` on -> probabilities, the operand of the second product.
+    // Scores s of the lane's 16 keys from `key` on are masked and the statistics follow their maximum; p = 2^(s ff + off).
     // ks, vs: the scales of their page; edge: some row does not see some key of the block.
-    __device__ __forceinline__ void softmax(f32x4 (&s)[NT][4], f16x8 (&pv)[LIMBS][NT][2], float ks, float vs, bool there, bool edge,
-                                            int32_t key) {
-        const float lv = __builtin_amdgcn_logf(vs), iv = 1.0f / vs;
+    __device__ __forceinline__ void scores(f32x4 (&s)[NT][4], float ks, float vs, bool there, bool edge, int32_t key, float (&ff)[NT],
+                                           float (&off)[NT]) {
+        const float lv = __builtin_amdgcn_logf(vs);
         float f[NT], top[NT];
         bool grows = false;
 #pragma unroll
@@ -269,22 +269,30 @@ struct Rows {
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
             // A row that has seen no key yet has m = -inf, and scores of -inf.
-            const float off = lv + kHeadroom - (m[u] == kNone ? 0.0f : m[u]);
+            off[u] = lv + kHeadroom - (m[u] == kNone ? 0.0f : m[u]);
             // 0 * -inf would be NaN where a page's keys are all zero and a key is masked.
-            const float ff = f[u] < 0x1p-120f ? 0x1p-120f : f[u];
-            float sum = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][t][i], ff, off));
-                    sum += e;
-                    const _Float16 h = static_cast<_Float16>(e);
-                    pv[0][u][t / 2][4 * (t % 2) + i] = h;
-                    if constexpr (LIMBS == 2) pv[LIMBS - 1][u][t / 2][4 * (t % 2) + i] = static_cast<_Float16>(e - static_cast<float>(h));
-                }
-            l[u] += sum == 0.0f ? 0.0f : sum * iv;
+            ff[u] = f[u] < 0x1p-120f ? 0x1p-120f : f[u];
         }
+    }
+    // Probabilities of half `c` of the keys: an operand of the second product.
+    template <int c>
+    __device__ __forceinline__ void probabilities(const f32x4 (&s)[NT][4], f16x8 (&pv)[LIMBS][NT], const float (&ff)[NT],
+                                                  const float (&off)[NT], float (&sum)[NT]) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][2 * c + j / 4][j % 4], ff[u], off[u]));
+                sum[u] += e;
+                const _Float16 h = static_cast<_Float16>(e);
+                pv[0][u][j] = h;
+                if constexpr (LIMBS == 2) pv[LIMBS - 1][u][j] = static_cast<_Float16>(e - static_cast<float>(h));
+            }
+    }
+    __device__ __forceinline__ void add(const float (&sum)[NT], float vs) {
+        const float iv = 1.0f / vs;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) l[u] += sum[u] == 0.0f ? 0.0f : sum[u] * iv;
     }
 
     // The rows, or with more than one part their unnormalised sums: lane (n, g) has the dimensions
@@ -317,16 +325,18 @@ struct Rows {
 // A workgroup's tile: its request, rows and part of the key blocks; false: nothing to do.
 struct Tile {
     Request q;
-    uint32_t r, row0, last, b0, b1, parts;
+    uint32_t kvh, r, row0, last, b0, b1, parts;
     int32_t seen_lo, seen_hi;  // keys some row sees
 };
 __device__ __forceinline__ bool tile_of(const AttendArgs &p, uint32_t M, uint32_t split, int *err, Tile *t) {
-    // Heavy tiles first: a prompt's last rows see the most keys.
-    const uint32_t slot = gridDim.x - 1 - blockIdx.x;
+    // Heavy tiles first (a prompt's last rows see the most keys), all heads' of them: the other order left the last
+    // head's longest tiles for the end.  With eight kv heads each XCD's L2 also has one head's keys.
+    t->kvh = uniform(blockIdx.x % p.c.kv_heads);
+    const uint32_t slot = uniform(p.slots - 1 - blockIdx.x / p.c.kv_heads);
     t->r = tile_request(p, slot, M);
     t->q = request_of(p, t->r);
     t->q.first = uniform(t->q.first), t->q.n = uniform(t->q.n), t->q.length = uniform(t->q.length);
-    if (blockIdx.x + blockIdx.y + blockIdx.z == 0)  // offsets out of order may leave a request without a tile
+    if (blockIdx.x + blockIdx.z == 0)  // offsets out of order may leave a request without a tile
         for (uint32_t i = threadIdx.x; i < p.a.requests; i += blockDim.x)
             if (request_of(p, i).bad) raise_error(err, kErrIndex);
     const uint32_t rows = t->q.n * p.group, start = tile_start(p, t->r, M);
@@ -378,9 +388,10 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
     __shared__ float join_ml[4][16 * NT][2];
     __shared__ f32x4 join_acc[3][NT * DT][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t n = lane & 15, g = lane / 16, kvh = blockIdx.y;
+    const uint32_t n = lane & 15, g = lane / 16;
     Tile tile;
     if (!tile_of(p, 16 * NT, blockIdx.z, err, &tile)) return;
+    const uint32_t kvh = tile.kvh;
     const uint32_t page_mask = p.c.page_size - 1;
     const int32_t *table = p.a.block_table + static_cast<uint64_t>(tile.r) * p.a.max_pages;
     const uint8_t *kc = static_cast<const uint8_t *>(p.c.k), *vc = static_cast<const uint8_t *>(p.c.v);
@@ -457,8 +468,12 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
         }
         const bool more = kAhead && b + 4 < tile.b1;
         if (more) fetch_keys(b + 4);
-        f16x8 pv[LIMBS][NT][2];
-        rows.softmax(s, pv, ks, vs, there, edge, key);
+        f16x8 pv[2][LIMBS][NT];
+        float ff[NT], off[NT], sum[NT] = {};
+        rows.scores(s, ks, vs, there, edge, key, ff, off);
+        rows.template probabilities<0>(s, pv[0], ff, off, sum);
+        rows.template probabilities<1>(s, pv[1], ff, off, sum);
+        rows.add(sum, vs);
         if (edge && FMT == kE4m3)
 #pragma unroll
             for (int d = 0; d < DT; ++d) keep_bytes(vraw[d], there ? tile.seen_hi - key : 0);
@@ -470,7 +485,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
 #pragma unroll
-                    for (int i = 0; i < LIMBS; ++i) rows.acc[u][d] = mfma(vv, pv[i][u][c], rows.acc[u][d]);
+                    for (int i = 0; i < LIMBS; ++i) rows.acc[u][d] = mfma(vv, pv[c][i][u], rows.acc[u][d]);
             }
         if (more) {
             fetch_values();
@@ -530,9 +545,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
     constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT;
     __shared__ f16x8 kf[2][4][KS][64], vf[2][DT][2][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t n = lane & 15, g = lane / 16, kvh = blockIdx.y;
+    const uint32_t n = lane & 15, g = lane / 16;
     Tile tile;
     if (!tile_of(p, 64 * NT, blockIdx.z, err, &tile)) return;
+    const uint32_t kvh = tile.kvh;
     R rows;
     rows.load(p, tile.q, min(tile.row0 + wave * 16 * NT, tile.last), tile.last, kvh);
     const bool idle = tile.row0 + wave * 16 * NT > tile.last;  // converts only
@@ -603,33 +619,40 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
         const int32_t base = static_cast<int32_t>(64 * b);
         if (!idle && base < rows.any_hi && base + 64 > rows.any_lo) {
             const bool edge = base < rows.all_lo || base + 64 > rows.all_hi || __ballot(there) != ~0ull;
-            f16x8 pv[LIMBS][NT][2];
-            {
-                // Products of one step of dimensions, four key tiles by NT row tiles, do not wait for each other.
-                f32x4 s[NT][4];
+            // Products of one step of dimensions, four key tiles by NT row tiles, do not wait for each other.
+            f32x4 s[NT][4];
 #pragma unroll
-                for (int k = 0; k < KS; ++k)
+            for (int k = 0; k < KS; ++k)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const f16x8 kv = kf[b & 1][t][k][lane];
-#pragma unroll
-                        for (int i = 0; i < LIMBS; ++i)
-#pragma unroll
-                            for (int u = 0; u < NT; ++u)
-                                s[u][t] = mfma(kv, rows.qv[i][u][k], k || i ? s[u][t] : f32x4{0, 0, 0, 0});
-                    }
-                rows.softmax(s, pv, ks, vs, there, edge, base + 16 * static_cast<int32_t>(g));
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const f16x8 vv = vf[b & 1][d][c][lane];
+                for (int t = 0; t < 4; ++t) {
+                    const f16x8 kv = kf[b & 1][t][k][lane];
 #pragma unroll
                     for (int i = 0; i < LIMBS; ++i)
 #pragma unroll
-                        for (int u = 0; u < NT; ++u) rows.acc[u][d] = mfma(vv, pv[i][u][c], rows.acc[u][d]);
+                        for (int u = 0; u < NT; ++u) s[u][t] = mfma(kv, rows.qv[i][u][k], k || i ? s[u][t] : f32x4{0, 0, 0, 0});
                 }
+            float ff[NT], off[NT], sum[NT] = {};
+            rows.scores(s, ks, vs, there, edge, base + 16 * static_cast<int32_t>(g), ff, off);
+            f16x8 pv[2][LIMBS][NT];
+            rows.template probabilities<0>(s, pv[0], ff, off, sum);
+            rows.template probabilities<1>(s, pv[1], ff, off, sum);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const f16x8 vv = vf[b & 1][d][0][lane];
+#pragma unroll
+                for (int i = 0; i < LIMBS; ++i)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) rows.acc[u][d] = mfma(vv, pv[0][i][u], rows.acc[u][d]);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const f16x8 vv = vf[b & 1][d][1][lane];
+#pragma unroll
+                for (int i = 0; i < LIMBS; ++i)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) rows.acc[u][d] = mfma(vv, pv[1][i][u], rows.acc[u][d]);
+            }
+            rows.add(sum, vs);
         }
         if (b + 1 < tile.b1) convert(b + 1);
     }
@@ -764,7 +787,7 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
 
 template <typename T, int D, int FMT>
 int attend_launch(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s) {
-    const dim3 grid(p.slots, p.c.kv_heads, p.splits);
+    const dim3 grid(p.slots * p.c.kv_heads, 1, p.splits);
     constexpr int most = D == 256 ? 1 : 2;  // row tiles of the kernel for few rows
     const bool wide = static_cast<uint64_t>(p.c.pages) * p.c.page_size * p.c.kv_heads * D > 0xffffffffull;
     if (!plan.shared) k_attend_tile<T, D, FMT, 2><<<grid, 256, 0, s>>>(p, err);

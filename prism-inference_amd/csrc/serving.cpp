@@ -244,7 +244,7 @@ int prism_hip_attention_device(prism_hip_ctx *c, const prism_kv_cache *cache, co
     if (!std::isfinite(a->scale)) return bad(c, "scale must be finite");
     if (a->window && !a->causal) return bad(c, "a window needs the causal mask");
     if (a->window > 0x7fffffffu || a->max_length > 0x7fffffffu) return bad(c, "window or max_length out of range");
-    if (a->requests > kMostTokens || !a->max_pages || static_cast<uint64_t>(a->max_pages) * cache->page_size > 0x7fffffffull)
+    if (static_cast<uint64_t>(a->requests) * cache->kv_heads > kMostTokens || !a->max_pages || static_cast<uint64_t>(a->max_pages) * cache->page_size > 0x7fffffffull)
         return bad(c, "requests or max_pages out of range");
     if (a->tokens == 0 || a->requests == 0) return PRISM_OK;
     rc = check_rows(c, a->dtype, a->q, a->q_stride, a->heads, cache->head_dim);
