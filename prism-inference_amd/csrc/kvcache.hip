@@ -8,13 +8,15 @@ namespace {
 
 // ---- plan -------------------------------------------------------------------------------
 // Exclusive sums over the requests of their new tokens, of the pages they need and of those
-// they give back; every token's position, page and slot follows from these by itself.  One
-// workgroup makes the sums (a few thousand requests are a few loads a thread).  Few requests stay in
-// its LDS and it fills their tokens too; else a grid does, whose wavefronts look the request of
-// their first token up 64 offsets at a time and the others' in the 64 offsets behind it.
+// they give back; every token's position, page and slot follows from these by itself.  A workgroup
+// makes the sums of a few thousand requests in its LDS (a few loads a thread) and fills tokens; many
+// tokens take several workgroups, each with sums of its own (2048 requests, 88000 tokens: 13.7 us where sums and
+// tokens in two launches took 9.2 and 7.0 and the gap between).  Where the step writes over its own lengths or count they would
+// race, and more requests do not fit: there one workgroup makes the sums and a grid fills, whose wavefronts look
+// the request of their first token up 64 offsets at a time and the others' in the 64 offsets behind it.
 
 constexpr uint32_t kPlanThreads = 1024;
-constexpr uint32_t kPlanOwnTokens = 4096, kPlanOwnRequests = 1024;
+constexpr uint32_t kPlanOwnTokens = 4096, kPlanOwnRequests = 4096;
 
 struct PlanScratch {
     int32_t *need_base, *back_base;  // [requests + 1]
@@ -106,6 +108,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(prism_kv_plan p, PlanScra
     constexpr uint32_t kOwn = OWN ? kPlanOwnRequests : 1;
     __shared__ int32_t own_offset[kOwn], own_old[kOwn], own_need[kOwn], own_back[kOwn];
     const uint32_t tid = threadIdx.x, wave = tid / 64, waves = blockDim.x / 64;
+    const bool lead = blockIdx.x == 0;
     if (tid == 0) bad_any = 0;
     __syncthreads();
     const uint32_t each = (p.requests + blockDim.x - 1) / blockDim.x;
@@ -147,9 +150,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(prism_kv_plan p, PlanScra
     for (uint32_t r = r0; r < r1; ++r) {
         const int32_t n = p.lengths[r], a = p.added[r];
         const int32_t offset = refused ? 0 : static_cast<int32_t>(before[0]);
-        p.offsets[r] = offset;
+        if (lead) p.offsets[r] = offset;
         if (refused) {
-            p.new_lengths[r] = n;
+            if (lead) p.new_lengths[r] = n;
             continue;
         }
         if constexpr (OWN) {
@@ -161,14 +164,14 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(prism_kv_plan p, PlanScra
             sc.need_base[r] = static_cast<int32_t>(before[1]);
             sc.back_base[r] = static_cast<int32_t>(before[2]);
         }
-        p.new_lengths[r] = a == -1 ? 0 : n + a;
+        if (lead) p.new_lengths[r] = a == -1 ? 0 : n + a;
         const int64_t held = pages_of(n, p.page_size);
         before[0] += a == -1 ? 0 : a;
         before[1] += a == -1 ? 0 : pages_of(static_cast<int64_t>(n) + a, p.page_size) - held;
         before[2] += a == -1 ? held : 0;
     }
     const int32_t tokens = refused ? 0 : static_cast<int32_t>(total[0]), back = refused ? 0 : static_cast<int32_t>(total[2]);
-    if (tid == 0) {
+    if (tid == 0 && lead) {
         p.offsets[p.requests] = tokens;
         p.counts[0] = static_cast<int32_t>(refused ? count : height - total[1]);
         p.counts[1] = tokens;
@@ -184,9 +187,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(prism_kv_plan p, PlanScra
     }
     if constexpr (OWN) {
         __syncthreads();
-        for (int32_t b = static_cast<int32_t>(tid); b < back; b += static_cast<int32_t>(blockDim.x))
-            p.free_pages[count + b] = page_given_back(p, own_back, b);
-        for (uint32_t t = tid; t < p.max_tokens; t += blockDim.x) {
+        const uint32_t at = blockIdx.x * blockDim.x + tid, step = gridDim.x * blockDim.x;
+        for (uint32_t b = at; b < static_cast<uint32_t>(back); b += step)
+            p.free_pages[count + b] = page_given_back(p, own_back, static_cast<int32_t>(b));
+        for (uint32_t t = at; t < p.max_tokens; t += step) {
             if (static_cast<int32_t>(t) >= tokens) {
                 plan_no_token(p, t);
                 continue;
@@ -629,14 +633,19 @@ int append_typed(const AppendArgs &a, uint32_t each, dim3 grid, int *err, hipStr
 
 }  // namespace
 
+static bool overlap(const int32_t *a, uint64_t n, const int32_t *b, uint64_t m) { return a < b + m && b < a + n; }
+
 size_t plan_scratch_bytes(uint32_t requests) { return sizeof(int32_t) * (2 * (static_cast<size_t>(requests) + 1) + 4); }
 
 int launch_kv_plan(const prism_kv_plan &p, void *scratch, int *err, hipStream_t s) {
     const PlanScratch sc = plan_scratch(scratch, p.requests);
     const uint32_t wide = p.requests > p.max_tokens ? p.requests : p.max_tokens;
     const uint32_t threads = wide >= kPlanThreads ? kPlanThreads : (wide + 63) / 64 * 64;
-    if (p.max_tokens <= kPlanOwnTokens && p.requests <= kPlanOwnRequests) {
-        k_plan<true><<<1, threads, 0, s>>>(p, sc, err);
+    const bool apart = !overlap(p.lengths, p.requests, p.new_lengths, p.requests) && !overlap(p.free_count, 1, p.counts, 4);
+    if (p.requests <= kPlanOwnRequests && (apart || p.max_tokens <= kPlanOwnTokens)) {
+        uint32_t blocks = p.max_tokens <= kPlanOwnTokens ? 1 : (p.max_tokens + threads - 1) / threads;
+        if (blocks > 256) blocks = 256;
+        k_plan<true><<<blocks, threads, 0, s>>>(p, sc, err);
         return launch_status();
     }
     k_plan<false><<<1, threads, 0, s>>>(p, sc, err);
@@ -657,6 +666,7 @@ int launch_kv_append(const prism_kv_cache &cache, int dtype, const void *k, uint
                      uint64_t v_stride, const int32_t *slots, uint32_t tokens, int *err, hipStream_t s) {
     const AppendArgs a{cache, k, v, k_stride, v_stride, slots, tokens};
     const uint32_t each = tokens <= 1024 ? 4 : tokens <= 4096 ? 16 : 32;
+    // Tasks of one window far apart: with them side by side a prompt's append took 25 us instead of 17.
     const dim3 grid((tokens + each - 1) / each, 2 * cache.kv_heads);
     if (dtype == PRISM_DTYPE_F32) return append_typed<float>(a, each, grid, err, s);
     if (dtype == PRISM_DTYPE_F16) return append_typed<_Float16>(a, each, grid, err, s);
