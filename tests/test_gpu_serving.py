@@ -12,7 +12,7 @@ import pytest
 import prism_hip as ph
 import serving_oracle as so
 import synth
-from hiprt import DeviceBuffer, Graph, synchronize
+from hiprt import DeviceBuffer, Graph, hip, synchronize
 
 pytestmark = pytest.mark.gpu
 
@@ -283,6 +283,22 @@ def test_gpu_append(ctx, dtype, fmt, d, kv, page):
         held.check(so.append(cache, k.x, v.x, slots, page))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("runs", [[(3, 5000)], [(2, 1)] * 1500, [(0, 1), (15, 3)] * 1300, [(9, 40)] * 60], ids=["prompt", "single", "pairs", "chunks"])
+def test_gpu_append_of_many_tokens(ctx, dtype, runs):
+    """Each window of tokens a workgroup looks at, full of runs or of one."""
+    rng = np.random.default_rng(len(runs))
+    kv, d, page = 2, 64, 16
+    tokens = sum(n for _, n in runs)
+    cache = make_cache(rng, tokens // page + 2 * len(runs) + 3, kv, page, d, "int8")
+    slots = make_slots(rng, runs, page, cache["k"].shape[0])
+    k, v = (Rows(rng.standard_normal((tokens, kv, d)) * 2.0 ** rng.integers(-3, 3, (tokens, 1, 1)), dtype) for _ in range(2))
+    held = Device(cache, page)
+    ctx.kv_append_device(held.desc, DTYPE[dtype], k, k.stride, v, v.stride, dev(slots), tokens)
+    assert ctx.sync() == 0
+    held.check(so.append(cache, k.x, v.x, slots, page))
+
+
 def test_gpu_append_edges_of_the_scale(ctx):
     """Magnitudes on both sides of qmax * 2^e, zeros, the smallest and the largest floats."""
     d, page = 64, 16
@@ -438,6 +454,8 @@ BATCHES = {
     "chunk": [(70, 70), (33, 200), (1, 130)],
     "prompt": [(200, 200)],
     "mixed": [(90, 150), (1, 1), (1, 333), (2, 64), (130, 131)],
+    "drafts": [(7, 64), (6, 200), (8, 8)],             # 17 to 32 rows a request
+    "long-among-single": [(60, 60)] + [(1, 50)] * 20,  # many tiles of few rows for one request
 }
 
 
@@ -601,6 +619,120 @@ def test_gpu_attention_nonfinite_query(ctx):
     keep[7, 2] = False
     check(got[keep], want[keep], tol[keep])
     assert np.isnan(got[7, 2]).all()
+
+
+def test_gpu_attention_of_thousands_of_requests(ctx):
+    """More requests than one look-up step covers, some of them without tokens or keys."""
+    rng = np.random.default_rng(16)
+    r, page, d, heads, kv = 5000, 16, 64, 2, 1
+    added, lengths = rng.choice([0, 1, 1, 1, 2], r), rng.integers(0, 41, r)
+    offsets = np.concatenate([[0], np.cumsum(added)])
+    table, pages = make_table(rng, lengths, page)
+    cache = make_cache(rng, pages, kv, page, d, "int8")
+    held = Device(cache, page)
+    q = Rows(rng.standard_normal((offsets[-1], heads, d)), "f16")
+    for max_length in (40, 4000):  # unsplit and split
+        call, out = attend(ctx, held, q, offsets, lengths, table, 0.125, max_length=max_length)
+        assert ctx.sync() == 0
+        want, tol = so.attention(cache, q.x, offsets, lengths, table, page, 0.125, dtype="f16")
+        check(out.read(), want, tol)
+
+
+@pytest.mark.parametrize("window", [1, 2, 65, 10000])
+@pytest.mark.parametrize("added", [1, 40])
+def test_gpu_attention_windows_and_a_negative_scale(ctx, window, added):
+    rng = np.random.default_rng(window)
+    page, d, heads, kv, n = 32, 128, 4, 2, 400
+    table, pages = make_table(rng, [n], page)
+    cache = make_cache(rng, pages, kv, page, d, "int8")
+    cache["k_scale"] *= 0.25
+    held = Device(cache, page)
+    q = Rows(rng.standard_normal((added, heads, d)), "f32")
+    for scale in (d ** -0.5, -d ** -0.5, 0.0):
+        call, out = attend(ctx, held, q, [0, added], [n], table, scale, True, window)
+        assert ctx.sync() == 0
+        want, tol = so.attention(cache, q.x, [0, added], [n], table, page, scale, True, window)
+        check(out.read(), want, tol)
+
+
+@pytest.mark.parametrize("added", [1, 9, 200])
+def test_gpu_cache_past_32_bits(ctx, added):
+    """Keys and values of 4.4 GB each: pages on both sides of the 4 GB line, appended and attended."""
+    rng = np.random.default_rng(17)
+    page, d, heads, kv, pages, n = 256, 128, 8, 8, 17000, 700
+    unit = kv * page * d
+    assert pages * unit > 1 << 32
+    used = np.array([16999, 3, 16500, 16384], np.int32)  # the last and one beyond the line's page, and low ones
+    small = make_cache(rng, len(used), kv, page, d, "int8")
+    small["k_scale"] *= 0.25
+    buf = {"k": DeviceBuffer(pages * unit), "v": DeviceBuffer(pages * unit), "k_scale": DeviceBuffer(pages * kv * 4), "v_scale": DeviceBuffer(pages * kv * 4)}
+
+    def move(name, i, back=False):
+        size = unit if name in "kv" else kv * 4
+        host = np.ascontiguousarray(small[name][i])
+        at = int(used[i]) * size
+        if not back:
+            buf[name].upload(host, at)
+            return None
+        got = np.empty_like(host)
+        assert hip().hipMemcpy(got.ctypes.data, buf[name].data_ptr() + at, size, 2) == 0
+        return got
+
+    for i in range(len(used)):
+        for name in buf:
+            move(name, i)
+    desc = ph.KvCache(**buf, format=ph.CACHE_INT8, pages=pages, page_size=page, kv_heads=kv, head_dim=d)
+    k, v = (rng.standard_normal((added, kv, d)).astype(np.float32) for _ in range(2))
+    first = n - added
+    where = np.arange(first, n)
+    slots = used[where // page] * page + where % page
+    ctx.kv_append_device(desc, ph.DTYPE_F32, dev(k), kv * d, dev(v), kv * d, dev(slots.astype(np.int32)), added)
+    q = Rows(rng.standard_normal((added, heads, d)), "bf16")
+    table = used[None]
+
+    class Held:
+        pass
+
+    Held.desc = desc
+    call, out = attend(ctx, Held, q, [0, added], [n], table, d ** -0.5)
+    assert ctx.sync() == 0
+    want = so.append(small, k, v, (where // page * page + where % page).astype(np.int32), page)
+    for i in range(len(used)):
+        for name in buf:
+            assert np.array_equal(move(name, i, True), want[name][i]), (name, i)
+    exact, tol = so.attention(want, q.x, [0, added], [n], np.arange(len(used))[None], page, d ** -0.5, dtype="bf16")
+    check(out.read(), exact, tol)
+
+
+def test_gpu_attention_graphs_share_scratch(ctx):
+    """Two captured calls whose partial results share the context's scratch, replayed in turn after a
+    larger eager call, with eager work between; and a second context at the same time."""
+    rng = np.random.default_rng(18)
+    page, d, heads, kv = 16, 128, 8, 2
+    cases, graphs = [], []
+    with ph.Context(0) as other:
+        for n, added in ((3000, 1), (1700, 2)):
+            table, pages = make_table(rng, [n], page)
+            cache = make_cache(rng, pages, kv, page, d, "int8")
+            cache["k_scale"] *= 0.25
+            held = Device(cache, page)
+            q = Rows(rng.standard_normal((added, heads, d)), "f32")
+            call, out = attend(ctx, held, q, [0, added], [n], table, d ** -0.5)
+            assert ctx.sync() == 0
+            cases.append((call, out, held, so.attention(cache, q.x, [0, added], [n], table, page, d ** -0.5)))
+            graphs.append(Graph(ctx.stream(), lambda: ctx.attention_device(held.desc, call)))
+        big, pages = make_table(rng, [20000], page)
+        bigger = Device(make_cache(rng, pages, kv, page, d, "int8"), page)
+        attend(ctx, bigger, Rows(rng.standard_normal((3, heads, d)), "f32"), [0, 3], [20000], big, d ** -0.5)
+        for _ in range(3):
+            for graph, (call, out, held, _) in zip(graphs, cases):
+                other.attention_device(held.desc, call)  # the same rows from another stream
+                assert other.sync() == 0
+                out.buf.upload(out.before)
+                graph.launch()
+            assert ctx.sync() == 0
+            for _, out, _, (want, tol) in cases:
+                check(out.read(), want, tol)
 
 
 # ---- together ---------------------------------------------------------------------------------
