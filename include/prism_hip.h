@@ -463,8 +463,10 @@ int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, 
  * see is left out, and PRISM_ERR_INVALID_INPUT at sync, as are lengths past max_pages
  * pages and offsets out of order; a non-finite output is PRISM_ERR_NONFINITE.
  * max_length sizes the work split and should bound the lengths (any value is correct).
- * Statistics and sums are binary32; codes are exact in the products' binary16 operands.  For F16 and BF16
- * the probabilities are rounded to binary16, for F32 q and the probabilities enter in two binary16 parts. */
+ * Statistics and sums are binary32.  Codes are exact in the products' binary16 operands; the
+ * probabilities, times their page's value scale, are rounded to binary16 (F16, BF16) or enter, as q
+ * does, in two binary16 parts (F32), with all their bits down to 2^-25 of the row's largest.
+ * Scales are positive; requests * kv_heads is at most 2^23, tokens * heads 2^26. */
 typedef struct prism_attention {
     int dtype;
     uint32_t requests, tokens, heads, max_pages, max_length;
