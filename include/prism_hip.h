@@ -385,7 +385,8 @@ typedef struct prism_kv_cache {
  * max_tokens, a length past max_pages pages, a negative one, or no room for pages given
  * back is refused as a whole: new_lengths = lengths, no tokens, the stack and table as
  * they were, counts = {free pages, 0, 0, pages short}, and the next prism_hip_sync is
- * PRISM_ERR_RESOURCE (pages short) or PRISM_ERR_INVALID_INPUT. */
+ * PRISM_ERR_RESOURCE (pages short) or PRISM_ERR_INVALID_INPUT.  A token whose page is negative in
+ * the table or on the stack has slot -1, and the sync is PRISM_ERR_INVALID_INPUT. */
 typedef struct prism_kv_plan {
     uint32_t requests, max_pages, max_tokens, page_size, free_capacity;
     const int32_t *lengths, *added;
@@ -398,7 +399,8 @@ int prism_hip_kv_plan_device(prism_hip_ctx *ctx, const prism_kv_plan *plan, void
 /* Rotary positions.  The rotation keeps the frequencies (radians a position) of dims / 2
  * pairs on the device; dims is even, 2 to 256.  Pairs are (i, i + dims/2), or (2i, 2i + 1)
  * where interleaved; dimensions from dims on pass unrotated.  magnitude multiplies the
- * cosines and sines (1 without scaling).  NULL on failure.  Destroy it before its context.
+ * cosines and sines (1 without scaling).  NULL on failure.  Destroy it before its context, and
+ * after the graphs that use it.
  * prism_hip_rope_frequencies fills out[dims / 2] on the host: base^(-2i/dims), for long
  * contexts divided by factor: each (original = 0), or by how often the pair turns in the
  * `original` positions the model has seen, r = original * f / 2 pi: kept from beta turns,
@@ -413,7 +415,8 @@ void prism_hip_rope_destroy(prism_hip_rope *rope);
  * positions[t]; norm, if not NULL, first takes x to x / sqrt(mean(x^2) + eps) * norm[i]
  * (binary32 norm[head_dim]).  Computed in binary64, rounded once to binary32 and from
  * there to the type.  Strides are elements between tokens, at least heads * head_dim;
- * out may be x with the same stride.  A non-finite x is PRISM_ERR_NONFINITE at sync. */
+ * out may be x with the same stride.  A non-finite x, or a result past the type's largest
+ * value, is PRISM_ERR_NONFINITE at sync. */
 int prism_hip_rope_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, int dtype, const void *x, uint64_t x_stride,
                           const int32_t *positions, uint32_t tokens, uint32_t heads, uint32_t head_dim,
                           const float *norm, float eps, void *out, uint64_t out_stride, void *stream);
@@ -453,8 +456,8 @@ int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, 
 
 /* Attention of q [tokens][heads][head_dim] over the cache.  Request r has the tokens
  * offsets[r] .. offsets[r + 1] - 1 (offsets ascend from 0 to at most `tokens`; rows behind
- * the last are not written) and the lengths[r] keys and values of its block table row, heads a multiple of
- * kv_heads (head h reads kv head h / (heads / kv_heads)).
+ * the last are not written) and the lengths[r] keys and values of its block table row, heads a
+ * multiple of kv_heads (head h reads kv head h / (heads / kv_heads)).  out may be q with the same stride.
  *   out = softmax(scale * q k^T) v over the allowed keys; a row without any is 0.
  * causal: the request's tokens are its last, so token i of n sees the positions up to
  * lengths[r] - n + i, with window > 0 only the last `window` of them; else (window = 0)

@@ -67,7 +67,7 @@ __device__ __forceinline__ int32_t page_given_back(const prism_kv_plan &p, const
 }
 
 __device__ __forceinline__ void plan_token(const prism_kv_plan &p, const int32_t *back_base, uint32_t t, uint32_t r, int32_t old,
-                                           int32_t offset, int32_t need_base, int32_t count, int32_t back) {
+                                           int32_t offset, int32_t need_base, int32_t count, int32_t back, int *err) {
     const int32_t page = static_cast<int32_t>(p.page_size);
     const int32_t position = old + static_cast<int32_t>(t) - offset;
     const int32_t held = static_cast<int32_t>(pages_of(old, p.page_size)), j = position / page, place = position % page;
@@ -82,7 +82,9 @@ __device__ __forceinline__ void plan_token(const prism_kv_plan &p, const int32_t
     }
     const int64_t s = static_cast<int64_t>(id) * page + place;
     p.positions[t] = position;
-    p.slots[t] = id >= 0 && s <= 0x7fffffff ? static_cast<int32_t>(s) : -1;
+    const bool page_ok = id >= 0 && s <= 0x7fffffff;
+    if (!page_ok) raise_error(err, kErrIndex);
+    p.slots[t] = page_ok ? static_cast<int32_t>(s) : -1;
     p.owners[t] = static_cast<int32_t>(r);
 }
 __device__ __forceinline__ void plan_no_token(const prism_kv_plan &p, uint32_t t) {
@@ -196,12 +198,12 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(prism_kv_plan p, PlanScra
                 continue;
             }
             const uint32_t r = last_at_most(own_offset, p.requests, static_cast<int32_t>(t));
-            plan_token(p, own_back, t, r, own_old[r], own_offset[r], own_need[r], count, back);
+            plan_token(p, own_back, t, r, own_old[r], own_offset[r], own_need[r], count, back, err);
         }
     }
 }
 
-__global__ __launch_bounds__(256) void k_plan_fill(prism_kv_plan p, PlanScratch sc) {
+__global__ __launch_bounds__(256) void k_plan_fill(prism_kv_plan p, PlanScratch sc, int *err) {
     const uint32_t t = blockIdx.x * 256 + threadIdx.x;
     const int32_t tokens = sc.head[0], count = sc.head[1], back = sc.head[2];
     for (int32_t b = static_cast<int32_t>(t); b < back; b += static_cast<int32_t>(gridDim.x * 256))
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(256) void k_plan_fill(prism_kv_plan p, PlanScratch 
     if (static_cast<int32_t>(t & ~63u) < tokens) {
         const uint32_t r = last_at_most_wave(p.offsets, p.requests, static_cast<int32_t>(t));
         if (static_cast<int32_t>(t) < tokens) {
-            plan_token(p, sc.back_base, t, r, p.new_lengths[r] - p.added[r], p.offsets[r], sc.need_base[r], count, back);
+            plan_token(p, sc.back_base, t, r, p.new_lengths[r] - p.added[r], p.offsets[r], sc.need_base[r], count, back, err);
             return;
         }
     }
@@ -239,6 +241,13 @@ __device__ __forceinline__ void rope_table(double (*cs)[128], double (*sn)[128],
     __syncthreads();
 }
 
+// Whether four values are finite once they are rounded to the type.
+template <typename T>
+__device__ __forceinline__ bool fits(f32x4 v) {
+    const f32x4 r = __builtin_convertvector(__builtin_convertvector(v, typename Four<T>::type), f32x4);
+    return finite(r[0]) && finite(r[1]) && finite(r[2]) && finite(r[3]);
+}
+
 // dims a multiple of 8: a lane has four pairs of a row (four elements of each half, or eight
 // neighbours where interleaved), or eight elements behind the rotated ones.
 template <typename T, int D, bool INTERLEAVED>
@@ -262,7 +271,7 @@ __global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation r
         s[j] = turns ? sn[wave][4 * li + j] : 0.0;
     }
     const uint32_t h0 = blockIdx.y * heads_each, h1 = min(a.heads + b.heads, h0 + heads_each);
-    bool bad = false;
+    bool bad = false, over = false;
     // The heads of a, then those of b.
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -313,6 +322,7 @@ __global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation r
                     if constexpr (INTERLEAVED) (j < 2 ? o0 : o1)[2 * (j & 1)] = f, (j < 2 ? o0 : o1)[2 * (j & 1) + 1] = g;
                     else o0[j] = f, o1[j] = g;
                 }
+                over |= !fits<T>(o0) || !fits<T>(o1);
                 if (h + u * kRows < to) {
                     store4(out + (h + u * kRows) * D + e0, o0);
                     store4(out + (h + u * kRows) * D + e1, o1);
@@ -321,6 +331,7 @@ __global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation r
         }
     }
     if (bad) raise_error(err, kErrInput);
+    if (over) raise_error(err, kErrNonfinite);
 }
 
 // Any dims: a lane has four consecutive elements and looks their partners up.
@@ -335,7 +346,7 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeRows a, RopeRows b, Rotati
     const uint32_t h0 = blockIdx.y * heads_each, h1 = min(a.heads + b.heads, h0 + heads_each);
     const uint32_t groups = (h1 - h0 + kRows - 1) / kRows;
     const uint32_t e0 = 4 * (lane % kLanes);
-    bool bad = false;
+    bool bad = false, over = false;
     for (uint32_t it = threadIdx.x / 64; it < nt * groups; it += 4) {
         const uint32_t t = it / groups, h = h0 + it % groups * kRows + lane / kLanes;
         const uint32_t hc = min(h, h1 - 1);
@@ -375,9 +386,11 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeRows a, RopeRows b, Rotati
             }
             out[j] = static_cast<float>(y);
         }
+        over |= !fits<T>(out);
         if (h < h1) store4(static_cast<T *>(m.out) + (t0 + t) * m.out_stride + row + e0, out);
     }
     if (bad) raise_error(err, kErrInput);
+    if (over) raise_error(err, kErrNonfinite);
 }
 
 // ---- append -----------------------------------------------------------------------------
@@ -654,7 +667,7 @@ int launch_kv_plan(const prism_kv_plan &p, void *scratch, int *err, hipStream_t 
     k_plan<false><<<1, threads, 0, s>>>(p, sc, err);
     const int rc = launch_status();
     if (rc) return rc;
-    k_plan_fill<<<(p.max_tokens + 255) / 256, 256, 0, s>>>(p, sc);
+    k_plan_fill<<<(p.max_tokens + 255) / 256, 256, 0, s>>>(p, sc, err);
     return launch_status();
 }
 

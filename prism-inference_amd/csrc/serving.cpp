@@ -251,6 +251,7 @@ int prism_hip_attention_device(prism_hip_ctx *c, const prism_kv_cache *cache, co
     if (!rc) rc = check_rows(c, a->dtype, a->out, a->out_stride, a->heads, cache->head_dim);
     if (rc) return rc;
     if (!a->offsets || !a->lengths || !a->block_table) return bad(c, "null device pointer");
+    if (a->q == a->out && a->q_stride != a->out_stride) return bad(c, "attention in place needs one stride");
     OnDevice on(c);
     const size_t need = attention_scratch_bytes(*cache, *a, c->cus);
     if (need) rc = ensure(c, c->att, need);

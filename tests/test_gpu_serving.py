@@ -152,6 +152,17 @@ def test_gpu_plan_refuses_a_step_as_a_whole(ctx, what):
     assert ctx.sync() == 0
 
 
+@pytest.mark.parametrize("max_tokens", [40, 5000])
+def test_gpu_plan_flags_negative_pages(ctx, max_tokens):
+    """A held page and a free one below zero: their tokens have no slot, the others theirs."""
+    table = np.array([[3, -1, -1], [-5, -1, -1], [1, -1, -1]], np.int32)
+    free = np.array([7, -2, 8], np.int32)
+    rc, got = run_plan(ctx, np.array([4, 10, 15]), np.array([20, 2, 2]), table, free, 3, 16, max_tokens)
+    assert rc == ph.ERR_INVALID_INPUT and ctx.sync() == 0
+    assert got[3][:12].tolist() == list(range(3 * 16 + 4, 4 * 16)) and got[3][12:20].tolist() == list(range(8 * 16, 8 * 16 + 8))
+    assert got[3][20:22].tolist() == [-1, -1] and got[3][22:24].tolist() == [31, -1] and got[5].tolist() == [1, 24, 2, 0]
+
+
 def test_gpu_plan_carries_its_state_through_a_graph(ctx):
     """Lengths and the free count in place: replays of one captured step are steps."""
     r, page = 5, 16
@@ -219,6 +230,20 @@ def test_gpu_rope_flags_a_nonfinite_row_and_keeps_the_others(ctx):
     keep = np.ones((4, 2), bool)
     keep[2, 1] = False
     assert np.allclose(got[keep], want[keep], rtol=1e-6, atol=1e-6)
+    rope.close()
+
+
+@pytest.mark.parametrize("dims", [64, 66])
+@pytest.mark.parametrize("dtype,most", [("f32", 3e38), ("f16", 6e4), ("bf16", 3.3e38)])
+def test_gpu_rope_flags_results_past_the_type(ctx, dtype, most, dims):
+    x = np.full((2, 3, 128), 1.0)
+    x[1, 2, :] = most  # turned by 45 degrees a pair is 1.4 times as long, or none
+    freq = np.full(dims // 2, np.pi / 4)
+    rope = ph.Rope(ctx, dims, freq)
+    rows, out = Rows(x, dtype), Rows(np.zeros_like(x), dtype)
+    for position, rc in ((1, ph.ERR_NONFINITE), (0, 0)):
+        ctx.rope_device(rope, DTYPE[dtype], rows, rows.stride, i32([position] * 2), 2, 3, 128, out, out.stride)
+        assert ctx.sync() == rc
     rope.close()
 
 
@@ -599,6 +624,23 @@ def test_gpu_attention_ranges(ctx, dtype):
         assert ctx.sync() == 0
         want, tol = so.attention(cache, q.x, [0, 2], [n], table, page, scale, dtype=dtype)
         check(out.read(), want, tol)
+
+
+@pytest.mark.parametrize("batch", ["step", "mixed", "prompt", "drafts"])
+def test_gpu_attention_in_place(ctx, batch):
+    rng = np.random.default_rng(19)
+    added, lengths = (list(x) for x in zip(*BATCHES[batch]))
+    offsets, page, d, heads, kv = np.concatenate([[0], np.cumsum(added)]), 16, 128, 8, 2
+    table, pages = make_table(rng, lengths, page)
+    cache = make_cache(rng, pages, kv, page, d, "int8")
+    cache["k_scale"] *= 0.25
+    held = Device(cache, page)
+    for max_length in (max(lengths), 4000):
+        q = Rows(rng.standard_normal((offsets[-1], heads, d)), "f32", pad=4)
+        attend(ctx, held, q, offsets, lengths, table, d ** -0.5, max_length=max_length, out=q)
+        assert ctx.sync() == 0
+        want, tol = so.attention(cache, q.x, offsets, lengths, table, page, d ** -0.5)
+        check(q.read(), want, tol)
 
 
 def test_gpu_attention_nonfinite_query(ctx):

@@ -138,7 +138,7 @@ def test_attention_refusals(stub):
             refused(attend, **{name: None})
         for bad in (dict(dtype=9), dict(heads=0), dict(heads=5), dict(scale=float("nan")), dict(window=5, causal=0), dict(window=1 << 31),
                     dict(max_length=1 << 31), dict(max_pages=0), dict(max_pages=1 << 28), dict(requests=(1 << 22) + 1), dict(q=X + 2),
-                    dict(q_stride=767), dict(out_stride=767), dict(tokens=1 << 24), dict(tokens=1 << 23, heads=16)):
+                    dict(q_stride=767), dict(out_stride=767), dict(out=X, out_stride=770), dict(tokens=1 << 24), dict(tokens=1 << 23, heads=16)):
             refused(attend, **bad)
         assert ph.lib().prism_hip_attention_device(ctx.handle, None, None, None) == ph.ERR_INVALID_INPUT
         """)
