@@ -399,9 +399,10 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
     const uint32_t kgroup = (lane >> 2) & 3;  // 16-key group whose keys this lane loads for the first product
     // Registers of codes are filled again as soon as a product has used them, the next block's keys behind the
     // first product and its values behind the second; its table entries are a block further ahead.
-    // Heads of 256 have no registers for that (spilled, 205 us instead of 153 for eight long requests):
-    // their codes are loaded at the block's start, two wavefronts a SIMD covering each other.
-    constexpr bool kAhead = D < 256;
+    // Heads of 256, and two row tiles of binary32 at 128, have no registers for that (spilled: 205 us instead of 153
+    // for eight long requests, 206 instead of 91 for 24 rows a request): their codes are loaded at the
+    // block's start, two wavefronts a SIMD covering each other.
+    constexpr bool kAhead = D < 256 && !(D == 128 && NT == 2 && LIMBS == 2);
     int32_t id_k = 0, id_v = 0;
     u32x4 kraw[4][D / 64], vraw[DT];
     typedef std::conditional_t<WIDE, uint64_t, uint32_t> Offset;
