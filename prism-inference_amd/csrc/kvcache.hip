@@ -1,5 +1,7 @@
 // kvcache.hip -- what keeps the paged 8-bit cache of many requests (gfx950): pages and slots
 // of a step's new tokens, rotary positions, and the append that quantizes keys and values.
+#include <type_traits>
+
 #include "serve_common.hpp"
 
 namespace prism {
@@ -283,16 +285,22 @@ __global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation r
         if (m.norm) w0 = load4(m.norm + e0), w1 = load4(m.norm + e1);
         const T *x = static_cast<const T *>(m.x) + t * m.x_stride;
         T *out = static_cast<T *>(m.out) + t * m.out_stride;
-        for (uint32_t h = from + lane / kLanes; h - lane / kLanes < to; h += kRows * kFlight) {
+        // Row groups whose heads are all there run without a condition; the rest of them (all, where a token has
+        // few heads) leave out the missing ones.  Conditions everywhere cost 24 -> 29 us for 24 heads of
+        // 256, none 64 us instead of 34 for 3 + 1 heads of 64.
+        auto rows = [&](uint32_t base, auto whole) {
+            const uint32_t h = base + lane / kLanes;
             f32x4 v0[kFlight], v1[kFlight];
 #pragma unroll
             for (uint32_t u = 0; u < kFlight; ++u) {
+                if (!whole && base + u * kRows >= to) break;
                 const uint32_t hh = min(h + u * kRows, to - 1);
                 v0[u] = load4(x + hh * D + e0);
                 v1[u] = load4(x + hh * D + e1);
             }
 #pragma unroll
             for (uint32_t u = 0; u < kFlight; ++u) {
+                if (!whole && base + u * kRows >= to) break;
                 double y[8];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -328,7 +336,10 @@ __global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation r
                     store4(out + (h + u * kRows) * D + e1, o1);
                 }
             }
-        }
+        };
+        uint32_t base = from;
+        for (; base + (kFlight - 1) * kRows < to; base += kRows * kFlight) rows(base, std::true_type());
+        if (base < to) rows(base, std::false_type());
     }
     if (bad) raise_error(err, kErrInput);
     if (over) raise_error(err, kErrNonfinite);
