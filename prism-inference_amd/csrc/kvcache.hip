@@ -411,7 +411,7 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeRows a, RopeRows b, Rotati
 // registers hold (single tokens above all) go to one wavefront each, longer ones to all four, which
 // exchange their magnitudes.  Earlier codes of the page are rewritten only where the scale grew.
 // 8192 bf16 tokens of 8 heads of 128 into e4m3 pages of 64 take 17 us (50 MB, 2.9 TB/s), 48 ragged f16 chunks of 4 heads of
-// 256 21 us, 32 single f32 tokens 6 us: a few chains of loads per wavefront and its VALU work, not yet memory.
+// 256 20 us, 32 single f32 tokens 4 us: a few chains of loads per wavefront and its VALU work, not yet memory.
 
 template <int FMT>
 __device__ __forceinline__ float least_scale(float most) {  // 2^e, most <= qmax 2^e

@@ -540,7 +540,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 // converted to binary16 once by the workgroup, a quarter by each wavefront, into LDS in the order of the
 // operands (a fragment is 16 consecutive bytes a lane: no bank conflicts); the next block's codes
 // come from memory meanwhile and are converted behind the products, so a block costs one barrier.
-// A prompt of 8192 tokens (32 heads of 128 on 8) takes 615 us, 894 TFLOP/s: VALU issue fills 56 % of the cycles (some 380
+// A prompt of 8192 tokens (32 heads of 128 on 8) takes 610 us, 901 TFLOP/s: VALU issue fills 56 % of the cycles (some 380
 // instructions a block and wavefront, 80 of them conversions), the matrix cores 37 %.  Converting in every
 // wavefront took 1240 us, eight wavefronts a workgroup 827 where four took 755.
 template <typename T, int D, int FMT, int NT>
