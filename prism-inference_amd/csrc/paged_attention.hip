@@ -356,19 +356,22 @@ __device__ __forceinline__ bool tile_of(const AttendArgs &p, uint32_t M, uint32_
     return split < t->parts;
 }
 
-// The table's entry for 16 keys from `key` on: their page, where some row sees one of them (key < end) and
-// the entry is a page; else page 0 stands in and they count as masked.  Entries and scales are taken as
-// loaded and looked at where they are used, blocks later.
-__device__ __forceinline__ int32_t entry_at(const AttendArgs &p, const int32_t *table, int32_t key, int32_t end) {
-    return table[min(key, end - 1) >> p.page_log2];
+// Some row of the tile sees one of the 16 keys from `key` on.  The first block of a window and the last of the
+// keys also cover pages that none sees, whose columns, scales and codes may be anything.
+__device__ __forceinline__ bool seen(const Tile &t, int32_t key) { return key < t.seen_hi && key > t.seen_lo - 16; }
+// The table's entry for 16 keys from `key` on (the nearest seen column's where none is seen): their page, where
+// they are seen and the entry is a page; else page 0 stands in and they count as masked.  Entries and scales
+// are taken as loaded and looked at where they are used, blocks later.
+__device__ __forceinline__ int32_t entry_at(const AttendArgs &p, const Tile &t, const int32_t *table, int32_t key) {
+    return table[min(max(key, t.seen_lo), t.seen_hi - 1) >> p.page_log2];
 }
-__device__ __forceinline__ bool is_page(const AttendArgs &p, int32_t id, int32_t key, int32_t end) {
-    return key < end && static_cast<uint32_t>(id) < p.c.pages;
+__device__ __forceinline__ bool is_page(const AttendArgs &p, const Tile &t, int32_t id, int32_t key) {
+    return seen(t, key) && static_cast<uint32_t>(id) < p.c.pages;
 }
 __device__ __forceinline__ float value_scale(float v, bool there) {  // log2 and 1 / v stay finite; NaN stays NaN
     return !there ? 1.0f : v < 0x1p-100f ? 0x1p-100f : v;
 }
-// Bytes behind the keys may hold NaN codes, which zero probabilities do not silence: the first `keep` of 16 stay.
+// Bytes behind the keys, and stand-ins, may hold NaN codes, which zero probabilities do not silence: the first `keep` of 16 stay.
 __device__ __forceinline__ void keep_bytes(u32x4 &v, int32_t keep) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -411,15 +414,15 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
     bool there_next = false, missing = false;
     auto look = [&](uint32_t b) {
         const int32_t base = static_cast<int32_t>(64 * b);
-        id_k = entry_at(p, table, base + 16 * static_cast<int32_t>(kgroup), tile.seen_hi);
-        id_v = entry_at(p, table, base + 16 * static_cast<int32_t>(g), tile.seen_hi);
+        id_k = entry_at(p, tile, table, base + 16 * static_cast<int32_t>(kgroup));
+        id_v = entry_at(p, tile, table, base + 16 * static_cast<int32_t>(g));
     };
     auto fetch_keys = [&](uint32_t b) {
         const int32_t base = static_cast<int32_t>(64 * b);
         const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
-        there_next = is_page(p, id_v, key_v, tile.seen_hi);
-        missing |= !there_next && key_v < tile.seen_hi && key_v + 16 > tile.seen_lo;
-        const Offset unit_k = static_cast<Offset>(is_page(p, id_k, key_k, tile.seen_hi) ? id_k : 0) * p.c.kv_heads + kvh;
+        there_next = is_page(p, tile, id_v, key_v);
+        missing |= !there_next && seen(tile, key_v);
+        const Offset unit_k = static_cast<Offset>(is_page(p, tile, id_k, key_k) ? id_k : 0) * p.c.kv_heads + kvh;
         const Offset unit_v = static_cast<Offset>(there_next ? id_v : 0) * p.c.kv_heads + kvh;
         ks_next = p.c.k_scale[unit_v];
         vs_next = p.c.v_scale[unit_v];
@@ -560,7 +563,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
     const uint32_t page_mask = p.c.page_size - 1;
     const int32_t *table = p.a.block_table + static_cast<uint64_t>(tile.r) * p.a.max_pages;
     const uint8_t *kc = static_cast<const uint8_t *>(p.c.k), *vc = static_cast<const uint8_t *>(p.c.v);
-    const int32_t seen_lo = tile.seen_lo, seen_hi = tile.seen_hi;
     const uint32_t kgroup = (lane >> 2) & 3;
     bool missing = false;
 
@@ -571,15 +573,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
     int32_t id_k = 0, id_v = 0;
     auto look = [&](uint32_t b) {  // the table's entries of block b
         const int32_t base = static_cast<int32_t>(64 * b);
-        id_k = entry_at(p, table, base + 16 * static_cast<int32_t>(kgroup), seen_hi);
-        id_v = entry_at(p, table, base + 16 * static_cast<int32_t>(g), seen_hi);
+        id_k = entry_at(p, tile, table, base + 16 * static_cast<int32_t>(kgroup));
+        id_v = entry_at(p, tile, table, base + 16 * static_cast<int32_t>(g));
     };
     auto fetch = [&](uint32_t b) {  // its codes and scales, from the pages that look found
         const int32_t base = static_cast<int32_t>(64 * b);
         const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
-        there_next = is_page(p, id_v, key_v, seen_hi);
-        missing |= !there_next && key_v < seen_hi && key_v + 16 > seen_lo;
-        const uint64_t unit_k = static_cast<uint64_t>(is_page(p, id_k, key_k, seen_hi) ? id_k : 0) * p.c.kv_heads + kvh;
+        there_next = is_page(p, tile, id_v, key_v);
+        missing |= !there_next && seen(tile, key_v);
+        const uint64_t unit_k = static_cast<uint64_t>(is_page(p, tile, id_k, key_k) ? id_k : 0) * p.c.kv_heads + kvh;
         const uint64_t unit_v = static_cast<uint64_t>(there_next ? id_v : 0) * p.c.kv_heads + kvh;
         ks_next = p.c.k_scale[unit_v];
         vs_next = p.c.v_scale[unit_v];
@@ -595,7 +597,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
 #pragma unroll
         for (int k = 0; k < KS; ++k) kf[at][wave][k][lane] = halves<FMT>(kraw[k / 2][2 * (k % 2)], kraw[k / 2][2 * (k % 2) + 1]);
         if (FMT == kE4m3) {
-            const int32_t left = seen_hi - static_cast<int32_t>(64 * b + 16 * g);
+            const int32_t left = tile.seen_hi - static_cast<int32_t>(64 * b + 16 * g);
             if (__ballot(!there_next || left < 16))
 #pragma unroll
                 for (int d = 0; d < DT / 4; ++d) keep_bytes(vraw[d], there_next ? left : 0);

@@ -777,6 +777,31 @@ def test_gpu_attention_graphs_share_scratch(ctx):
                 check(out.read(), want, tol)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("added,longest", [(1, 300), (1, 20000), (7, 300), (40, 300)], ids=["single", "split", "draft", "chunk"])
+def test_gpu_attention_pages_before_a_window_hold_anything(ctx, added, longest, page, dtype, fmt):
+    """Columns before a window name pages that may hold anything: NaN and infinite scales, NaN codes. The window begins
+    inside a block of 64 keys, with pages between the block's first key and its own."""
+    rng = np.random.default_rng(20)
+    d, heads, kv, n = 128, 8, 2, 300
+    table, pages = make_table(rng, [n], page)
+    cache = make_cache(rng, pages, kv, page, d, fmt)
+    cache["k_scale"] *= 0.25
+    q = Rows(rng.standard_normal((added, heads, d)), dtype)
+    for lo in (128 + page, 128 + page + 5, 128 + 63):
+        window = n - added + 1 - lo
+        want, tol = so.attention(cache, q.x, [0, added], [n], table, page, d ** -0.5, True, window, dtype)
+        for bad in (np.nan, np.inf):
+            held = {k: (a.copy() if isinstance(a, np.ndarray) else a) for k, a in cache.items()}
+            before = table[0, : lo // page]
+            held["k"][before], held["v"][before], held["k_scale"][before], held["v_scale"][before] = 0x7F, 0xFF, bad, bad
+            call, out = attend(ctx, Device(held, page), q, [0, added], [n], table, d ** -0.5, True, window, max_length=longest)
+            assert ctx.sync() == 0, (lo, bad)
+            check(out.read(), want, tol)
+
+
 # ---- together ---------------------------------------------------------------------------------
 
 
