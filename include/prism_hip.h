@@ -464,7 +464,7 @@ int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, 
  * every key, whatever their number: states of another length, an encoder's for instance.
  * Table columns no row sees are not read.  A page outside the cache among those it does
  * see is left out, and PRISM_ERR_INVALID_INPUT at sync, as are lengths past max_pages
- * pages and offsets out of order; a non-finite output is PRISM_ERR_NONFINITE.
+ * pages and offsets out of order; an output that is not finite in its type is PRISM_ERR_NONFINITE.
  * max_length sizes the work split and should bound the lengths (any value is correct).
  * Statistics and sums are binary32.  Codes are exact in the products' binary16 operands; the
  * probabilities, times their page's value scale, are rounded to binary16 (F16, BF16) or enter, as q

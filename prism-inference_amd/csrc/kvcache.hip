@@ -243,13 +243,6 @@ __device__ __forceinline__ void rope_table(double (*cs)[128], double (*sn)[128],
     __syncthreads();
 }
 
-// Whether four values are finite once they are rounded to the type.
-template <typename T>
-__device__ __forceinline__ bool fits(f32x4 v) {
-    const f32x4 r = __builtin_convertvector(__builtin_convertvector(v, typename Four<T>::type), f32x4);
-    return finite(r[0]) && finite(r[1]) && finite(r[2]) && finite(r[3]);
-}
-
 // dims a multiple of 8: a lane has four pairs of a row (four elements of each half, or eight
 // neighbours where interleaved), or eight elements behind the rotated ones.
 template <typename T, int D, bool INTERLEAVED>

@@ -151,8 +151,7 @@ __device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_
 
 template <typename T>
 __device__ __forceinline__ void write_row(const AttendArgs &p, uint32_t token, uint32_t head, uint32_t dim, f32x4 v, bool *bad) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *bad |= !finite(v[i]);
+    *bad |= !fits<T>(v);
     store4(static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * p.c.head_dim + dim, v);
 }
 
@@ -743,9 +742,9 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
     T *out = static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * D + E * lane;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        const float v = acc[i] * inv;
-        bad |= !finite(v);
-        out[i] = static_cast<T>(v);
+        const T v = static_cast<T>(acc[i] * inv);
+        bad |= !finite(static_cast<float>(v));
+        out[i] = v;
     }
     if (bad) raise_error(err, kErrNonfinite);
 }

@@ -46,6 +46,12 @@ template <typename T>
 __device__ __forceinline__ void store4(T *p, f32x4 v) {  // ties to even
     store_any(p, __builtin_convertvector(v, typename Four<T>::type));
 }
+// Whether four values are finite once they are rounded to the type.
+template <typename T>
+__device__ __forceinline__ bool fits(f32x4 v) {
+    const f32x4 r = __builtin_convertvector(__builtin_convertvector(v, typename Four<T>::type), f32x4);
+    return finite(r[0]) && finite(r[1]) && finite(r[2]) && finite(r[3]);
+}
 
 constexpr int kInt8 = PRISM_CACHE_INT8, kE4m3 = PRISM_CACHE_E4M3;
 

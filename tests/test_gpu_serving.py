@@ -802,6 +802,27 @@ def test_gpu_attention_pages_before_a_window_hold_anything(ctx, added, longest, 
             check(out.read(), want, tol)
 
 
+@pytest.mark.parametrize("dtype,scale", [("f16", 2.0 ** 10), ("bf16", 2.677e36)])
+@pytest.mark.parametrize("added,n", [(1, 40), (1, 3000), (60, 90)], ids=["rows", "split", "tile"])
+def test_gpu_attention_flags_results_past_the_type(ctx, added, n, dtype, scale):
+    """Results that binary32 holds and the type does not: 127 * 2^10 in binary16, 3.3998e38 in bfloat16."""
+    rng = np.random.default_rng(21)
+    page, d, heads, kv = 16, 64, 4, 1
+    table, pages = make_table(rng, [n], page)
+    cache = make_cache(rng, pages, kv, page, d, "int8")
+    cache["k"][:], cache["v"][:] = 0, 127
+    q = Rows(rng.standard_normal((added, heads, d)), dtype)
+    for factor, rc in ((1.0, ph.ERR_NONFINITE), (0.5, 0)):
+        cache["v_scale"][:] = scale * factor
+        call, out = attend(ctx, Device(cache, page), q, [0, added], [n], table, 0.125)
+        assert ctx.sync() == rc and ctx.sync() == 0
+        got, want = out.read(), 127.0 * float(np.float32(scale * factor))
+        if rc:
+            assert np.isposinf(got).all()
+        else:  # equal probabilities: the division and the type's half step
+            assert (np.abs(got - want) <= (so.HALF[dtype] + 2.0 ** -20) * want).all()
+
+
 # ---- together ---------------------------------------------------------------------------------
 
 
