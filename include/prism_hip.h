@@ -469,7 +469,8 @@ int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, 
  * Statistics and sums are binary32.  Codes are exact in the products' binary16 operands; the
  * probabilities, times their page's value scale, are rounded to binary16 (F16, BF16) or enter, as q
  * does, in two binary16 parts (F32), with all their bits down to 2^-25 of the row's largest.
- * Scales are positive; requests * kv_heads is at most 2^23, tokens * heads 2^26. */
+ * Value scales are 2^-100 to 2^121, as the append makes them, in any mixture (a smaller one counts as 2^-100), key
+ * scales positive; requests * kv_heads is at most 2^23, tokens * heads 2^26. */
 typedef struct prism_attention {
     int dtype;
     uint32_t requests, tokens, heads, max_pages, max_length;

@@ -27,6 +27,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 // contributions down to 2^-25 of the largest.
 constexpr float kHeadroom = 11.0f, kSlack = 4.0f;
 constexpr float kNone = -__builtin_inff();
+// The denominator l is held times 2^-12 relative to the numerator.  A key's term of it is 2^(S - m + 11 - 12): with value
+// scales of 2^-100 to 2^121, as the append makes them, S - m of the largest term is between -121 and 104, so
+// neither the smallest sum leaves binary32's normal numbers nor that of 2^24 keys its range.
+constexpr float kSumShift = 12.0f, kSumUnit = 0x1p-12f;
+// While every value scale met is within 2^+-40, the largest p of a row and those of keys that matter to l are less than
+// 2^100 apart, and l takes a key's p over the scale.  Past that p may vanish where the key's weight does not (a page of
+// zeros, scale 2^-100, beside one of 2^38): from there on l's terms are exponentials of their own.  Looking for such
+// scales costs a prompt 1.4 % (608 -> 617 us); a second copy of the loop for them cost long caches and chunks 3 to 8 % in spills.
+constexpr float kWide = 40.0f;
 
 struct AttendArgs {
     prism_kv_cache c;
@@ -155,6 +164,14 @@ __device__ __forceinline__ void write_row(const AttendArgs &p, uint32_t token, u
     store4(static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * p.c.head_dim + dim, v);
 }
 
+// The sum l of a row whose reference goes up by -by: in two steps, since 2^by alone may vanish where the result does not.
+__device__ __forceinline__ float scaled_sum(float l, float by) {
+    const float half = __builtin_amdgcn_exp2f(0.5f * by);
+    return l * half * half;
+}
+// What takes the numerator to the row (past 2^114, tens of thousands of keys with values below 2^-93, with fewer bits).
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : kSumUnit / l; }
+
 // What both kernels below share: a wavefront's 16 * NT rows, their queries, statistics and sums.
 // T: type of q and out; LIMBS: binary16 parts of q and of the probabilities (2 for binary32).
 template <typename T, int D, int FMT, int NT>
@@ -169,6 +186,7 @@ struct Rows {
     float kf[NT];                  // base-2 softmax scale of the row's integer-like queries, not negative
     f16x8 qv[LIMBS][NT][KS];
     float m[NT], l[NT];
+    bool wide = false;             // a value scale past kWide has been met (the same in all lanes)
     f32x4 acc[NT][DT];
 
     __device__ __forceinline__ void load(const AttendArgs &p, const Request &q, uint32_t base_row, uint32_t last, uint32_t kvh) {
@@ -258,9 +276,9 @@ struct Rows {
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
                 const float next = fmaxf(m[u], top[u]);
-                const float alpha = next == kNone ? 1.0f : __builtin_amdgcn_exp2f(m[u] - next);
+                const float by = next == kNone ? 0.0f : m[u] - next, alpha = __builtin_amdgcn_exp2f(by);
                 m[u] = next;
-                l[u] *= alpha;
+                l[u] = scaled_sum(l[u], by);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) acc[u][d] *= alpha;
             }
@@ -271,6 +289,21 @@ struct Rows {
             off[u] = lv + kHeadroom - (m[u] == kNone ? 0.0f : m[u]);
             // 0 * -inf would be NaN where a page's keys are all zero and a key is masked.
             ff[u] = f[u] < 0x1p-120f ? 0x1p-120f : f[u];
+        }
+        wide |= __ballot(fabsf(lv) > kWide) != 0;
+        if (__builtin_expect(wide, 0)) {
+            // vs = mantissa 2^e: p / vs = 2^(z - e - m) / mantissa, so that the rounding of log2 vs cancels here as well.
+            const float e = static_cast<float>(__builtin_amdgcn_frexp_expf(vs)), over = 1.0f / __builtin_amdgcn_frexp_mantf(vs);
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const float at = lv - e + (kHeadroom - kSumShift) - (m[u] == kNone ? 0.0f : m[u]);
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][t][i], ff[u], at));
+                l[u] = __builtin_fmaf(sum, over, l[u]);
+            }
         }
     }
     // Probabilities of half `c` of the keys: an operand of the second product.
@@ -289,7 +322,7 @@ struct Rows {
             }
     }
     __device__ __forceinline__ void add(const float (&sum)[NT], float vs) {
-        const float iv = 1.0f / vs;
+        const float iv = wide ? 0.0f : kSumUnit / vs;  // wide: l has the terms already
 #pragma unroll
         for (int u = 0; u < NT; ++u) l[u] += sum[u] == 0.0f ? 0.0f : sum[u] * iv;
     }
@@ -304,7 +337,7 @@ struct Rows {
         for (int t = 0; t < NT; ++t) {
             if (!live[t]) continue;
             if (parts == 1) {
-                const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+                const float inv = inverse(l[t]);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) write_row<T>(p, token[t], head[t], 16 * d + 4 * g, acc[t][d] * inv, &bad);
             } else {
@@ -519,13 +552,13 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
         for (int w = 1; w < 4; ++w) top = fmaxf(top, join_ml[w][16 * t + n][0]);
         const float ref = top == kNone ? 0.0f : top;
         const float mine = __builtin_amdgcn_exp2f(rows.m[t] - ref);
-        rows.l[t] *= mine;
+        rows.l[t] = scaled_sum(rows.l[t], rows.m[t] - ref);
 #pragma unroll
         for (int d = 0; d < DT; ++d) rows.acc[t][d] *= mine;
 #pragma unroll
         for (int w = 1; w < 4; ++w) {
             const float other = __builtin_amdgcn_exp2f(join_ml[w][16 * t + n][0] - ref);
-            rows.l[t] += other * join_ml[w][16 * t + n][1];
+            rows.l[t] += scaled_sum(join_ml[w][16 * t + n][1], join_ml[w][16 * t + n][0] - ref);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const f32x4 v = join_acc[w - 1][t * DT + d][lane];
@@ -715,7 +748,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
             const float w = s0 + u < parts ? __builtin_amdgcn_exp2f(f[u] - ref) : 0.0f;
             // A part no key of which the row sees has sums of zero; those of a duplicate count for nothing.
             if (s0 + u < parts) {
-                l = __builtin_fmaf(pl[u], w, l);
+                l += scaled_sum(pl[u], f[u] - ref);
 #pragma unroll
                 for (int i = 0; i < E; ++i) acc[i] = __builtin_fmaf(v[u][i], w, acc[i]);
             }
@@ -737,7 +770,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
             for (int i = 0; i < E; ++i) acc[i] += join[w][E * lane + i];
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = inverse(l);
     bool bad = false;
     T *out = static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * D + E * lane;
 #pragma unroll

@@ -823,6 +823,50 @@ def test_gpu_attention_flags_results_past_the_type(ctx, added, n, dtype, scale):
             assert (np.abs(got - want) <= (so.HALF[dtype] + 2.0 ** -20) * want).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("added,longest", [(2, 300), (2, 20000), (40, 300), (40, 20000)], ids=["rows", "rows-split", "tile", "tile-split"])
+@pytest.mark.parametrize("big", [2.0 ** 38, 2.0 ** 110])
+@pytest.mark.parametrize("order", ["zeros first", "zeros last", "mixed", "random"])
+def test_gpu_attention_value_scales_far_apart(ctx, order, big, added, longest, dtype):
+    """Pages of zeros, whose scale is the smallest, beside pages of large values: their keys weigh as much as any."""
+    rng = np.random.default_rng(22)
+    page, d, heads, kv, n = 16, 64, 4, 1, 700
+    table, pages = make_table(rng, [n], page)
+    cache = make_cache(rng, pages, kv, page, d, "int8")
+    cache["k_scale"][:] = 2.0 ** -7
+    cols = np.arange(-(-n // page))
+    zero = {"zeros first": cols < 22, "zeros last": cols >= 22, "mixed": cols % 3 == 0, "random": rng.random(len(cols)) < 0.1}[order]
+    used = table[0, : len(cols)]
+    cache["v_scale"][used, 0] = big
+    if order == "random":
+        cache["v_scale"][used, 0] = np.float32(1.3) * np.float32(2.0) ** rng.integers(-95, int(np.log2(big)), len(cols)).astype(np.float32)
+    cache["v"][used[zero]], cache["v_scale"][used[zero]] = 0, 2.0 ** -100
+    q = Rows(rng.standard_normal((added, heads, d)), dtype)
+    held = Device(cache, page)
+    for causal in (True, False):
+        call, out = attend(ctx, held, q, [0, added], [n], table, d ** -0.5, causal, max_length=longest)
+        assert ctx.sync() == 0
+        want, tol = so.attention(cache, q.x, [0, added], [n], table, page, d ** -0.5, causal, dtype=dtype)
+        check(out.read(), want, tol)
+
+
+@pytest.mark.parametrize("added", [1, 20])
+def test_gpu_attention_a_long_cache_of_zeros(ctx, added):
+    """A million keys whose values are zero, then sixteen that are not: every key weighs the same."""
+    page, d, heads, kv, columns = 16, 64, 4, 1, (1 << 16) + 1
+    cache = make_cache(np.random.default_rng(23), 2, kv, page, d, "int8")
+    cache["k"][:], cache["v"][0], cache["v"][1] = 0, 0, 64
+    cache["v_scale"][:, 0] = 2.0 ** -100, 1.0
+    table = np.zeros((1, columns), np.int32)
+    table[0, -1] = 1
+    q = Rows(np.ones((added, heads, d)), "f32")
+    n = columns * page
+    call, out = attend(ctx, Device(cache, page), q, [0, added], [n], table, 0.125, False, max_length=1)  # one part
+    assert ctx.sync() == 0
+    # Sums of equal powers of two: an ulp of exp2 and the division are all that rounds.
+    assert (np.abs(out.read() * n / 1024 - 1) <= 2.0 ** -20).all()
+
+
 # ---- together ---------------------------------------------------------------------------------
 
 
