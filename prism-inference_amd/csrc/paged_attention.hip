@@ -215,9 +215,9 @@ struct Rows {
                 for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(x[j][k]));
             }
             most = across_max(most);
-            // A power of two takes the row's largest value to [2^13, 2^14); the sign of the scale goes along.
+            // A power of two, at most 2^113, takes the row's largest value to [2^13, 2^14); the sign of the scale goes along.
             int e = static_cast<int>(__float_as_uint(most) >> 23 & 255) - 127;
-            e = !finite(most) || e < -100 ? 0 : e;
+            e = !finite(most) ? 0 : max(e, -100);
             float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
             if (p.a.scale < 0.0f) up = -up;
             kf[t] = fabsf(p.a.scale) * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);

@@ -867,6 +867,25 @@ def test_gpu_attention_a_long_cache_of_zeros(ctx, added):
     assert (np.abs(out.read() * n / 1024 - 1) <= 2.0 ** -20).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("added", [2, 40])
+def test_gpu_attention_of_tiny_queries(ctx, added, dtype):
+    """Queries below 2^-100 under a scale that brings their scores to one."""
+    rng = np.random.default_rng(24)
+    page, d, heads, kv, n = 16, 128, 4, 1, 200
+    table, pages = make_table(rng, [n], page)
+    cache = make_cache(rng, pages, kv, page, d, "int8")
+    cache["k_scale"] *= 0.25
+    held = Device(cache, page)
+    for power in (-98, -106, -112):
+        q = Rows(rng.standard_normal((added, heads, d)) * 2.0 ** power, dtype)
+        scale = float(np.float32(d ** -0.5)) * 2.0 ** -power
+        call, out = attend(ctx, held, q, [0, added], [n], table, scale)
+        assert ctx.sync() == 0
+        want, tol = so.attention(cache, q.x, [0, added], [n], table, page, scale, dtype=dtype)
+        check(out.read(), want, tol)
+
+
 # ---- together ---------------------------------------------------------------------------------
 
 
