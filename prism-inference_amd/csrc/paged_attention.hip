@@ -488,7 +488,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
         const int32_t base = static_cast<int32_t>(64 * b), key = base + 16 * static_cast<int32_t>(g);
         const bool there = there_next;
         const float ks = there ? ks_next : 0.0f, vs = value_scale(vs_next, there);
-        const bool edge = base < rows.all_lo || base + 64 > rows.all_hi || __ballot(there) != ~0ull;
+        const bool edge = base < rows.all_lo || base > rows.all_hi - 64 || __ballot(there) != ~0ull;
         f32x4 s[NT][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -655,8 +655,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
             if (b + 2 < tile.b1) look(b + 2);
         }
         const int32_t base = static_cast<int32_t>(64 * b);
-        if (!idle && base < rows.any_hi && base + 64 > rows.any_lo) {
-            const bool edge = base < rows.all_lo || base + 64 > rows.all_hi || __ballot(there) != ~0ull;
+        if (!idle && base < rows.any_hi && base > rows.any_lo - 64) {  // base + 64 may be 2^31
+            const bool edge = base < rows.all_lo || base > rows.all_hi - 64 || __ballot(there) != ~0ull;
             // Products of one step of dimensions, four key tiles by NT row tiles, do not wait for each other.
             f32x4 s[NT][4];
 #pragma unroll

@@ -886,6 +886,30 @@ def test_gpu_attention_of_tiny_queries(ctx, added, dtype):
         check(out.read(), want, tol)
 
 
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("added", [1, 40])
+def test_gpu_attention_at_the_longest_length(ctx, added, page):
+    """The last positions below 2^31, through a window: the columns before it are not even there to be read."""
+    rng = np.random.default_rng(25)
+    d, heads, kv, window = 64, 4, 1, 150
+    columns = (2 ** 31 - 1) // page
+    n, near = columns * page, 640 + 64 - page  # the same place in a block of 64 keys
+    table, pages = make_table(rng, [near], page)
+    cache = make_cache(rng, pages, kv, page, d, "int8")
+    held = Device(cache, page)
+    q = Rows(rng.standard_normal((added, heads, d)), "f32")
+    want, tol = so.attention(cache, q.x, [0, added], [near], table, page, 0.125, True, window)
+    big = DeviceBuffer(columns * 4)
+    tail = np.ascontiguousarray(table[0, : near // page])
+    big.upload(tail, (columns - len(tail)) * 4)
+    out = Rows(np.full(q.shape, 3.0), "f32")
+    ctx.attention_device(held.desc, ph.Attention(dtype=ph.DTYPE_F32, requests=1, tokens=added, heads=heads, max_pages=columns, max_length=n, q=q,
+                                                 q_stride=q.stride, out=out, out_stride=out.stride, offsets=i32([0, added]), lengths=i32([n]),
+                                                 block_table=big, scale=0.125, causal=1, window=window))
+    assert ctx.sync() == 0
+    check(out.read(), want, tol)
+
+
 # ---- together ---------------------------------------------------------------------------------
 
 
