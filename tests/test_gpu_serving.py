@@ -910,6 +910,72 @@ def test_gpu_attention_at_the_longest_length(ctx, added, page):
     check(out.read(), want, tol)
 
 
+@pytest.mark.parametrize("alias", [False, True])
+@pytest.mark.parametrize("tokens", ["few", "many"])
+def test_gpu_plan_of_many_requests_without_tokens(ctx, tokens, alias):
+    """More requests than one workgroup's LDS holds, hundreds in a row without a token."""
+    r, page = 6000, 16
+    rng = np.random.default_rng(26)
+    lengths, added, table, free, count = make_plan(rng, r, page, 40, 3)
+    added[:] = 0
+    added[[0, 1, 70, 199, 200, 700, 5998]] = [3, 1, 2, 1, 40, 1, 5] if tokens == "few" else [3, 700, 2, 1, 4000, 1, 500]
+    added[[5, 300, 5999]] = -1
+    columns = -(-int((lengths + added).max()) // page)
+    table = np.concatenate([table, np.full((r, columns), -1, np.int32)], 1)
+    free = np.concatenate([free[:count], np.arange(len(free), len(free) + 400, dtype=np.int32), free[count:]])
+    count += 400
+    room = int(np.maximum(added, 0).sum()) + 130
+    case = lengths, added, table, free, count
+    rc, got = run_plan(ctx, *case, page, room, alias)
+    assert rc == 0
+    for g, w in zip(got, so.plan(*case, page, room)):
+        assert np.array_equal(g, np.asarray(w))
+
+
+@pytest.mark.parametrize("dtype,fmt,d,heads,kv,added", [("f32", "e4m3", 128, 24, 8, 8), ("bf16", "e4m3", 64, 48, 16, 7), ("f16", "int8", 128, 16, 8, 12),
+                                                       ("bf16", "int8", 256, 8, 4, 1), ("f32", "e4m3", 256, 8, 4, 3), ("f16", "e4m3", 256, 8, 4, 40)])
+def test_gpu_attention_past_32_bits_in_every_form(ctx, dtype, fmt, d, heads, kv, added):
+    """One and two row tiles and whole tiles over codes of 4.4 GB."""
+    rng = np.random.default_rng(27)
+    page, n = 256, 900
+    unit = kv * page * d
+    pages = (1 << 32) // unit + 700
+    used = np.array([pages - 1, 3, pages - 500, (1 << 32) // unit], np.int32)
+    small = make_cache(rng, len(used), kv, page, d, fmt)
+    small["k_scale"] *= 0.25 if fmt == "int8" else 0.0625
+    buf = {"k": DeviceBuffer(pages * unit), "v": DeviceBuffer(pages * unit), "k_scale": DeviceBuffer(pages * kv * 4), "v_scale": DeviceBuffer(pages * kv * 4)}
+    for name, b in buf.items():
+        for i, p in enumerate(used):
+            b.upload(np.ascontiguousarray(small[name][i]), int(p) * (unit if name in "kv" else kv * 4))
+
+    class Held:
+        desc = ph.KvCache(**buf, format=FORMAT[fmt], pages=pages, page_size=page, kv_heads=kv, head_dim=d)
+
+    q = Rows(rng.standard_normal((added, heads, d)), dtype)
+    call, out = attend(ctx, Held, q, [0, added], [n], used[None], d ** -0.5)
+    assert ctx.sync() == 0
+    want, tol = so.attention(small, q.x, [0, added], [n], np.arange(len(used))[None], page, d ** -0.5, dtype=dtype)
+    check(out.read(), want, tol)
+
+
+@pytest.mark.parametrize("batch,longest", [("step", 500), ("step", 20000), ("drafts", 4000), ("mixed", 333), ("prompt", 20000)])
+def test_gpu_attention_repeats_itself(ctx, batch, longest):
+    """The same call gives the same bits, split or not."""
+    rng = np.random.default_rng(28)
+    added, lengths = (list(x) for x in zip(*BATCHES[batch]))
+    offsets, page, d, heads, kv = np.concatenate([[0], np.cumsum(added)]), 16, 128, 8, 2
+    table, pages = make_table(rng, lengths, page)
+    held = Device(make_cache(rng, pages, kv, page, d, "int8"), page)
+    q = Rows(rng.standard_normal((offsets[-1], heads, d)), "f16")
+    first = None
+    for _ in range(5):
+        call, out = attend(ctx, held, q, offsets, lengths, table, d ** -0.5, max_length=longest)
+        assert ctx.sync() == 0
+        got = out.read()
+        first = got if first is None else first
+        assert np.array_equal(got, first)
+
+
 # ---- together ---------------------------------------------------------------------------------
 
 
