@@ -368,7 +368,7 @@ typedef struct prism_kv_cache {
     uint32_t pages, page_size, kv_heads, head_dim;
 } prism_kv_cache;
 
-/* One step of `requests` requests: pages, positions and slots of their new tokens.
+/* One step of `requests` (1 to 2^23) requests: pages, positions and slots of their new tokens.
  *   lengths[r]  tokens of request r in the cache; added[r] its new tokens, or -1: the
  *               request has ended and gives back the pages of its lengths[r] tokens.
  *   block_table [requests][max_pages]: column j holds the page of positions
@@ -428,10 +428,11 @@ int prism_hip_rope_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, int dt
  *   tokens: code(x / s), ties to even; where s grew, the codes of the places before the
  *   first new one become code(code * old scale / s).  Other places keep their bytes.
  * Scales the append makes are powers of two, so a page is rescaled by whole bits and
- * however often it grows loses less than one step of its last scale.
+ * however often it grows loses less than one step of its last scale.  (Where a page came with a
+ * scale of the caller's that is none, the quotients are products with 1 / s in binary32.)
  * Slots: -1 writes nothing (padding); the new tokens of one page stand together, in
  * consecutive slots.  A slot outside the cache, or a page's token that does not follow the
- * one before it, is not written and PRISM_ERR_INVALID_INPUT at sync; the same page in
+ * one before it and those that follow it, are not written and PRISM_ERR_INVALID_INPUT at sync; the same page in
  * two places of the batch is the caller's error and leaves that page undefined.  A NaN
  * is stored as 0, an infinity as the largest code, and either is PRISM_ERR_NONFINITE. */
 int prism_hip_kv_append_device(prism_hip_ctx *ctx, const prism_kv_cache *cache, int dtype, const void *k,
@@ -465,10 +466,11 @@ int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, 
  * Table columns no row sees are not read.  A page outside the cache among those it does
  * see is left out, and PRISM_ERR_INVALID_INPUT at sync, as are lengths past max_pages
  * pages and offsets out of order; an output that is not finite in its type is PRISM_ERR_NONFINITE.
- * max_length sizes the work split and should bound the lengths (any value is correct).
- * Statistics and sums are binary32.  Codes are exact in the products' binary16 operands; the
- * probabilities, times their page's value scale, are rounded to binary16 (F16, BF16) or enter, as q
- * does, in two binary16 parts (F32), with all their bits down to 2^-25 of the row's largest.
+ * max_length sizes the work split and should bound the lengths (any value is correct); the parts' sums take context
+ * scratch, at most 136 MB for heads of 128 and 270 MB for heads of 256 on 256 CUs.
+ * Statistics and sums are binary32.  Codes are exact in the products' binary16 operands.  F32 q enters in two binary16
+ * parts: 2^-22 of its row's largest value.  A probability times its page's value scale enters in one (F16, BF16) or two
+ * (F32): off by 2^-11 or 2^-22 of itself, and by up to 2^-36 of the row's largest such product.
  * Value scales are 2^-100 to 2^121, as the append makes them, in any mixture (a smaller one counts as 2^-100), key
  * scales positive; requests * kv_heads is at most 2^23, tokens * heads 2^26. */
 typedef struct prism_attention {

@@ -23,8 +23,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities enter the second product as 2^11 2^(z - m), with m at most kSlack below the largest z
-// (rows are rescaled only where it grew by more): at most 2^15, and full binary16 precision for
-// contributions down to 2^-25 of the largest.
+// (rows are rescaled only where it grew by more): at most 2^15.  One binary16 part has its full precision, half a step of
+// 2^-11, for contributions down to 2^-25 of the largest, two have theirs, 2^-22, down to 2^-14; below, and in all, the
+// error is at most 2^-36 of the largest.  One part rounds a 16-bit result's terms no more than the result is rounded.
 constexpr float kHeadroom = 11.0f, kSlack = 4.0f;
 constexpr float kNone = -__builtin_inff();
 // The denominator l is held times 2^-12 relative to the numerator.  A key's term of it is 2^(S - m + 11 - 12): with value
@@ -436,7 +437,8 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
     // first product and its values behind the second; its table entries are a block further ahead.
     // Heads of 256, and two row tiles of binary32 at 128, have no registers for that (spilled: 205 us instead of 153
     // for eight long requests, 206 instead of 91 for 24 rows a request): their codes are loaded at the
-    // block's start, two wavefronts a SIMD covering each other.
+    // block's start, two wavefronts a SIMD covering each other; binary32 with heads of 256 has registers for one
+    // wavefront only, and four values spilled to accumulation registers (171 us where the 16-bit types take 151).
     constexpr bool kAhead = D < 256 && !(D == 128 && NT == 2 && LIMBS == 2);
     int32_t id_k = 0, id_v = 0;
     u32x4 kraw[4][D / 64], vraw[DT];
@@ -575,8 +577,10 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 // converted to binary16 once by the workgroup, a quarter by each wavefront, into LDS in the order of the
 // operands (a fragment is 16 consecutive bytes a lane: no bank conflicts); the next block's codes
 // come from memory meanwhile and are converted behind the products, so a block costs one barrier.
-// A prompt of 8192 tokens (32 heads of 128 on 8) takes 610 us, 901 TFLOP/s: VALU issue fills 56 % of the cycles (some 380
-// instructions a block and wavefront, 80 of them conversions), the matrix cores 37 %.  Converting in every
+// A prompt of 8192 tokens (32 heads of 128 on 8) takes 617 to 624 us, 881 TFLOP/s: VALU issue fills 56 % of the cycles (some 390
+// instructions a block and wavefront, 80 of them conversions), the matrix cores 37 %; 248 registers leave two wavefronts a
+// SIMD.  Binary32 at 128 takes 976 us (both products twice; eight registers spilled), heads of 64 477 us,
+// heads of 256 2040 us (one wavefront a SIMD).  Converting in every
 // wavefront took 1240 us, eight wavefronts a workgroup 827 where four took 755.
 template <typename T, int D, int FMT, int NT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArgs p, int *err) {
@@ -791,6 +795,10 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     const uint32_t group = a.heads / c.kv_heads;
     const uint64_t typical = (static_cast<uint64_t>(a.tokens) * group + a.requests - 1) / a.requests;  // rows of a request
     Plan p;
+    // 16 requests of 4000 keys, heads of 128 in binary16, whole tiles against shared rows: 8 rows a request 52 / 34 us, 24
+    // 51 / 41, 32 51 / 55, 48 87 / 54, 96 93 / 79; 64 requests of 1000 keys 39 / 34, 40 / 45, 39 / 61, 68 / 43, 74 / 72.
+    // Times rise where rows begin another tile, so no one line fits all; binary32 (24 rows 75 / 50, 48 rows 128 / 69) and
+    // heads of 256 (174 / 75, 250 / 120) are for shared rows further up.
     p.shared = typical <= 32;
     p.nt = p.shared && (c.head_dim == 256 || typical <= 16) ? 1 : 2;
     p.M = p.shared ? 16 * p.nt : 64 * p.nt;
