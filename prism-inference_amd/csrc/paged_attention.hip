@@ -165,10 +165,11 @@ __device__ __forceinline__ void write_row(const AttendArgs &p, uint32_t token, u
     store4(static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * p.c.head_dim + dim, v);
 }
 
-// The sum l of a row whose reference goes up by -by: in two steps, since 2^by alone may vanish where the result does not.
+// The sum l of a row whose reference goes up by -by: by 2^by, as its numerator, so that the rounding of 2^by cancels, and in
+// two steps where 2^by nears the smallest normal number and the sum need not.
 __device__ __forceinline__ float scaled_sum(float l, float by) {
-    const float half = __builtin_amdgcn_exp2f(0.5f * by);
-    return l * half * half;
+    const bool deep = by < -100.0f;
+    return l * (deep ? 0x1p-100f : 1.0f) * __builtin_amdgcn_exp2f(deep ? by + 100.0f : by);
 }
 // What takes the numerator to the row (past 2^114, tens of thousands of keys with values below 2^-93, with fewer bits).
 __device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : kSumUnit / l; }
