@@ -35,7 +35,7 @@ constexpr float kSumShift = 12.0f, kSumUnit = 0x1p-12f;
 // While every value scale met is within 2^+-40, the largest p of a row and those of keys that matter to l are less than
 // 2^100 apart, and l takes a key's p over the scale.  Past that p may vanish where the key's weight does not (a page of
 // zeros, scale 2^-100, beside one of 2^38): from there on l's terms are exponentials of their own.  Looking for such
-// scales costs a prompt 1.4 % (608 -> 617 us); a second copy of the loop for them cost long caches and chunks 3 to 8 % in spills.
+// scales costs a prompt 1.4 % (608 -> 617 us, 660 -> 668 on another card); a second copy of the loop for them cost long caches and chunks 3 to 8 % in spills.
 constexpr float kWide = 40.0f;
 
 struct AttendArgs {
@@ -578,7 +578,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 // converted to binary16 once by the workgroup, a quarter by each wavefront, into LDS in the order of the
 // operands (a fragment is 16 consecutive bytes a lane: no bank conflicts); the next block's codes
 // come from memory meanwhile and are converted behind the products, so a block costs one barrier.
-// A prompt of 8192 tokens (32 heads of 128 on 8) takes 617 to 624 us, 881 TFLOP/s: VALU issue fills 56 % of the cycles (some 390
+// A prompt of 8192 tokens (32 heads of 128 on 8) takes 617 to 672 us, card by card, 820 to 890 TFLOP/s: VALU issue fills 56 % of the cycles (some 390
 // instructions a block and wavefront, 80 of them conversions), the matrix cores 37 %; 248 registers leave two wavefronts a
 // SIMD.  Binary32 at 128 takes 976 us (both products twice; eight registers spilled), heads of 64 477 us,
 // heads of 256 2040 us (one wavefront a SIMD).  Converting in every
