@@ -471,7 +471,7 @@ int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, 
  * Statistics and sums are binary32.  Codes are exact in the products' binary16 operands.  F32 q enters in two binary16
  * parts: 2^-22 of its row's largest value.  A probability times its page's value scale enters in one (F16, BF16) or two
  * (F32): off by 2^-11 or 2^-22 of itself, and by up to 2^-36 of the row's largest such product.
- * Value scales are 2^-100 to 2^121, as the append makes them, in any mixture (a smaller one counts as 2^-100), key
+ * Value scales are 2^-100 to 2^122, as the append makes them, in any mixture (a smaller one counts as 2^-100), key
  * scales positive; requests * kv_heads is at most 2^23, tokens * heads 2^26. */
 typedef struct prism_attention {
     int dtype;

@@ -29,13 +29,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeadroom = 11.0f, kSlack = 4.0f;
 constexpr float kNone = -__builtin_inff();
 // The denominator l is held times 2^-12 relative to the numerator.  A key's term of it is 2^(S - m + 11 - 12): with value
-// scales of 2^-100 to 2^121, as the append makes them, S - m of the largest term is between -121 and 104, so
+// scales of 2^-100 to 2^122, as the append makes them, S - m of the largest term is between -122 and 104, so
 // neither the smallest sum leaves binary32's normal numbers nor that of 2^24 keys its range.
 constexpr float kSumShift = 12.0f, kSumUnit = 0x1p-12f;
 // While every value scale met is within 2^+-40, the largest p of a row and those of keys that matter to l are less than
 // 2^100 apart, and l takes a key's p over the scale.  Past that p may vanish where the key's weight does not (a page of
-// zeros, scale 2^-100, beside one of 2^38): from there on l's terms are exponentials of their own.  Looking for such
-// scales costs a prompt 1.4 % (608 -> 617 us, 660 -> 668 on another card); a second copy of the loop for them cost long caches and chunks 3 to 8 % in spills.
+// zeros, scale 2^-100, beside one of 2^38): from there on l's terms are exponentials of their own, relative to the largest
+// S the lane has met (a reference of its own, in LDS: no register is left for it) until the keys are done.  Looking for
+// such scales costs a prompt 1.4 % (627 -> 636 us); a second copy of the loop for them cost long caches and chunks 3 to 8 %.
 constexpr float kWide = 40.0f;
 
 struct AttendArgs {
@@ -165,11 +166,18 @@ __device__ __forceinline__ void write_row(const AttendArgs &p, uint32_t token, u
     store4(static_cast<T *>(p.a.out) + token * p.a.out_stride + static_cast<uint64_t>(head) * p.c.head_dim + dim, v);
 }
 
+// The lane, made where it is used (the mask is opaque, so it is not made ahead): no register holds it meanwhile.
+__device__ __forceinline__ uint32_t this_lane() {
+    uint32_t all = ~0u;
+    asm volatile("" : "+s"(all));
+    return __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u));
+}
 // The sum l of a row whose reference goes up by -by: by 2^by, as its numerator, so that the rounding of 2^by cancels, and in
 // two steps where 2^by nears the smallest normal number and the sum need not.
 __device__ __forceinline__ float scaled_sum(float l, float by) {
     const bool deep = by < -100.0f;
-    return l * (deep ? 0x1p-100f : 1.0f) * __builtin_amdgcn_exp2f(deep ? by + 100.0f : by);
+    const float f = __builtin_amdgcn_exp2f(deep ? 0.5f * by : by);
+    return l * f * (deep ? f : 1.0f);
 }
 // What takes the numerator to the row (past 2^114, tens of thousands of keys with values below 2^-93, with fewer bits).
 __device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : kSumUnit / l; }
@@ -248,9 +256,9 @@ struct Rows {
     }
 
     // Scores s of the lane's 16 keys from `key` on are masked and the statistics follow their maximum; p = 2^(s ff + off).
-    // ks, vs: the scales of their page; edge: some row does not see some key of the block.
+    // ks, vs: the scales of their page; edge: some row does not see some key of the block; ref: the lanes' references of l.
     __device__ __forceinline__ void scores(f32x4 (&s)[NT][4], float ks, float vs, bool there, bool edge, int32_t key, float (&ff)[NT],
-                                           float (&off)[NT]) {
+                                           float (&off)[NT], float (*ref)[64]) {
         const float lv = __builtin_amdgcn_logf(vs);
         float f[NT], top[NT];
         bool grows = false;
@@ -280,7 +288,7 @@ struct Rows {
                 const float next = fmaxf(m[u], top[u]);
                 const float by = next == kNone ? 0.0f : m[u] - next, alpha = __builtin_amdgcn_exp2f(by);
                 m[u] = next;
-                l[u] = scaled_sum(l[u], by);
+                l[u] = wide ? l[u] : scaled_sum(l[u], by);  // wide: l has its own reference
 #pragma unroll
                 for (int d = 0; d < DT; ++d) acc[u][d] *= alpha;
             }
@@ -292,19 +300,30 @@ struct Rows {
             // 0 * -inf would be NaN where a page's keys are all zero and a key is masked.
             ff[u] = f[u] < 0x1p-120f ? 0x1p-120f : f[u];
         }
-        wide |= __ballot(fabsf(lv) > kWide) != 0;
+        if (__builtin_expect(__ballot(fabsf(lv) > kWide) != 0 && !wide, 0)) {
+            wide = true;
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {  // l 2^(m + 1) = mantissa 2^(exponent + m + 1)
+                ref[u][this_lane()] = l[u] == 0.0f ? kNone : m[u] + (kSumShift - kHeadroom) + static_cast<float>(__builtin_amdgcn_frexp_expf(l[u]));
+                l[u] = __builtin_amdgcn_frexp_mantf(l[u]);
+            }
+        }
         if (__builtin_expect(wide, 0)) {
-            // vs = mantissa 2^e: p / vs = 2^(z - e - m) / mantissa, so that the rounding of log2 vs cancels here as well.
-            const float e = static_cast<float>(__builtin_amdgcn_frexp_expf(vs)), over = 1.0f / __builtin_amdgcn_frexp_mantf(vs);
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
-                const float at = lv - e + (kHeadroom - kSumShift) - (m[u] == kNone ? 0.0f : m[u]);
-                float sum = 0.0f;
+                const float before = ref[u][this_lane()];
+                float next = before, sum = 0.0f;
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][t][i], ff[u], at));
-                l[u] = __builtin_fmaf(sum, over, l[u]);
+                    for (int i = 0; i < 4; ++i) next = fmaxf(next, s[u][t][i] * ff[u]);
+                ref[u][this_lane()] = next;
+                next = next == kNone ? 0.0f : next;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][t][i], ff[u], -next));
+                l[u] = __builtin_fmaf(l[u], __builtin_amdgcn_exp2f(before - next), sum);
             }
         }
     }
@@ -327,6 +346,18 @@ struct Rows {
         const float iv = wide ? 0.0f : kSumUnit / vs;  // wide: l has the terms already
 #pragma unroll
         for (int u = 0; u < NT; ++u) l[u] += sum[u] == 0.0f ? 0.0f : sum[u] * iv;
+    }
+
+    // l once the keys are done: the row's, of all four lanes, relative to m.
+    __device__ __forceinline__ void total(const float (*ref)[64]) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            if (wide && l[u] != 0.0f) {
+                const float half = __builtin_amdgcn_exp2f(0.5f * (ref[u][this_lane()] - m[u] + (kHeadroom - kSumShift)));
+                l[u] = l[u] * half * half;
+            }
+            l[u] = across_sum(l[u]);
+        }
     }
 
     // The rows, or with more than one part their unnormalised sums: lane (n, g) has the dimensions
@@ -425,6 +456,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
     constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT;
     __shared__ float join_ml[4][16 * NT][2];
     __shared__ f32x4 join_acc[3][NT * DT][64];
+    __shared__ float sum_ref[4][NT][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = lane & 15, g = lane / 16;
     Tile tile;
@@ -510,7 +542,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
         if (more) fetch_keys(b + 4);
         f16x8 pv[2][LIMBS][NT];
         float ff[NT], off[NT], sum[NT] = {};
-        rows.scores(s, ks, vs, there, edge, key, ff, off);
+        rows.scores(s, ks, vs, there, edge, key, ff, off, sum_ref[wave]);
         rows.template probabilities<0>(s, pv[0], ff, off, sum);
         rows.template probabilities<1>(s, pv[1], ff, off, sum);
         rows.add(sum, vs);
@@ -535,9 +567,9 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
     if (missing) raise_error(err, kErrIndex);
 
     // The four wavefronts' rows join in the first.
+    rows.total(sum_ref[wave]);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        rows.l[t] = across_sum(rows.l[t]);
         if (g == 0) {
             join_ml[wave][16 * t + n][0] = rows.m[t];
             join_ml[wave][16 * t + n][1] = rows.l[t];
@@ -579,8 +611,8 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 // operands (a fragment is 16 consecutive bytes a lane: no bank conflicts); the next block's codes
 // come from memory meanwhile and are converted behind the products, so a block costs one barrier.
 // A prompt of 8192 tokens (32 heads of 128 on 8) takes 617 to 672 us, card by card, 820 to 890 TFLOP/s: VALU issue fills 56 % of the cycles (some 390
-// instructions a block and wavefront, 80 of them conversions), the matrix cores 37 %; 248 registers leave two wavefronts a
-// SIMD.  Binary32 at 128 takes 976 us (both products twice; eight registers spilled), heads of 64 477 us,
+// instructions a block and wavefront, 80 of them conversions), the matrix cores 37 %; 246 registers leave two wavefronts a
+// SIMD.  Binary32 at 128 takes 976 us (both products twice; four registers spilled), heads of 64 477 us,
 // heads of 256 2040 us (one wavefront a SIMD).  Converting in every
 // wavefront took 1240 us, eight wavefronts a workgroup 827 where four took 755.
 template <typename T, int D, int FMT, int NT>
@@ -588,6 +620,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
     typedef Rows<T, D, FMT, NT> R;
     constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT;
     __shared__ f16x8 kf[2][4][KS][64], vf[2][DT][2][64];
+    __shared__ float sum_ref[4][NT][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = lane & 15, g = lane / 16;
     Tile tile;
@@ -675,7 +708,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
                         for (int u = 0; u < NT; ++u) s[u][t] = mfma(kv, rows.qv[i][u][k], k || i ? s[u][t] : f32x4{0, 0, 0, 0});
                 }
             float ff[NT], off[NT], sum[NT] = {};
-            rows.scores(s, ks, vs, there, edge, base + 16 * static_cast<int32_t>(g), ff, off);
+            rows.scores(s, ks, vs, there, edge, base + 16 * static_cast<int32_t>(g), ff, off, sum_ref[wave]);
             f16x8 pv[2][LIMBS][NT];
             rows.template probabilities<0>(s, pv[0], ff, off, sum);
             rows.template probabilities<1>(s, pv[1], ff, off, sum);
@@ -701,8 +734,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend_tile(AttendArg
     }
     if (missing) raise_error(err, kErrIndex);
     if (idle) return;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) rows.l[t] = across_sum(rows.l[t]);
+    rows.total(sum_ref[wave]);
     rows.write(p, tile.parts, blockIdx.z, err);
 }
 

@@ -976,6 +976,30 @@ def test_gpu_attention_repeats_itself(ctx, batch, longest):
         assert np.array_equal(got, first)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("added,longest", [(1, 80), (1, 4000), (40, 80)], ids=["rows", "split", "tile"])
+def test_gpu_attention_of_the_largest_and_smallest_values(ctx, added, longest, fmt):
+    """Appended pages of zeros, of the smallest floats and of the largest, attended together and each kind alone."""
+    rng = np.random.default_rng(29)
+    page, d, heads, kv, n = 16, 64, 4, 1, 80
+    table, pages = make_table(rng, [n], page)
+    cache = make_cache(rng, pages, kv, page, d, fmt)
+    held = Device(cache, page)
+    slots = (table[0, np.arange(n) // page] * page + np.arange(n) % page).astype(np.int32)
+    k = rng.standard_normal((n, kv, d)).astype(np.float32)
+    for kinds in ((0.0, 3.4e38, 1.0, 1e-38, 3.4e38), (0.0,) * 5, (1e-28,) * 5, (3.4e38,) * 5, (1e-20, 0.0, 1e-20, 0.0, 0.0)):
+        v = (rng.choice([-1, 1], (n, kv, d)) * rng.uniform(0.5, 1, (n, kv, d)) * np.repeat(kinds, page)[:, None, None]).astype(np.float32)
+        held = Device(cache, page)
+        ctx.kv_append_device(held.desc, ph.DTYPE_F32, dev(k), kv * d, dev(v), kv * d, dev(slots), n)
+        want_cache = so.append(cache, k, v, slots, page)
+        q = Rows(rng.standard_normal((added, heads, d)), "f32")
+        call, out = attend(ctx, held, q, [0, added], [n], table, d ** -0.5, max_length=longest)
+        assert ctx.sync() == 0
+        held.check(want_cache)
+        want, tol = so.attention(want_cache, q.x, [0, added], [n], table, page, d ** -0.5)
+        check(out.read(), want, tol)
+
+
 # ---- together ---------------------------------------------------------------------------------
 
 
