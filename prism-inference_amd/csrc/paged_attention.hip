@@ -610,7 +610,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 // converted to binary16 once by the workgroup, a quarter by each wavefront, into LDS in the order of the
 // operands (a fragment is 16 consecutive bytes a lane: no bank conflicts); the next block's codes
 // come from memory meanwhile and are converted behind the products, so a block costs one barrier.
-// A prompt of 8192 tokens (32 heads of 128 on 8) takes 617 to 672 us, card by card, 820 to 890 TFLOP/s: VALU issue fills 56 % of the cycles (some 390
+// A prompt of 8192 tokens (32 heads of 128 on 8) takes 617 to 672 us, card by card, 820 to 890 TFLOP/s: VALU issue fills 55 % of the cycles (some 390
 // instructions a block and wavefront, 80 of them conversions), the matrix cores 37 %; 246 registers leave two wavefronts a
 // SIMD.  Binary32 at 128 takes 976 us (both products twice; four registers spilled), heads of 64 477 us,
 // heads of 256 2040 us (one wavefront a SIMD).  Converting in every
