@@ -341,7 +341,7 @@ int prism_hip_sync(prism_hip_ctx *ctx, void *stream);
 /* The context's internal stream (a hipStream_t), for ordering caller work. */
 void *prism_hip_stream(prism_hip_ctx *ctx);
 
-/* ---- serving many requests: the paged 8-bit cache ----------------------------------
+/* ---- serving many requests: the paged cache of 8 or 4 bits a value -------------------
  * What runs between the projections of a batch of requests.  All of it is device memory
  * of the caller's and stream ordered, as the device-pointer calls above: the calls take
  * the context stream, report at the next prism_hip_sync and can be captured once each has
@@ -351,19 +351,34 @@ void *prism_hip_stream(prism_hip_ctx *ctx);
 #define PRISM_DTYPE_F32 0
 #define PRISM_DTYPE_F16 1
 #define PRISM_DTYPE_BF16 2
-/* 8-bit codes: two's complement -127..127, or OCP e4m3 (largest value 448). */
+/* 8-bit codes: two's complement -127..127, or OCP e4m3 (largest value 448).  4-bit codes: OCP
+ * e2m1, a sign and a magnitude of 0, 0.5, 1, 1.5, 2, 3, 4 or 6. */
 #define PRISM_CACHE_INT8 0
 #define PRISM_CACHE_E4M3 1
+#define PRISM_CACHE_E2M1 4
 
 /* One layer's cache of `pages` pages of page_size positions (16, 32, 64, 128 or 256) for
  * kv_heads heads of head_dim (64, 128 or 256) values.  Codes:
  *   k[page][head][position][dimension], v[page][head][dimension][position]
  * (values transposed, so that both products of the attention read runs of bytes); a value
  * is its code times k_scale / v_scale[page][head].  pages * page_size < 2^31.  The memory
- * may start as it is: a page's scales are set when its first position is written. */
+ * may start as it is: a page's scales are set when its first position is written.
+ * PRISM_CACHE_E2M1 has codes of 4 bits, two dimensions a byte, the first of them in its low half, and a
+ * scale for each 32 consecutive dimensions of a position and head, held as the byte e + 127 of 2^e, e -23 to 13:
+ *   k[page][head][position][head_dim / 2], v the same,
+ *   k_exponent / v_exponent[page][head][head_dim / 32][position], aligned to 16 bytes
+ * (4.25 bits a value; every value is one of binary16, of magnitude 2^-24 to 49152).  Each position stands by
+ * itself: its bytes are set when it is written, and no other's change. */
 typedef struct prism_kv_cache {
     void *k, *v;
-    float *k_scale, *v_scale;
+    union {
+        float *k_scale;
+        uint8_t *k_exponent;
+    };
+    union {
+        float *v_scale;
+        uint8_t *v_exponent;
+    };
     uint32_t format; /* PRISM_CACHE_* */
     uint32_t pages, page_size, kv_heads, head_dim;
 } prism_kv_cache;
@@ -434,7 +449,11 @@ int prism_hip_rope_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, int dt
  * consecutive slots.  A slot outside the cache, or a page's token that does not follow the
  * one before it and those that follow it, are not written and PRISM_ERR_INVALID_INPUT at sync; the same page in
  * two places of the batch is the caller's error and leaves that page undefined.  A NaN
- * is stored as 0, an infinity as the largest code, and either is PRISM_ERR_NONFINITE. */
+ * is stored as 0, an infinity as the largest code, and either is PRISM_ERR_NONFINITE.
+ * PRISM_CACHE_E2M1: slots in any order; every 32 dimensions of a token and head by themselves, M their
+ * largest magnitude, e the least integer from -23 to 13 with M <= 6 * 2^e (13 if none): code(x / 2^e), ties to
+ * the even code.  A magnitude past 49152 is stored as the largest code and is PRISM_ERR_NONFINITE, as a NaN (0)
+ * and an infinity are.  The same slot twice in the batch is the caller's error and leaves that slot undefined. */
 int prism_hip_kv_append_device(prism_hip_ctx *ctx, const prism_kv_cache *cache, int dtype, const void *k,
                                uint64_t k_stride, const void *v, uint64_t v_stride, const int32_t *slots,
                                uint32_t tokens, void *stream);
@@ -455,6 +474,13 @@ typedef struct prism_qkv_append {
 int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, const prism_kv_cache *cache,
                                 const prism_qkv_append *step, void *stream);
 
+/* Reads slots of a cache of any format back: k, v [tokens][kv_heads][head_dim] of type dtype, a value its code times
+ * its scale, rounded once.  A slot of -1 leaves its token's rows as they were; so does one outside the cache, with
+ * PRISM_ERR_INVALID_INPUT at sync.  Any order of slots, the same one any number of times.  A value that is not
+ * finite in the type is PRISM_ERR_NONFINITE.  k or v may be NULL (not read).  Strides as for the append. */
+int prism_hip_kv_read_device(prism_hip_ctx *ctx, const prism_kv_cache *cache, int dtype, const int32_t *slots,
+                             uint32_t tokens, void *k, uint64_t k_stride, void *v, uint64_t v_stride, void *stream);
+
 /* Attention of q [tokens][heads][head_dim] over the cache.  Request r has the tokens
  * offsets[r] .. offsets[r + 1] - 1 (offsets ascend from 0 to at most `tokens`; rows behind
  * the last are not written) and the lengths[r] keys and values of its block table row, heads a
@@ -472,7 +498,9 @@ int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, 
  * parts: 2^-22 of its row's largest value.  A probability times its page's value scale enters in one (F16, BF16) or two
  * (F32): off by 2^-11 or 2^-22 of itself, and by up to 2^-36 of the row's largest such product.
  * Value scales are 2^-100 to 2^122, as the append makes them, in any mixture (a smaller one counts as 2^-100), key
- * scales positive; requests * kv_heads is at most 2^23, tokens * heads 2^26. */
+ * scales positive; requests * kv_heads is at most 2^23, tokens * heads 2^26.
+ * PRISM_CACHE_E2M1: a probability by itself enters in one or two parts, off by 2^-11 or 2^-22 of itself and by up to 2^-36
+ * of the row's largest; the scales' bytes are 104 to 140, as the append makes them, wherever a row sees the position. */
 typedef struct prism_attention {
     int dtype;
     uint32_t requests, tokens, heads, max_pages, max_length;
@@ -487,6 +515,33 @@ typedef struct prism_attention {
 } prism_attention;
 int prism_hip_attention_device(prism_hip_ctx *ctx, const prism_kv_cache *cache, const prism_attention *call,
                                void *stream);
+
+/* ---- log probabilities of an answer --------------------------------------------------
+ * What a request asks of the head's logits [tokens][vocab] (rows of type dtype, `stride` elements apart, at least vocab;
+ * vocab 1 to 2^24): with m the row's largest logit and S = sum exp(x - m),
+ *   logprobs[t]     x[targets[t]] - m - log S, the log probability of a given token; 0 for a target of -1 (none)
+ *   entropy[t]      log S - sum exp(x - m) (x - m) / S, in nats
+ *   top_ids[t][i], top_logprobs[t][i]   the `top` (0 to 64) most probable tokens, largest first, equal logits
+ *                   by ascending id (-0 equals 0).
+ * A logit of -infinity is a word left out: its probability is 0, its log probability -infinity, and it is no
+ * alternative; places past the words there are have the id -1 and -infinity.  A row without any word has entropy 0
+ * and every log probability -infinity.  A NaN or +infinity makes its row's results NaN (ids -1) and is
+ * PRISM_ERR_NONFINITE at sync; a target below -1 or from vocab on gives NaN and is PRISM_ERR_INVALID_INPUT.
+ * targets and logprobs are NULL together (no targets), top_ids and top_logprobs where top is 0; entropy may be NULL.
+ * Sums are binary32, without the largest term, so that neither the entropy of a sure row nor its first token's
+ * log probability loses digits.  Rows of few tokens are split over workgroups, whose results take context
+ * scratch.  tokens is at most 2^23.  The reference samples on the host (src/sampling/); this is a design of its own. */
+typedef struct prism_logprobs {
+    int dtype;
+    uint32_t tokens, vocab, top;
+    const void *logits;
+    uint64_t stride;
+    const int32_t *targets;
+    float *logprobs, *entropy;
+    int32_t *top_ids;
+    float *top_logprobs;
+} prism_logprobs;
+int prism_hip_logprobs_device(prism_hip_ctx *ctx, const prism_logprobs *call, void *stream);
 
 /* ---- full-attention decode step ---------------------------------------------------
  * A resident decoder over a context: the layer loop of the reference's Qwen35 graph

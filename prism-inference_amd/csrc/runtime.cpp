@@ -377,7 +377,7 @@ void prism_hip_destroy(prism_hip_ctx *c) {
     if (c->staging.side) (void)hipStreamSynchronize(c->staging.side);
     staging_free(c->staging);
     for (DevBuf *b : {&c->x, &c->act, &c->act2, &c->out, &c->gate, &c->up, &c->h, &c->hr, &c->res, &c->pre, &c->sk, &c->lora, &c->plan,
-                      &c->rope, &c->att})
+                      &c->rope, &c->att, &c->logits})
         if (b->p) (void)hipFree(b->p);
     for (void *p : c->retired) (void)hipFree(p);
     if (c->err) (void)hipFree(c->err);

@@ -85,7 +85,7 @@ struct prism_hip_ctx {
     int64_t next_id = 1;
     int *err = nullptr;  // device error flag
     prism::rt::DevBuf x, act, act2, out, gate, up, h, hr, res, pre, sk, lora;
-    prism::rt::DevBuf plan, rope, att;  // serving.cpp
+    prism::rt::DevBuf plan, rope, att, logits;  // serving.cpp
     // Whether the current device call took one of them, whether a captured one ever did (a graph
     // may hold any of them from then on), and those outgrown since, kept for such graphs.
     bool scratch_used = false, scratch_captured = false;

@@ -1,4 +1,4 @@
-// serve_common.hpp -- element types and 8-bit codes shared by kvcache.hip and paged_attention.hip.
+// serve_common.hpp -- element types and 8-bit codes shared by the kernels between and behind the projections of many requests.
 #pragma once
 
 #include "device_common.hpp"
@@ -7,6 +7,7 @@
 
 namespace prism {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));

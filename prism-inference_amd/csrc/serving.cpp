@@ -1,5 +1,5 @@
-// serving.cpp -- the paged 8-bit cache of the C ABI: argument checks, scratch and launches of
-// kvcache.hip and paged_attention.hip.
+// serving.cpp -- the paged caches of the C ABI and the log probabilities of its answers: argument checks, scratch and
+// launches of kvcache.hip, kvcache4.hip, paged_attention.hip, paged_attention4.hip and logprobs.hip.
 #include <cmath>
 #include <new>
 
@@ -32,7 +32,7 @@ struct OnDevice {
 };
 
 // Bounds that keep every grid below 2^32 work-items.
-constexpr uint64_t kMostTokens = 1u << 23, kMostHeads = 1u << 12, kMostRows = 1u << 26;
+constexpr uint64_t kMostTokens = 1u << 23, kMostHeads = 1u << 12, kMostRows = 1u << 26, kMostWords = 1u << 24;
 
 bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 size_t type_size(int dtype) { return dtype == PRISM_DTYPE_F32 ? 4 : 2; }
@@ -49,13 +49,14 @@ int enter(prism_hip_ctx *c, void *stream, hipStream_t *s) {
 
 int check_cache(prism_hip_ctx *c, const prism_kv_cache *k) {
     if (!k || !k->k || !k->v || !k->k_scale || !k->v_scale) return bad(c, "null cache");
-    if (k->format != PRISM_CACHE_INT8 && k->format != PRISM_CACHE_E4M3) return bad(c, "unknown cache format");
+    const bool four = k->format == PRISM_CACHE_E2M1;
+    if (k->format != PRISM_CACHE_INT8 && k->format != PRISM_CACHE_E4M3 && !four) return bad(c, "unknown cache format");
     if (!head_dim_ok(k->head_dim)) return fail(c, PRISM_ERR_UNSUPPORTED, "cache head_dim must be 64, 128 or 256");
     if (!page_ok(k->page_size)) return fail(c, PRISM_ERR_UNSUPPORTED, "cache page_size must be 16, 32, 64, 128 or 256");
     if (!k->pages || static_cast<uint64_t>(k->pages) * k->page_size > 0x7fffffffull) return bad(c, "cache needs 1 .. 2^31 - 1 positions");
     if (!k->kv_heads || k->kv_heads > kMostHeads) return bad(c, "cache kv_heads out of range");
-    if (!aligned(k->k, 16) || !aligned(k->v, 16) || !aligned(k->k_scale, 4) || !aligned(k->v_scale, 4))
-        return bad(c, "cache codes must be 16-byte aligned");
+    if (!aligned(k->k, 16) || !aligned(k->v, 16) || !aligned(k->k_scale, four ? 16 : 4) || !aligned(k->v_scale, four ? 16 : 4))
+        return bad(c, "cache codes must be 16-byte aligned, scales to theirs");
     return PRISM_OK;
 }
 
@@ -73,6 +74,13 @@ int check_dtype(prism_hip_ctx *c, int dtype) {
 int check_eps(prism_hip_ctx *c, float eps) { return std::isfinite(eps) && eps >= 0.0f ? PRISM_OK : bad(c, "eps must be finite and not negative"); }
 int check_counts(prism_hip_ctx *c, uint64_t tokens, uint64_t heads) {
     return tokens <= kMostTokens && heads && heads <= kMostHeads && tokens * heads <= kMostRows ? PRISM_OK : bad(c, "tokens or heads out of range");
+}
+
+int append(prism_hip_ctx *c, const prism_kv_cache &cache, int dtype, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
+           const int32_t *slots, uint32_t tokens, hipStream_t s) {
+    const int rc = cache.format == PRISM_CACHE_E2M1 ? launch_kv_append4(cache, dtype, k, k_stride, v, v_stride, slots, tokens, c->err, s)
+                                                    : launch_kv_append(cache, dtype, k, k_stride, v, v_stride, slots, tokens, c->err, s);
+    return launch_result(c, rc, "append launch");
 }
 
 int check_rope(prism_hip_ctx *c, const prism_hip_rope *rope, uint32_t head_dim) {
@@ -197,7 +205,7 @@ int prism_hip_kv_append_device(prism_hip_ctx *c, const prism_kv_cache *cache, in
     if (!rc) rc = check_append(c, cache, dtype, k, k_stride, v, v_stride, slots, tokens);
     if (rc || tokens == 0) return rc;
     OnDevice on(c);
-    return launch_result(c, launch_kv_append(*cache, dtype, k, k_stride, v, v_stride, slots, tokens, c->err, s), "append launch");
+    return append(c, *cache, dtype, k, k_stride, v, v_stride, slots, tokens, s);
 }
 
 int prism_hip_qkv_append_device(prism_hip_ctx *c, const prism_hip_rope *rope, const prism_kv_cache *cache, const prism_qkv_append *a,
@@ -226,8 +234,24 @@ int prism_hip_qkv_append_device(prism_hip_ctx *c, const prism_hip_rope *rope, co
     const RopeRows k{a->k, c->rope.p, a->k_stride, width, kv, a->k_norm};
     rc = launch_result(c, launch_rope(a->dtype, rope->rot, q, k, a->positions, a->tokens, d, a->eps, c->err, s), "rotation launch");
     if (rc) return rc;
-    return launch_result(c, launch_kv_append(*cache, a->dtype, c->rope.p, width, a->v, a->v_stride, a->slots, a->tokens, c->err, s),
-                         "append launch");
+    return append(c, *cache, a->dtype, c->rope.p, width, a->v, a->v_stride, a->slots, a->tokens, s);
+}
+
+int prism_hip_kv_read_device(prism_hip_ctx *c, const prism_kv_cache *cache, int dtype, const int32_t *slots, uint32_t tokens, void *k,
+                             uint64_t k_stride, void *v, uint64_t v_stride, void *stream) {
+    hipStream_t s;
+    int rc = enter(c, stream, &s);
+    if (!rc) rc = check_cache(c, cache);
+    if (!rc) rc = check_dtype(c, dtype);
+    if (!rc) rc = check_counts(c, tokens, cache->kv_heads);
+    if (rc || tokens == 0) return rc;
+    if (!k && !v) return bad(c, "null device pointer");
+    if (k) rc = check_rows(c, dtype, k, k_stride, cache->kv_heads, cache->head_dim);
+    if (!rc && v) rc = check_rows(c, dtype, v, v_stride, cache->kv_heads, cache->head_dim);
+    if (!rc && !slots) rc = bad(c, "null device pointer");
+    if (rc) return rc;
+    OnDevice on(c);
+    return launch_result(c, launch_kv_read(*cache, dtype, slots, tokens, k, k_stride, v, v_stride, c->err, s), "cache read launch");
 }
 
 int prism_hip_attention_device(prism_hip_ctx *c, const prism_kv_cache *cache, const prism_attention *a, void *stream) {
@@ -253,10 +277,38 @@ int prism_hip_attention_device(prism_hip_ctx *c, const prism_kv_cache *cache, co
     if (!a->offsets || !a->lengths || !a->block_table) return bad(c, "null device pointer");
     if (a->q == a->out && a->q_stride != a->out_stride) return bad(c, "attention in place needs one stride");
     OnDevice on(c);
-    const size_t need = attention_scratch_bytes(*cache, *a, c->cus);
+    const bool four = cache->format == PRISM_CACHE_E2M1;
+    const size_t need = four ? attention4_scratch_bytes(*cache, *a, c->cus) : attention_scratch_bytes(*cache, *a, c->cus);
     if (need) rc = ensure(c, c->att, need);
     if (rc) return rc;
-    return launch_result(c, launch_attention_paged(*cache, *a, c->att.p, c->cus, c->err, s), "attention launch");
+    return launch_result(c, four ? launch_attention4_paged(*cache, *a, c->att.p, c->cus, c->err, s)
+                                 : launch_attention_paged(*cache, *a, c->att.p, c->cus, c->err, s), "attention launch");
+}
+
+int prism_hip_logprobs_device(prism_hip_ctx *c, const prism_logprobs *a, void *stream) {
+    CaptureNote note(c);
+    hipStream_t s;
+    int rc = enter(c, stream, &s);
+    if (rc) return rc;
+    if (!a) return bad(c, "null call");
+    rc = check_dtype(c, a->dtype);
+    if (rc) return rc;
+    if (a->tokens > kMostTokens || !a->vocab || a->vocab > kMostWords || a->top > 64) return bad(c, "tokens, vocab or top out of range");
+    if (!a->targets != !a->logprobs) return bad(c, "targets and logprobs come together");
+    if (a->top ? !a->top_ids || !a->top_logprobs : a->top_ids || a->top_logprobs) return bad(c, "top_ids and top_logprobs come with top");
+    if (!a->logprobs && !a->entropy && !a->top) return bad(c, "no result asked for");
+    for (const void *p : {static_cast<const void *>(a->targets), static_cast<const void *>(a->logprobs), static_cast<const void *>(a->entropy),
+                          static_cast<const void *>(a->top_ids), static_cast<const void *>(a->top_logprobs)})
+        if (!aligned(p, 4)) return bad(c, "results not aligned to their type");
+    if (a->tokens == 0) return PRISM_OK;
+    if (!a->logits) return bad(c, "null device pointer");
+    if (!aligned(a->logits, type_size(a->dtype))) return bad(c, "rows not aligned to their type");
+    if (a->stride < a->vocab || a->stride > (1ull << 40)) return bad(c, "row stride below vocab");
+    OnDevice on(c);
+    const size_t need = logprobs_scratch_bytes(*a, c->cus);
+    if (need) rc = ensure(c, c->logits, need);
+    if (rc) return rc;
+    return launch_result(c, launch_logprobs(*a, c->logits.p, c->cus, c->err, s), "log probabilities launch");
 }
 
 }  // extern "C"

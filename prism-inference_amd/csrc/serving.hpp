@@ -1,5 +1,6 @@
 // serving.hpp -- launchers of the kernels between the projections of many requests
-// (kvcache.hip, paged_attention.hip), internal to libprism_hip.
+// (kvcache.hip, kvcache4.hip, paged_attention.hip, paged_attention4.hip) and behind their head
+// (logprobs.hip), internal to libprism_hip.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -33,10 +34,24 @@ int launch_rope(int dtype, const Rotation &rot, const RopeRows &a, const RopeRow
                 uint32_t tokens, uint32_t head_dim, float eps, int *err, hipStream_t s);
 int launch_kv_append(const prism_kv_cache &cache, int dtype, const void *k, uint64_t k_stride, const void *v,
                      uint64_t v_stride, const int32_t *slots, uint32_t tokens, int *err, hipStream_t s);
+// The same into a cache of 4 bits a value (kvcache4.hip).
+int launch_kv_append4(const prism_kv_cache &cache, int dtype, const void *k, uint64_t k_stride, const void *v,
+                      uint64_t v_stride, const int32_t *slots, uint32_t tokens, int *err, hipStream_t s);
+// Slots of a cache of any format as rows (k or v may be null).
+int launch_kv_read(const prism_kv_cache &cache, int dtype, const int32_t *slots, uint32_t tokens, void *k, uint64_t k_stride,
+                   void *v, uint64_t v_stride, int *err, hipStream_t s);
 
 // Scratch of an attention call (partial results of key ranges; 0: none).
 size_t attention_scratch_bytes(const prism_kv_cache &cache, const prism_attention &a, uint32_t cus);
 int launch_attention_paged(const prism_kv_cache &cache, const prism_attention &a, void *scratch, uint32_t cus, int *err,
                            hipStream_t s);
+// The same over a cache of 4 bits a value (paged_attention4.hip).
+size_t attention4_scratch_bytes(const prism_kv_cache &cache, const prism_attention &a, uint32_t cus);
+int launch_attention4_paged(const prism_kv_cache &cache, const prism_attention &a, void *scratch, uint32_t cus, int *err,
+                            hipStream_t s);
+
+// Log probabilities of rows of logits (logprobs.hip); scratch of rows split over workgroups (0: none).
+size_t logprobs_scratch_bytes(const prism_logprobs &call, uint32_t cus);
+int launch_logprobs(const prism_logprobs &call, void *scratch, uint32_t cus, int *err, hipStream_t s);
 
 }  // namespace prism

@@ -49,6 +49,7 @@ DTYPE_BF16 = 2
 
 CACHE_INT8 = 0
 CACHE_E4M3 = 1
+CACHE_E2M1 = 4
 
 Q8K_DTYPE = np.dtype([("scale", "<f4"), ("values", "i1", (256,)), ("sums", "<i2", (16,))])
 Q8_DTYPE = np.dtype([("scale", "<f4"), ("sum", "<f4"), ("values", "i1", (32,))])
@@ -136,7 +137,9 @@ def lib() -> ctypes.CDLL:
         "prism_hip_rope_device": (I, [P, P, I, P, U64, P, U32, U32, U32, P, F, P, U64, P]),
         "prism_hip_kv_append_device": (I, [P, P, I, P, U64, P, U64, P, U32, P]),
         "prism_hip_qkv_append_device": (I, [P, P, P, P, P]),
+        "prism_hip_kv_read_device": (I, [P, P, I, P, U32, P, U64, P, U64, P]),
         "prism_hip_attention_device": (I, [P, P, P, P]),
+        "prism_hip_logprobs_device": (I, [P, P, P]),
         "prism_hip_decoder_create": (P, [P, P, U32]),
         "prism_hip_decoder_destroy": (None, [P]),
         "prism_hip_decoder_set_layer": (I, [P, U32, P, P, P, P, P, P, P, P, P]),
@@ -360,7 +363,7 @@ class _Described(ctypes.Structure):
 
 
 class KvCache(_Described):
-    """prism_kv_cache: one layer's paged 8-bit cache."""
+    """prism_kv_cache: one layer's paged cache; the scales of CACHE_E2M1 are its exponent bytes."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
         (n, ctypes.c_uint32) for n in ("format", "pages", "page_size", "kv_heads", "head_dim")]
 
@@ -386,6 +389,13 @@ class Attention(_Described):
         ("q", ctypes.c_void_p), ("q_stride", ctypes.c_uint64), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_uint64)] + [
         (n, ctypes.c_void_p) for n in ("offsets", "lengths", "block_table")] + [
         ("scale", ctypes.c_float), ("causal", ctypes.c_int), ("window", ctypes.c_uint32)]
+
+
+class Logprobs(_Described):
+    """prism_logprobs: given tokens, entropy and alternatives of rows of logits."""
+    _fields_ = [("dtype", ctypes.c_int)] + [(n, ctypes.c_uint32) for n in ("tokens", "vocab", "top")] + [
+        ("logits", ctypes.c_void_p), ("stride", ctypes.c_uint64)] + [
+        (n, ctypes.c_void_p) for n in ("targets", "logprobs", "entropy", "top_ids", "top_logprobs")]
 
 
 def rope_frequencies(dims: int, base: float, factor: float = 1.0, original: float = 0.0, alpha: float = 1.0,
@@ -692,8 +702,15 @@ class Context:
     def qkv_append_device(self, rope: "Rope", cache: KvCache, step: QkvAppend, stream=None):
         self._check(lib().prism_hip_qkv_append_device(self._h, rope.handle, ctypes.byref(cache), ctypes.byref(step), stream))
 
+    def kv_read_device(self, cache: KvCache, dtype: int, slots, tokens: int, k, k_stride: int, v, v_stride: int, stream=None):
+        self._check(lib().prism_hip_kv_read_device(self._h, ctypes.byref(cache), dtype, _ptr(slots), tokens, _ptr(k), k_stride, _ptr(v),
+                                                   v_stride, stream))
+
     def attention_device(self, cache: KvCache, call: Attention, stream=None):
         self._check(lib().prism_hip_attention_device(self._h, ctypes.byref(cache), ctypes.byref(call), stream))
+
+    def logprobs_device(self, call: Logprobs, stream=None):
+        self._check(lib().prism_hip_logprobs_device(self._h, ctypes.byref(call), stream))
 
     def sync(self, stream=None) -> int:
         return lib().prism_hip_sync(self._h, stream)
