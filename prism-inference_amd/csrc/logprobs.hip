@@ -3,9 +3,11 @@
 // A part of a row is held as its largest logit m and, of all its others, s = sum exp(x - m) and t = sum exp(x - m) (x - m), so
 // that log S = log1p(s) and the entropy log1p(s) - t / (1 + s) keep their digits where one word has nearly all the
 // weight.  A wavefront keeps one m for all its lanes: a new largest is rare (the logarithm of the tiles), so the loop over the
-// row has no exchange between lanes, only a look whether any lane has a logit above what is held.
-// The alternatives ride along: a wavefront keeps the largest in a list, and that look is against the last of
-// them.  One pass over the logits, whose bytes bound long rows.
+// row has no exchange between lanes, only a look whether any lane has a logit above m.
+//
+// The alternatives cost that loop one number for each 16 to 256 logits: the largest of a lane's group of them.  The k largest logits
+// are among the groups whose largest is no smaller than the k-th largest of the lanes' largest, a few more than k groups unless
+// many logits are equal, and only these are read again.
 #include "serve_common.hpp"
 
 namespace prism {
@@ -16,6 +18,8 @@ constexpr float kLog2e = 1.4426950408889634f, kNone = -__builtin_inff();
 constexpr uint32_t kEach = 16, kTile = 64 * kEach;  // logits a lane and a wavefront take at a time
 constexpr uint32_t kRoom = 128;                     // of a wavefront's list, twice the most alternatives
 constexpr uint32_t kMostParts = 64;
+constexpr uint32_t kGroups = 16;       // of a lane in a part
+constexpr uint32_t kCandidates = 512;  // groups to read again that a workgroup notes down
 
 struct Softmax {
     float m, s, t;
@@ -94,93 +98,82 @@ struct Largest {
         count = min(count, k);
         if (count == k) least = held[k - 1];
     }
-    // With the largest order of each lane's keys: where k lanes or more have keys of account, none below the k-th
-    // largest of those can be among the k largest of all.  Its bits from the top.
-    __device__ __forceinline__ void raise(uint32_t order) {
-        if (static_cast<uint32_t>(__builtin_popcountll(__ballot(order > static_cast<uint32_t>(least >> 32)))) < k) return;
-        uint32_t at = 0;
-#pragma unroll 1
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-            if (static_cast<uint32_t>(__builtin_popcountll(__ballot(order >= (at | bit)))) >= k) at |= bit;
-        const uint64_t below = (static_cast<uint64_t>(at) << 32) - 1;
-        if (at && below > least) least = below;
-    }
-    // The lanes whose key is above `least`, where there is room for them.
-    __device__ __forceinline__ void put(uint64_t key) {
-        const uint64_t on = __ballot(key > least);
+    // The lanes whose key is above `least`.
+    __device__ __forceinline__ void add(uint64_t key) {
+        uint64_t on = __ballot(key > least);
         if (!on) return;
+        if (count + __builtin_popcountll(on) > kRoom) {
+            keep();
+            on = __ballot(key > least);
+        }
         if (key > least) held[count + __builtin_amdgcn_mbcnt_hi(on >> 32, __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(on), 0u))] = key;
         count += __builtin_popcountll(on);
         settle();
     }
-    // All keys of a tile, key(i) for i < kEach, whose largest order in this lane is `order`.
-    template <typename F>
-    __device__ __forceinline__ void add(uint32_t order, F key) {
-        raise(order);
-        uint32_t some = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) some += __builtin_popcountll(__ballot(key(i) > least));
-        if (count + some <= kRoom) {
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; ++i) put(key(i));
-            return;
-        }
-#pragma unroll 1
-        for (uint32_t i = 0; i < kEach; ++i) {  // many of one size, or rows that rise: sorted as often as it takes
-            uint64_t mine = key(0);
-#pragma unroll
-            for (uint32_t j = 1; j < kEach; ++j) mine = i == j ? key(j) : mine;
-            if (count + __builtin_popcountll(__ballot(mine > least)) > kRoom) keep();
-            put(mine);
-        }
-    }
 };
 
-// The lists of a workgroup's wavefronts, k ordered keys each, as one: into out[k].
+// The keys that a workgroup's wavefronts hold, at most 64 each, as one ordered list of the k largest: a key's place is the
+// number of larger ones.  counts[w] of held[w]; all[] has room for them and for three zeros.
 template <int WAVES>
-__device__ __forceinline__ void merge_lists(uint64_t (*held)[kRoom], uint64_t *out, uint32_t k) {
+__device__ __forceinline__ void merge_lists(const uint64_t (*held)[kRoom], const uint32_t *counts, uint64_t *all, uint64_t *out, uint32_t k) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        before += w < wave ? counts[w] : 0;
+        total += counts[w];
+    }
+    const uint64_t key = lane < counts[wave] ? held[wave][lane] : 0;
+    if (key) all[before + lane] = key;
+    if (threadIdx.x < 3) all[total + threadIdx.x] = 0;
     if (threadIdx.x < k) out[threadIdx.x] = 0;
     __syncthreads();
-    const uint64_t key = lane < k ? held[wave][lane] : 0;
-    uint32_t above = lane;
+    uint32_t above = 0;
+    if (__ballot(key != 0))
+        for (uint32_t i = 0; i < total; i += 4) {
+            uint64_t other[4];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) {
-        const uint64_t *other = held[(wave + w) % WAVES];
-        for (uint32_t i = 0; i < k; i += 4)
+            for (uint32_t j = 0; j < 4; ++j) other[j] = all[i + j];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) above += i + j < k && other[i + j] > key;
-    }
+            for (uint32_t j = 0; j < 4; ++j) above += other[j] > key;
+        }
     if (key && above < k) out[above] = key;
     __syncthreads();
 }
 
 struct LogprobsArgs {
     prism_logprobs a;
-    uint32_t parts, each;  // parts of a row, their logits
-    uint64_t *keys;        // [tokens][parts][top]
-    Softmax *sums;         // [tokens][parts]
+    uint32_t parts, each;    // parts of a row, their logits
+    uint32_t tiles, groups;  // tiles of a lane's group, groups of a lane in a part
+    float *largest;          // [tokens][parts][groups][threads], of rows in parts
+    Softmax *sums;           // [tokens][parts]
 };
 
-// A row's results from its sums and ordered alternatives; one wavefront.
+// The token that a row's log probability is asked of, and its logit; loaded before there is anything to wait for.
+struct Given {
+    int32_t id;
+    float logit;
+};
 template <typename T>
-__device__ __forceinline__ void write_row(const prism_logprobs &a, uint64_t row, Softmax w, const uint64_t *keys, int *err) {
+__device__ __forceinline__ Given given_of(const prism_logprobs &a, uint64_t row) {
+    Given g{-1, 0.0f};
+    if (a.targets) g.id = a.targets[row];
+    if (g.id >= 0 && g.id < static_cast<int64_t>(a.vocab)) g.logit = static_cast<float>(static_cast<const T *>(a.logits)[row * a.stride + g.id]);
+    return g;
+}
+
+// A row's results from its sums and ordered alternatives; one wavefront.
+__device__ __forceinline__ void write_row(const prism_logprobs &a, uint64_t row, Softmax w, Given g, const uint64_t *keys, int *err) {
     const uint32_t lane = threadIdx.x & 63;
     const float nan = __builtin_nanf(""), log_s = log1pf(w.s);
     const bool wrong = !(w.m < __builtin_inff()) || !(w.s >= 0.0f);
     if (lane == 0) {
         if (wrong) raise_error(err, kErrNonfinite);
         if (a.logprobs) {
-            const int32_t id = a.targets[row];
-            float lp = 0.0f;
-            if (id < -1 || id >= static_cast<int64_t>(a.vocab)) {
-                raise_error(err, kErrIndex);
-                lp = nan;
-            } else if (id >= 0) {
-                const float v = static_cast<float>(static_cast<const T *>(a.logits)[row * a.stride + id]);
-                lp = v == kNone ? kNone : (v - w.m) - log_s;
-            }
-            a.logprobs[row] = wrong ? nan : lp;
+            const bool outside = g.id < -1 || g.id >= static_cast<int64_t>(a.vocab);
+            if (outside) raise_error(err, kErrIndex);
+            const float lp = g.logit == kNone ? kNone : (g.logit - w.m) - log_s;
+            a.logprobs[row] = wrong || outside ? nan : g.id < 0 ? 0.0f : lp;
         }
         if (a.entropy) a.entropy[row] = wrong ? nan : w.m == kNone ? 0.0f : log_s - w.t / (1.0f + w.s);
     }
@@ -214,21 +207,139 @@ struct Logits {
     }
 };
 
+constexpr uint32_t kBuckets = 256;  // of lanes, whose largest bound the k-th largest of all
+
+// What finding the alternatives takes of LDS, for WAVES wavefronts.
+template <int WAVES>
+struct Shared {
+    uint64_t held[WAVES][kRoom], all[64 * WAVES + 3], merged[64];
+    uint32_t order[64 * WAVES < kBuckets ? 64 * WAVES : kBuckets], found[kCandidates], counts[WAVES], count;
+};
+template <>
+struct Shared<0> {
+    uint64_t merged[1];
+};
+
+// The row's alternatives into sh.merged, from the largest of its groups: largest[group][thread], `n` groups of the lanes of
+// FROM wavefronts.
+template <typename T, int WAVES, int FROM>
+__device__ __forceinline__ void alternatives(const LogprobsArgs &p, uint64_t row, const float *largest, uint32_t n, Shared<WAVES> &sh) {
+    constexpr uint32_t kThreads = 64 * WAVES, kSide = 64 * FROM, kFlight = 16;  // loads in flight
+    constexpr uint32_t kShare = kThreads / kBuckets > 1 ? kThreads / kBuckets : 1, kOrders = kThreads / kShare / 64;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64), k = p.a.top, all = n * kSide;
+    const T *x = static_cast<const T *>(p.a.logits) + row * p.a.stride;
+    uint32_t most = 0;
+    for (uint32_t i = 0; i < all; i += kFlight * kThreads) {
+        float v[kFlight];
+#pragma unroll
+        for (uint32_t j = 0; j < kFlight; ++j) v[j] = largest[min(i + j * kThreads + tid, all - 1)];
+#pragma unroll
+        for (uint32_t j = 0; j < kFlight; ++j) most = max(most, i + j * kThreads + tid < all ? order_of(v[j]) : 0);  // each in one bucket
+    }
+    uint32_t bucket = most;
+#pragma unroll
+    for (uint32_t d = 1; d < kShare; d *= 2) bucket = max(bucket, static_cast<uint32_t>(__shfl_xor(static_cast<int>(bucket), d)));
+    if (tid % kShare == 0) sh.order[tid / kShare] = bucket;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    // The k-th largest of the buckets' largest, its bits from the top (18 of them: sign, exponent and nine more; what is left out
+    // only lets some more groups in).
+    uint32_t order[kOrders], bound = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kOrders; ++w) order[w] = sh.order[64 * w + lane];
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit >= 1u << 14; bit >>= 1) {
+        uint32_t some = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kOrders; ++w) some += __builtin_popcountll(__ballot(order[w] >= (bound | bit)));
+        if (some >= k) bound |= bit;
+    }
+    const uint32_t least = max(bound, 1u);
+    if (__ballot(most >= least))
+        for (uint32_t i = 0; i < all; i += kFlight * kThreads) {
+            float v[kFlight];
+#pragma unroll
+            for (uint32_t j = 0; j < kFlight; ++j) v[j] = largest[min(i + j * kThreads + tid, all - 1)];
+#pragma unroll
+            for (uint32_t j = 0; j < kFlight; ++j) {
+                const uint32_t code = i + j * kThreads + tid;
+                if (code < all && order_of(v[j]) >= least) {
+                    const uint32_t at = atomicAdd(&sh.count, 1u);
+                    if (at < kCandidates) sh.found[at] = code;
+                }
+            }
+        }
+    __syncthreads();
+    const uint32_t found = sh.count;
+    Largest top;
+    top.init(sh.held[wave], k);
+    top.least = (static_cast<uint64_t>(least) << 32) - 1;
+    const uint32_t log2_tiles = p.tiles <= 1 ? 0 : 32 - __builtin_clz(p.tiles - 1), log2_each = 4 + log2_tiles;
+    // Logit e of a group: its id, and its key.
+    auto id_at = [&](uint32_t code, uint32_t e) -> uint32_t {
+        const uint32_t i = code / kSide, t = code % kSide, run = 16 / sizeof(T), j = e % kEach;
+        const uint32_t tile = i % p.groups * p.tiles + e / kEach;
+        return i / p.groups * p.each + (tile * FROM + t / 64) * kTile + j / run * (64 * run) + t % 64 * run + j % run;
+    };
+    auto key_at = [&](uint32_t code, uint32_t e) -> uint64_t {
+        const uint32_t id = id_at(code, e), end = min(p.a.vocab, (code / kSide / p.groups + 1) * p.each);
+        return e / kEach < p.tiles && id < end ? key_of(static_cast<float>(x[id]), id) : 0;
+    };
+    if (found <= kCandidates) {
+        const uint32_t units = found << log2_each;
+        for (uint32_t u = tid; u < (units + kThreads - 1) / kThreads * kThreads; u += 4 * kThreads) {
+            uint64_t key[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t v = u + j * kThreads;
+                key[j] = v < units ? key_at(sh.found[v >> log2_each], v & ((1u << log2_each) - 1)) : 0;
+            }
+#pragma unroll 1
+            for (uint32_t j = 0; j < 4; ++j) top.add(j == 0 ? key[0] : j == 1 ? key[1] : j == 2 ? key[2] : key[3]);
+        }
+    } else {
+        // Many of one size (words left out by a large negative logit, where fewer than k others are): each wavefront goes
+        // through every WAVES-th run of groups by ascending id and passes those whose best could not be among the k largest.
+        for (uint32_t i = 0; i < all; i += kThreads) {
+            const uint32_t mine = i + tid, order_i = mine < all ? order_of(largest[mine]) : 0;
+            const uint64_t best = order_i ? static_cast<uint64_t>(order_i) << 32 | (0xffffffffu - id_at(mine, 0)) : 0;
+            uint64_t todo = ~0ull;
+            for (;;) {
+                const uint64_t on = __ballot(best > top.least) & todo;
+                if (!on) break;
+                const uint32_t l = static_cast<uint32_t>(__builtin_ctzll(on));
+                todo &= ~(1ull << l);
+                for (uint32_t e = lane; e - lane < 1u << log2_each; e += 64) top.add(e >> log2_each == 0 ? key_at(i + 64 * wave + l, e) : 0);
+            }
+        }
+    }
+    if (top.count > 64) top.keep();
+    if (lane == 0) sh.counts[wave] = top.count;
+    __syncthreads();
+    merge_lists<WAVES>(sh.held, sh.counts, sh.all, sh.merged, k);
+}
+
 // A workgroup takes a part of a row, its wavefronts every WAVES-th tile of it.
 template <typename T, int WAVES, bool TOP>
 __global__ __launch_bounds__(64 * WAVES) void k_logprobs(LogprobsArgs p, int *err) {
-    __shared__ uint64_t held[TOP ? WAVES : 1][kRoom], merged[64];
-    __shared__ float part[WAVES][3];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    __shared__ Shared<TOP ? WAVES : 0> sh;
+    __shared__ float group_largest[TOP ? kGroups : 1][64 * WAVES], part[WAVES][3];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const uint64_t row = blockIdx.x / p.parts;
     const uint32_t which = blockIdx.x % p.parts;
     const uint32_t begin = which * p.each, end = min(p.a.vocab, begin + p.each);
     const T *x = static_cast<const T *>(p.a.logits) + row * p.a.stride;
     Softmax w{kNone, 0.0f, 0.0f};  // s and t of this lane
-    Largest top;
-    top.init(held[TOP ? wave : 0], p.a.top);
     Logits<T> next;
-    uint32_t base = begin + wave * kTile;
+    uint32_t base = begin + wave * kTile, left = p.tiles, group = 0;
+    float largest = kNone;
+    auto note = [&] {  // the largest of a group
+        if (p.parts == 1) group_largest[group][tid] = largest;
+        else p.largest[(static_cast<uint64_t>(blockIdx.x) * p.groups + group) * (64 * WAVES) + tid] = largest;
+        ++group;
+        left = p.tiles;
+        largest = kNone;
+    };
     if (base < end) next.load(x, base, end);
     for (; base < end; base += WAVES * kTile) {
         Logits<T> now = next;
@@ -236,31 +347,31 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(LogprobsArgs p, int *er
         float most = now.v[0];
 #pragma unroll
         for (uint32_t i = 1; i < kEach; ++i) most = fmaxf(most, now.v[i]);
-        // A later word of the size of the last alternative has a higher id.
-        if (__ballot(TOP ? order_of(most) > static_cast<uint32_t>(top.least >> 32) : most > w.m)) {
-            if constexpr (TOP) top.add(order_of(most), [&](uint32_t i) { return key_of(now.v[i], Logits<T>::id(base, i)); });
-            if (__ballot(most > w.m)) {
-                float m = most;
+        if constexpr (TOP) {
+            largest = fmaxf(largest, most);
+            if (--left == 0) note();
+        }
+        if (__ballot(most > w.m)) {
+            float m = most;
 #pragma unroll
-                for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-                if (w.m != kNone) {  // the former largest counts as another word, of lane 0
-                    const float d = w.m - m, e = exp_of(d);
-                    w.t = e * (w.t + d * w.s);
-                    w.s *= e;
-                    if (lane == 0) {
-                        w.s += e;
-                        w.t += e * d;
-                    }
+            for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+            if (w.m != kNone) {  // the former largest counts as another word, of lane 0
+                const float d = w.m - m, e = exp_of(d);
+                w.t = e * (w.t + d * w.s);
+                w.s *= e;
+                if (lane == 0) {
+                    w.s += e;
+                    w.t += e * d;
                 }
-                w.m = m;
-                uint64_t owner = 0;  // one logit of this size stands for m and is left out
+            }
+            w.m = m;
+            uint64_t owner = 0;  // one logit of this size stands for m and is left out
 #pragma unroll
-                for (uint32_t i = 0; i < kEach; ++i) {
-                    const uint64_t on = owner ? 0 : __ballot(now.v[i] == m);
-                    if (on) {
-                        owner = on;
-                        if (lane == static_cast<uint32_t>(__builtin_ctzll(on))) now.v[i] = kNone;
-                    }
+            for (uint32_t i = 0; i < kEach; ++i) {
+                const uint64_t on = owner ? 0 : __ballot(now.v[i] == m);
+                if (on) {
+                    owner = on;
+                    if (lane == static_cast<uint32_t>(__builtin_ctzll(on))) now.v[i] = kNone;
                 }
             }
         }
@@ -275,118 +386,102 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(LogprobsArgs p, int *er
         w.s += (s[0] + s[1]) + (s[2] + s[3]);
         w.t += (t[0] + t[1]) + (t[2] + t[3]);
     }
+    if constexpr (TOP)
+        while (group < p.groups) note();
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         w.s += __shfl_xor(w.s, d);
         w.t += __shfl_xor(w.t, d);
     }
-    if constexpr (TOP) {
-        top.keep();
-        if (top.count < p.a.top && lane >= top.count) held[wave][lane] = 0;
-    }
-    const uint64_t *keys = held[0];
     if constexpr (WAVES > 1) {
         if (lane == 0) {
             part[wave][0] = w.m;
             part[wave][1] = w.s;
             part[wave][2] = w.t;
         }
-        if constexpr (TOP) {
-            __syncthreads();
-            merge_lists<WAVES>(held, merged, p.a.top);
-            keys = merged;
-        } else {
-            __syncthreads();
-        }
-        if (wave) return;
+        __syncthreads();
         w = Softmax{part[0][0], part[0][1], part[0][2]};
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) w = joined(w, Softmax{part[i][0], part[i][1], part[i][2]});
-    } else {
-        settle();
     }
-    if (p.parts == 1) {
-        write_row<T>(p.a, row, w, keys, err);
+    if (p.parts > 1) {
+        if (tid == 0) p.sums[blockIdx.x] = w;
         return;
     }
-    if (lane == 0) p.sums[blockIdx.x] = w;
-    if (TOP && lane < p.a.top) p.keys[static_cast<uint64_t>(blockIdx.x) * p.a.top + lane] = keys[lane];
+    const Given given = given_of<T>(p.a, row);
+    if constexpr (TOP) {
+        __syncthreads();
+        alternatives<T, WAVES, WAVES>(p, row, &group_largest[0][0], p.groups, sh);
+    }
+    if (wave == 0) write_row(p.a, row, w, given, TOP ? sh.merged : nullptr, err);
 }
 
-// A workgroup joins the parts of a row, each wavefront a quarter of their lists first.
+// A workgroup finishes a row that was in parts.
+constexpr int kJoinWaves = 16;
 template <typename T, bool TOP>
-__global__ __launch_bounds__(256) void k_logprobs_join(LogprobsArgs p, int *err) {
-    __shared__ uint64_t held[4][kRoom], merged[64];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+__global__ __launch_bounds__(TOP ? 64 * kJoinWaves : 64) void k_logprobs_join(LogprobsArgs p, int *err) {
+    __shared__ Shared<TOP ? kJoinWaves : 0> sh;
     const uint64_t row = blockIdx.x;
-    if constexpr (TOP) {
-        const uint32_t some = (p.parts + 3) / 4, from = min(p.parts, wave * some), n = (min(p.parts, from + some) - from) * p.a.top;
-        const uint64_t *keys = p.keys + (row * p.parts + from) * p.a.top;
-        uint64_t key[kEach];
-        uint32_t most = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) {
-            key[i] = 64 * i + lane < n ? keys[64 * i + lane] : 0;
-            most = max(most, static_cast<uint32_t>(key[i] >> 32));
-        }
-        Largest top;
-        top.init(held[wave], p.a.top);
-        top.add(most, [&](uint32_t i) { return key[i]; });
-        top.keep();
-        if (lane >= top.count) held[wave][lane] = 0;
-        __syncthreads();
-        merge_lists<4>(held, merged, p.a.top);
-    }
-    if (wave) return;
+    const Given given = given_of<T>(p.a, row);
     Softmax w{kNone, 0.0f, 0.0f};
-    if (lane < p.parts) w = p.sums[row * p.parts + lane];
+    if (threadIdx.x < p.parts) w = p.sums[row * p.parts + threadIdx.x];
+    if constexpr (TOP) alternatives<T, kJoinWaves, 4>(p, row, p.largest + row * p.parts * p.groups * 256, p.parts * p.groups, sh);
+    if (threadIdx.x >= 64) return;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) w = joined(w, Softmax{__shfl_xor(w.m, d), __shfl_xor(w.s, d), __shfl_xor(w.t, d)});
-    write_row<T>(p.a, row, w, merged, err);
+    write_row(p.a, row, w, given, TOP ? sh.merged : nullptr, err);
 }
 
-struct Parts {
-    uint32_t parts, each;
+// How a call runs: wavefronts of a workgroup, parts of a row, and groups.
+struct Plan {
+    uint32_t waves, parts, each, tiles, groups;
 };
-// Rows are split until some 1024 workgroups share the logits, a tile for each wavefront at least.
-Parts parts_of(const prism_logprobs &a) {
-    const uint32_t tiles = (a.vocab + 4 * kTile - 1) / (4 * kTile);
-    uint32_t parts = (1024 + a.tokens - 1) / a.tokens;
+Plan plan_of(const prism_logprobs &a) {
+    Plan p;
+    p.waves = a.vocab <= 4 * kTile ? 1 : 4;
+    const uint32_t tiles = (a.vocab + p.waves * kTile - 1) / (p.waves * kTile);
+    // Rows are split until some 1024 workgroups share the logits, a tile for each wavefront at least.
+    uint32_t parts = p.waves == 1 ? 1 : (1024 + a.tokens - 1) / a.tokens;
     if (parts > tiles) parts = tiles;
     if (parts > kMostParts) parts = kMostParts;
-    const uint32_t some = (tiles + parts - 1) / parts;
-    return Parts{(tiles + some - 1) / some, some * 4 * kTile};
+    uint32_t some = (tiles + parts - 1) / parts;
+    if (some > kGroups * 16) some = kGroups * 16;  // groups of 256 logits at most
+    p.parts = (tiles + some - 1) / some;
+    p.each = some * p.waves * kTile;
+    p.tiles = (some + kGroups - 1) / kGroups;
+    p.groups = (some + p.tiles - 1) / p.tiles;
+    return p;
 }
 
 template <typename T, bool TOP>
-int logprobs_launch(const LogprobsArgs &p, int *err, hipStream_t s) {
+int logprobs_launch(const LogprobsArgs &p, uint32_t waves, int *err, hipStream_t s) {
     const uint32_t grid = p.a.tokens * p.parts;
-    if (p.a.vocab <= 2 * kTile) k_logprobs<T, 1, TOP><<<grid, 64, 0, s>>>(p, err);
+    if (waves == 1) k_logprobs<T, 1, TOP><<<grid, 64, 0, s>>>(p, err);
     else k_logprobs<T, 4, TOP><<<grid, 256, 0, s>>>(p, err);
     const int rc = launch_status();
     if (rc || p.parts == 1) return rc;
-    k_logprobs_join<T, TOP><<<p.a.tokens, 256, 0, s>>>(p, err);
+    k_logprobs_join<T, TOP><<<p.a.tokens, TOP ? 64 * kJoinWaves : 64, 0, s>>>(p, err);
     return launch_status();
 }
 template <typename T>
-int logprobs_typed(const LogprobsArgs &p, int *err, hipStream_t s) {
-    return p.a.top ? logprobs_launch<T, true>(p, err, s) : logprobs_launch<T, false>(p, err, s);
+int logprobs_typed(const LogprobsArgs &p, uint32_t waves, int *err, hipStream_t s) {
+    return p.a.top ? logprobs_launch<T, true>(p, waves, err, s) : logprobs_launch<T, false>(p, waves, err, s);
 }
 
 }  // namespace
 
 size_t logprobs_scratch_bytes(const prism_logprobs &a, uint32_t) {
-    const Parts q = parts_of(a);
-    return q.parts == 1 ? 0 : static_cast<size_t>(a.tokens) * q.parts * (sizeof(uint64_t) * a.top + sizeof(Softmax));
+    const Plan q = plan_of(a);
+    return q.parts == 1 ? 0 : static_cast<size_t>(a.tokens) * q.parts * (sizeof(Softmax) + (a.top ? 4ull * q.groups * 256 : 0));
 }
 
 int launch_logprobs(const prism_logprobs &a, void *scratch, uint32_t, int *err, hipStream_t s) {
-    const Parts q = parts_of(a);
-    LogprobsArgs p{a, q.parts, q.each, static_cast<uint64_t *>(scratch), nullptr};
-    p.sums = reinterpret_cast<Softmax *>(p.keys + static_cast<size_t>(a.tokens) * q.parts * a.top);
-    if (a.dtype == PRISM_DTYPE_F32) return logprobs_typed<float>(p, err, s);
-    if (a.dtype == PRISM_DTYPE_F16) return logprobs_typed<_Float16>(p, err, s);
-    return logprobs_typed<__bf16>(p, err, s);
+    const Plan q = plan_of(a);
+    LogprobsArgs p{a, q.parts, q.each, q.tiles, q.groups, static_cast<float *>(scratch), nullptr};
+    p.sums = reinterpret_cast<Softmax *>(p.largest + (a.top ? static_cast<size_t>(a.tokens) * q.parts * q.groups * 256 : 0));
+    if (a.dtype == PRISM_DTYPE_F32) return logprobs_typed<float>(p, q.waves, err, s);
+    if (a.dtype == PRISM_DTYPE_F16) return logprobs_typed<_Float16>(p, q.waves, err, s);
+    return logprobs_typed<__bf16>(p, q.waves, err, s);
 }
 
 }  // namespace prism
