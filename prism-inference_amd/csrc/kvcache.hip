@@ -2,7 +2,7 @@
 // of a step's new tokens, rotary positions, and the append that quantizes keys and values.
 #include <type_traits>
 
-#include "serve_common.hpp"
+#include "rope_rows.hpp"
 
 namespace prism {
 
@@ -221,122 +221,7 @@ __global__ __launch_bounds__(256) void k_plan_fill(prism_kv_plan p, PlanScratch 
 }
 
 // ---- rotary positions -------------------------------------------------------------------
-// A workgroup rotates kRopeTokens tokens of some heads, a wavefront one token: the workgroup makes
-// their cosines and sines in binary64 first (one pair of them serves every head), then each lane
-// keeps those of its four pairs and takes the heads, several rows in flight.  binary64 FMAs
-// run at the binary32 rate here, so the exact rotation costs no more than a rounded one; memory
-// bounds it: 4099 tokens x 24 heads of 256 bf16 take 24 us, 4.2 TB/s, 8192 x 40 of 128 35 us, 4.8 TB/s
-// (a lane with four elements that looked their partners up, one row in flight: 56 and 137).
-
-constexpr uint32_t kRopeTokens = 4;
-
-__device__ __forceinline__ void rope_table(double (*cs)[128], double (*sn)[128], const Rotation &rot, const int32_t *positions,
-                                           uint32_t nt) {
-    const uint32_t half = rot.dims / 2;
-    for (uint32_t i = threadIdx.x; i < nt * half; i += 256) {
-        const uint32_t t = i / half, k = i % half;
-        double s, c;
-        sincos(static_cast<double>(positions[t]) * rot.freq[k], &s, &c);
-        cs[t][k] = c * rot.magnitude;
-        sn[t][k] = s * rot.magnitude;
-    }
-    __syncthreads();
-}
-
-// dims a multiple of 8: a lane has four pairs of a row (four elements of each half, or eight
-// neighbours where interleaved), or eight elements behind the rotated ones.
-template <typename T, int D, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation rot, const int32_t *positions, uint32_t tokens,
-                                              uint32_t heads_each, double eps, int *err) {
-    constexpr uint32_t kLanes = D / 8, kRows = 64 / kLanes;  // lanes of a row, rows of a wavefront
-    constexpr uint32_t kFlight = 4;                          // row groups whose loads are in flight together
-    __shared__ double cs[kRopeTokens][128], sn[kRopeTokens][128];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, half = rot.dims / 2;
-    const uint32_t t0 = blockIdx.x * kRopeTokens, nt = min(kRopeTokens, tokens - t0);
-    rope_table(cs, sn, rot, positions + t0, nt);
-    if (wave >= nt) return;
-    const uint32_t li = lane % kLanes, t = t0 + wave;
-    const bool turns = 8 * li < rot.dims;
-    // This lane's two runs of four elements.
-    const uint32_t e0 = INTERLEAVED || !turns ? 8 * li : 4 * li, e1 = INTERLEAVED || !turns ? e0 + 4 : e0 + half;
-    double c[4], s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        c[j] = turns ? cs[wave][4 * li + j] : 1.0;
-        s[j] = turns ? sn[wave][4 * li + j] : 0.0;
-    }
-    const uint32_t h0 = blockIdx.y * heads_each, h1 = min(a.heads + b.heads, h0 + heads_each);
-    bool bad = false, over = false;
-    // The heads of a, then those of b.
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        const RopeRows &m = which ? b : a;
-        const uint32_t from = which ? max(h0, a.heads) - a.heads : h0;
-        const uint32_t to = which ? (h1 > a.heads ? h1 - a.heads : 0) : min(h1, a.heads);
-        if (from >= to) continue;
-        f32x4 w0{1, 1, 1, 1}, w1{1, 1, 1, 1};
-        if (m.norm) w0 = load4(m.norm + e0), w1 = load4(m.norm + e1);
-        const T *x = static_cast<const T *>(m.x) + t * m.x_stride;
-        T *out = static_cast<T *>(m.out) + t * m.out_stride;
-        // Row groups whose heads are all there run without a condition; the rest of them (all, where a token has
-        // few heads) leave out the missing ones.  Conditions everywhere cost 24 -> 29 us for 24 heads of
-        // 256, none 64 us instead of 34 for 3 + 1 heads of 64.
-        auto rows = [&](uint32_t base, auto whole) {
-            const uint32_t h = base + lane / kLanes;
-            f32x4 v0[kFlight], v1[kFlight];
-#pragma unroll
-            for (uint32_t u = 0; u < kFlight; ++u) {
-                if (!whole && base + u * kRows >= to) break;
-                const uint32_t hh = min(h + u * kRows, to - 1);
-                v0[u] = load4(x + hh * D + e0);
-                v1[u] = load4(x + hh * D + e1);
-            }
-#pragma unroll
-            for (uint32_t u = 0; u < kFlight; ++u) {
-                if (!whole && base + u * kRows >= to) break;
-                double y[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    bad |= !finite(v0[u][j]) || !finite(v1[u][j]);
-                    y[j] = v0[u][j];
-                    y[4 + j] = v1[u][j];
-                }
-                if (m.norm) {
-                    double q = 0.0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) q = __builtin_fma(y[j], y[j], q);
-#pragma unroll
-                    for (uint32_t d = 1; d < kLanes; d *= 2) q += __shfl_xor(q, d);
-                    const double scale = 1.0 / sqrt(q / D + eps);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        y[j] = y[j] * scale * static_cast<double>(w0[j]);
-                        y[4 + j] = y[4 + j] * scale * static_cast<double>(w1[j]);
-                    }
-                }
-                f32x4 o0, o1;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const double p = INTERLEAVED ? y[2 * j] : y[j], q = INTERLEAVED ? y[2 * j + 1] : y[4 + j];
-                    const float f = static_cast<float>(__builtin_fma(p, c[j], -(q * s[j])));
-                    const float g = static_cast<float>(__builtin_fma(q, c[j], p * s[j]));
-                    if constexpr (INTERLEAVED) (j < 2 ? o0 : o1)[2 * (j & 1)] = f, (j < 2 ? o0 : o1)[2 * (j & 1) + 1] = g;
-                    else o0[j] = f, o1[j] = g;
-                }
-                over |= !fits<T>(o0) || !fits<T>(o1);
-                if (h + u * kRows < to) {
-                    store4(out + (h + u * kRows) * D + e0, o0);
-                    store4(out + (h + u * kRows) * D + e1, o1);
-                }
-            }
-        };
-        uint32_t base = from;
-        for (; base + (kFlight - 1) * kRows < to; base += kRows * kFlight) rows(base, std::true_type());
-        if (base < to) rows(base, std::false_type());
-    }
-    if (bad) raise_error(err, kErrInput);
-    if (over) raise_error(err, kErrNonfinite);
-}
+// Dims that are multiples of 8 take k_rope (rope_rows.hpp).
 
 // Any dims: a lane has four consecutive elements and looks their partners up, one row in flight (4099 tokens x 24 heads of
 // 256 bf16 with 66 dims take 45 us where k_rope takes 20 with 64).
@@ -657,8 +542,8 @@ int rope_typed(const Rotation &rot, const RopeRows &a, const RopeRows &b, const 
     const uint32_t each = ((heads + parts - 1) / parts + least - 1) / least * least;
     const dim3 grid(tiles, (heads + each - 1) / each);
     if (!eights) k_rope_any<T, D><<<grid, 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, err);
-    else if (rot.interleaved) k_rope<T, D, true><<<grid, 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, err);
-    else k_rope<T, D, false><<<grid, 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, err);
+    else if (rot.interleaved) k_rope<T, D, true, NoAppend><<<grid, 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, NoAppend{}, err);
+    else k_rope<T, D, false, NoAppend><<<grid, 256, 0, s>>>(a, b, rot, positions, tokens, each, eps, NoAppend{}, err);
     return launch_status();
 }
 template <typename T>

@@ -3,30 +3,11 @@
 // A value of the 4-bit cache is an e2m1 code times 2^e, with one e for each 32 consecutive dimensions of a token and head.  The
 // scales are powers of two from 2^-23 to 2^13, so every value is one of binary16 and a token's bytes depend on nothing
 // else in the page: no page is rescaled, slots come in any order, and a step's tokens need no common writer.
-#include "serve_common.hpp"
+#include "rope_rows.hpp"
 
 namespace prism {
 
 namespace {
-
-constexpr int kE2m1 = PRISM_CACHE_E2M1;
-constexpr int kLeastExp = -23, kMostExp = 13;
-constexpr uint32_t kGroup = 32;  // dimensions of a scale
-
-// The least e with most <= 6 * 2^e (6 is 1.5 * 2^2), within the format's exponents.
-__device__ __forceinline__ int exponent_of(uint32_t most) {
-    const int e = static_cast<int>(most >> 23) - 127 - 2 + ((most & 0x7fffffu) > 0x400000u ? 1 : 0);
-    return min(max(e, kLeastExp), kMostExp);
-}
-__device__ __forceinline__ float power(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
-
-struct Append4Args {
-    prism_kv_cache c;
-    const void *k, *v;
-    uint64_t k_stride, v_stride;
-    const int32_t *slots;
-    uint32_t tokens;
-};
 
 // A lane has eight consecutive dimensions of one token and head, four lanes a scale.
 template <typename T, int D>
@@ -34,41 +15,16 @@ __global__ __launch_bounds__(256) void k_append4(Append4Args a, int *err) {
     constexpr uint32_t kLanes = D / 8, kRows = 256 / kLanes;
     const uint32_t li = threadIdx.x % kLanes, t = blockIdx.x * kRows + threadIdx.x / kLanes;
     const bool is_v = blockIdx.y >= a.c.kv_heads;
-    const uint32_t head = is_v ? blockIdx.y - a.c.kv_heads : blockIdx.y, ps = a.c.page_size;
-    const int32_t slot = t < a.tokens ? a.slots[t] : -1;
-    const bool there = slot >= 0 && static_cast<uint32_t>(slot) < a.c.pages * ps;
-    if (slot != -1 && !there && head + is_v + li == 0) raise_error(err, kErrIndex);
-    if (!there) return;  // whole rows leave, so the lanes of a scale stay together
+    const uint32_t head = is_v ? blockIdx.y - a.c.kv_heads : blockIdx.y;
+    if (t >= a.tokens) return;
+    bool there, bad = false, over = false;
+    const int32_t slot = slot_of(a, t, &there);
+    if (!there && blockIdx.y + li == 0) raise_error(err, kErrIndex);
+    if (slot < 0) return;  // whole rows leave, so the lanes of a scale stay together
     const T *x = static_cast<const T *>(is_v ? a.v : a.k) + t * (is_v ? a.v_stride : a.k_stride) + static_cast<uint64_t>(head) * D + 8 * li;
-    f32x4 w[2] = {load4(x), load4(x + 4)};
-    uint32_t most = 0;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float v = w[i / 4][i % 4];
-        bad |= !finite(v);
-        if (v != v) w[i / 4][i % 4] = 0.0f;
-        if (finite(v)) most = max(most, __float_as_uint(v) & 0x7fffffffu);
-    }
-    most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 1)));
-    most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 2)));
+    write_codes4<D>(a.c, is_v, head, static_cast<uint32_t>(slot), li, load4(x), load4(x + 4), &bad, &over);
     if (bad) raise_error(err, kErrInput);
-    if (most > __float_as_uint(49152.0f)) raise_error(err, kErrNonfinite);
-    const int e = exponent_of(most);
-    const float scale = power(e), top = 6.0f * scale;
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_fmed3f(w[i / 4][i % 4], -top, top);
-    uint32_t code = 0;
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[0], y[1], scale, 0);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], scale, 1);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[4], y[5], scale, 2);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[6], y[7], scale, 3);
-    const uint32_t place = static_cast<uint32_t>(slot) % ps;
-    const uint64_t unit = static_cast<uint64_t>(static_cast<uint32_t>(slot) / ps) * a.c.kv_heads + head;
-    uint8_t *codes = static_cast<uint8_t *>(is_v ? a.c.v : a.c.k) + (unit * ps + place) * (D / 2);
-    reinterpret_cast<uint32_t *>(codes)[li] = code;
-    if (li % 4 == 0) (is_v ? a.c.v_exponent : a.c.k_exponent)[(unit * (D / kGroup) + li / 4) * ps + place] = static_cast<uint8_t>(e + 127);
+    if (over) raise_error(err, kErrNonfinite);
 }
 
 struct ReadArgs {
@@ -135,6 +91,31 @@ int append4_typed(const Append4Args &a, int *err, hipStream_t s) {
     return launch_status();
 }
 
+template <typename T, int D>
+int qkv4_typed(const Rotation &rot, const RopeRows &q, const RopeRows &k, const int32_t *positions, float eps, const Append4Args &a, int *err,
+               hipStream_t s) {
+    const uint32_t tiles = (a.tokens + kRopeTokens - 1) / kRopeTokens, heads = q.heads + 2 * k.heads;
+    // Heads are split over workgroups until some 1024 of them share the rows, whole row groups each.
+    constexpr uint32_t least = 64 / (D / 8);
+    uint32_t parts = (1024 + tiles - 1) / tiles;
+    if (parts > (heads + least - 1) / least) parts = (heads + least - 1) / least;
+    const uint32_t each = ((heads + parts - 1) / parts + least - 1) / least * least;
+    const dim3 grid(tiles, (heads + each - 1) / each);
+    if (rot.interleaved) k_rope<T, D, true><<<grid, 256, 0, s>>>(q, k, rot, positions, a.tokens, each, eps, a, err);
+    else k_rope<T, D, false><<<grid, 256, 0, s>>>(q, k, rot, positions, a.tokens, each, eps, a, err);
+    return launch_status();
+}
+template <typename T>
+int qkv4_headed(const Rotation &rot, const RopeRows &q, const RopeRows &k, const int32_t *positions, float eps, const Append4Args &a, int *err,
+                hipStream_t s) {
+    switch (a.c.head_dim) {
+    case 64: return qkv4_typed<T, 64>(rot, q, k, positions, eps, a, err, s);
+    case 128: return qkv4_typed<T, 128>(rot, q, k, positions, eps, a, err, s);
+    case 256: return qkv4_typed<T, 256>(rot, q, k, positions, eps, a, err, s);
+    default: return kLaunchUnsupported;
+    }
+}
+
 template <typename T, int FMT>
 int read_headed(const ReadArgs &a, int *err, hipStream_t s) {
     const uint32_t rows = 256 / (a.c.head_dim / 8);
@@ -162,6 +143,14 @@ int launch_kv_append4(const prism_kv_cache &cache, int dtype, const void *k, uin
     if (dtype == PRISM_DTYPE_F32) return append4_typed<float>(a, err, s);
     if (dtype == PRISM_DTYPE_F16) return append4_typed<_Float16>(a, err, s);
     return append4_typed<__bf16>(a, err, s);
+}
+
+int launch_qkv_append4(const prism_kv_cache &cache, int dtype, const Rotation &rot, const RopeRows &q, const RopeRows &k, const void *v,
+                       uint64_t v_stride, const int32_t *positions, const int32_t *slots, uint32_t tokens, float eps, int *err, hipStream_t s) {
+    const Append4Args a{cache, nullptr, v, 0, v_stride, slots, tokens};
+    if (dtype == PRISM_DTYPE_F32) return qkv4_headed<float>(rot, q, k, positions, eps, a, err, s);
+    if (dtype == PRISM_DTYPE_F16) return qkv4_headed<_Float16>(rot, q, k, positions, eps, a, err, s);
+    return qkv4_headed<__bf16>(rot, q, k, positions, eps, a, err, s);
 }
 
 int launch_kv_read(const prism_kv_cache &cache, int dtype, const int32_t *slots, uint32_t tokens, void *k, uint64_t k_stride, void *v,

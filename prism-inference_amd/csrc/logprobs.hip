@@ -54,12 +54,6 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-// What a wavefront's lanes wrote to LDS is there for the others.
-__device__ __forceinline__ void settle() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // A wavefront's largest keys: `count` of them in LDS, of which at most the k largest matter; keys up to `least` no longer do.
 struct Largest {
     uint64_t *held;  // [kRoom]
@@ -113,7 +107,7 @@ struct Largest {
 };
 
 // The keys that a workgroup's wavefronts hold, at most 64 each, as one ordered list of the k largest: a key's place is the
-// number of larger ones.  counts[w] of held[w]; all[] has room for them and for three zeros.
+// number of larger ones.  counts[w] of held[w]; all[] has room for them and for seven zeros.
 template <int WAVES>
 __device__ __forceinline__ void merge_lists(const uint64_t (*held)[kRoom], const uint32_t *counts, uint64_t *all, uint64_t *out, uint32_t k) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
@@ -125,17 +119,17 @@ __device__ __forceinline__ void merge_lists(const uint64_t (*held)[kRoom], const
     }
     const uint64_t key = lane < counts[wave] ? held[wave][lane] : 0;
     if (key) all[before + lane] = key;
-    if (threadIdx.x < 3) all[total + threadIdx.x] = 0;
+    if (threadIdx.x < 7) all[total + threadIdx.x] = 0;
     if (threadIdx.x < k) out[threadIdx.x] = 0;
     __syncthreads();
     uint32_t above = 0;
     if (__ballot(key != 0))
-        for (uint32_t i = 0; i < total; i += 4) {
-            uint64_t other[4];
+        for (uint32_t i = 0; i < total; i += 8) {
+            uint64_t other[8];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) other[j] = all[i + j];
+            for (uint32_t j = 0; j < 8; ++j) other[j] = all[i + j];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) above += other[j] > key;
+            for (uint32_t j = 0; j < 8; ++j) above += other[j] > key;
         }
     if (key && above < k) out[above] = key;
     __syncthreads();
@@ -162,26 +156,33 @@ __device__ __forceinline__ Given given_of(const prism_logprobs &a, uint64_t row)
     return g;
 }
 
-// A row's results from its sums and ordered alternatives; one wavefront.
-__device__ __forceinline__ void write_row(const prism_logprobs &a, uint64_t row, Softmax w, Given g, const uint64_t *keys, int *err) {
-    const uint32_t lane = threadIdx.x & 63;
-    const float nan = __builtin_nanf(""), log_s = log1pf(w.s);
-    const bool wrong = !(w.m < __builtin_inff()) || !(w.s >= 0.0f);
-    if (lane == 0) {
-        if (wrong) raise_error(err, kErrNonfinite);
+// What a row's log probabilities are taken from.
+struct Scale {
+    float m, log_s;
+    bool wrong;
+};
+// A row's log probability and entropy from its sums, by one wavefront.
+__device__ __forceinline__ Scale write_sums(const prism_logprobs &a, uint64_t row, Softmax w, Given g, int *err) {
+    const float nan = __builtin_nanf("");
+    const Scale r{w.m, log1pf(w.s), !(w.m < __builtin_inff()) || !(w.s >= 0.0f)};
+    if ((threadIdx.x & 63) == 0) {
+        if (r.wrong) raise_error(err, kErrNonfinite);
         if (a.logprobs) {
             const bool outside = g.id < -1 || g.id >= static_cast<int64_t>(a.vocab);
             if (outside) raise_error(err, kErrIndex);
-            const float lp = g.logit == kNone ? kNone : (g.logit - w.m) - log_s;
-            a.logprobs[row] = wrong || outside ? nan : g.id < 0 ? 0.0f : lp;
+            const float lp = g.logit == kNone ? kNone : (g.logit - r.m) - r.log_s;
+            a.logprobs[row] = r.wrong || outside ? nan : g.id < 0 ? 0.0f : lp;
         }
-        if (a.entropy) a.entropy[row] = wrong ? nan : w.m == kNone ? 0.0f : log_s - w.t / (1.0f + w.s);
+        if (a.entropy) a.entropy[row] = r.wrong ? nan : r.m == kNone ? 0.0f : r.log_s - w.t / (1.0f + w.s);
     }
-    if (lane < a.top) {
-        const uint64_t key = keys[lane];
-        a.top_ids[row * a.top + lane] = wrong || !key ? -1 : static_cast<int32_t>(id_of(key));
-        a.top_logprobs[row * a.top + lane] = wrong ? nan : !key ? kNone : (logit_of(key) - w.m) - log_s;
-    }
+    return r;
+}
+// Its alternatives in order; threads 0 to top - 1.
+__device__ __forceinline__ void write_top(const prism_logprobs &a, uint64_t row, const Scale &r, const uint64_t *keys) {
+    if (threadIdx.x >= a.top) return;
+    const uint64_t key = keys[threadIdx.x], at = row * a.top + threadIdx.x;
+    a.top_ids[at] = r.wrong || !key ? -1 : static_cast<int32_t>(id_of(key));
+    a.top_logprobs[at] = r.wrong ? __builtin_nanf("") : !key ? kNone : (logit_of(key) - r.m) - r.log_s;
 }
 
 // One lane's logits of a tile.
@@ -212,29 +213,37 @@ constexpr uint32_t kBuckets = 256;  // of lanes, whose largest bound the k-th la
 // What finding the alternatives takes of LDS, for WAVES wavefronts.
 template <int WAVES>
 struct Shared {
-    uint64_t held[WAVES][kRoom], all[64 * WAVES + 3], merged[64];
-    uint32_t order[64 * WAVES < kBuckets ? 64 * WAVES : kBuckets], found[kCandidates], counts[WAVES], count;
-};
-template <>
-struct Shared<0> {
-    uint64_t merged[1];
+    uint64_t held[WAVES][kRoom], all[64 * WAVES + 7], merged[64];
+    uint32_t order[64 * WAVES < kBuckets ? 64 * WAVES : kBuckets], found[kCandidates], counts[WAVES], count, least;
+    Scale scale;
 };
 
-// The row's alternatives into sh.merged, from the largest of its groups: largest[group][thread], `n` groups of the lanes of
-// FROM wavefronts.
-template <typename T, int WAVES, int FROM>
-__device__ __forceinline__ void alternatives(const LogprobsArgs &p, uint64_t row, const float *largest, uint32_t n, Shared<WAVES> &sh) {
+// The row's alternatives, from the largest of its groups: largest[group][thread], `n` groups of the lanes of FROM
+// wavefronts.  Meanwhile the second wavefront (or the only one) makes sh.scale by `sums`.
+template <typename T, int WAVES, int FROM, typename F>
+__device__ __forceinline__ void alternatives(const LogprobsArgs &p, uint64_t row, const float *largest, uint32_t n, Shared<WAVES> &sh, F sums) {
     constexpr uint32_t kThreads = 64 * WAVES, kSide = 64 * FROM, kFlight = 16;  // loads in flight
     constexpr uint32_t kShare = kThreads / kBuckets > 1 ? kThreads / kBuckets : 1, kOrders = kThreads / kShare / 64;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64), k = p.a.top, all = n * kSide;
     const T *x = static_cast<const T *>(p.a.logits) + row * p.a.stride;
-    uint32_t most = 0;
-    for (uint32_t i = 0; i < all; i += kFlight * kThreads) {
+    uint32_t most = 0, here[kFlight];  // of the first groups, which are all of most rows
+    auto look = [&](uint32_t i, uint32_t(&o)[kFlight]) {
         float v[kFlight];
 #pragma unroll
         for (uint32_t j = 0; j < kFlight; ++j) v[j] = largest[min(i + j * kThreads + tid, all - 1)];
 #pragma unroll
-        for (uint32_t j = 0; j < kFlight; ++j) most = max(most, i + j * kThreads + tid < all ? order_of(v[j]) : 0);  // each in one bucket
+        for (uint32_t j = 0; j < kFlight; ++j) o[j] = i + j * kThreads + tid < all ? order_of(v[j]) : 0;
+    };
+    auto most_of = [&](const uint32_t(&o)[kFlight]) {
+#pragma unroll
+        for (uint32_t j = 0; j < kFlight; ++j) most = max(most, o[j]);
+    };
+    look(0, here);
+    most_of(here);
+    for (uint32_t i = kFlight * kThreads; i < all; i += kFlight * kThreads) {
+        uint32_t more[kFlight];
+        look(i, more);
+        most_of(more);
     }
     uint32_t bucket = most;
 #pragma unroll
@@ -242,33 +251,45 @@ __device__ __forceinline__ void alternatives(const LogprobsArgs &p, uint64_t row
     if (tid % kShare == 0) sh.order[tid / kShare] = bucket;
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    // The k-th largest of the buckets' largest, its bits from the top (18 of them: sign, exponent and nine more; what is left out
-    // only lets some more groups in).
-    uint32_t order[kOrders], bound = 0;
+    // The k-th largest of the buckets' largest, its bits from the top, two at a time (18 of them: sign, exponent and nine more;
+    // what is left out only lets some more groups in).
+    if (wave == 0) {
+        uint32_t order[kOrders], bound = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kOrders; ++w) order[w] = sh.order[64 * w + lane];
+        for (uint32_t w = 0; w < kOrders; ++w) order[w] = sh.order[64 * w + lane];
 #pragma unroll 1
-    for (uint32_t bit = 1u << 31; bit >= 1u << 14; bit >>= 1) {
-        uint32_t some = 0;
+        for (uint32_t bit = 1u << 30; bit >= 1u << 14; bit >>= 2) {
+            uint32_t some[3] = {};
 #pragma unroll
-        for (uint32_t w = 0; w < kOrders; ++w) some += __builtin_popcountll(__ballot(order[w] >= (bound | bit)));
-        if (some >= k) bound |= bit;
-    }
-    const uint32_t least = max(bound, 1u);
-    if (__ballot(most >= least))
-        for (uint32_t i = 0; i < all; i += kFlight * kThreads) {
-            float v[kFlight];
+            for (uint32_t i = 0; i < 3; ++i)
 #pragma unroll
-            for (uint32_t j = 0; j < kFlight; ++j) v[j] = largest[min(i + j * kThreads + tid, all - 1)];
-#pragma unroll
-            for (uint32_t j = 0; j < kFlight; ++j) {
-                const uint32_t code = i + j * kThreads + tid;
-                if (code < all && order_of(v[j]) >= least) {
-                    const uint32_t at = atomicAdd(&sh.count, 1u);
-                    if (at < kCandidates) sh.found[at] = code;
-                }
-            }
+                for (uint32_t w = 0; w < kOrders; ++w) some[i] += __builtin_popcountll(__ballot(order[w] >= (bound | (i + 1) * bit)));
+            bound |= some[2] >= k ? 3 * bit : some[1] >= k ? 2 * bit : some[0] >= k ? bit : 0;
         }
+        if (lane == 0) sh.least = max(bound, 1u);
+    }
+    if (wave == (WAVES > 1 ? 1 : 0)) {
+        const Scale r = sums();
+        if (lane == 0) sh.scale = r;
+    }
+    __syncthreads();
+    const uint32_t least = sh.least;
+    auto note = [&](uint32_t i, const uint32_t(&o)[kFlight]) {
+#pragma unroll
+        for (uint32_t j = 0; j < kFlight; ++j)
+            if (o[j] >= least) {
+                const uint32_t at = atomicAdd(&sh.count, 1u);
+                if (at < kCandidates) sh.found[at] = i + j * kThreads + tid;
+            }
+    };
+    if (__ballot(most >= least)) {
+        note(0, here);
+        for (uint32_t i = kFlight * kThreads; i < all; i += kFlight * kThreads) {
+            uint32_t more[kFlight];
+            look(i, more);
+            note(i, more);
+        }
+    }
     __syncthreads();
     const uint32_t found = sh.count;
     Largest top;
@@ -317,12 +338,12 @@ __device__ __forceinline__ void alternatives(const LogprobsArgs &p, uint64_t row
     if (lane == 0) sh.counts[wave] = top.count;
     __syncthreads();
     merge_lists<WAVES>(sh.held, sh.counts, sh.all, sh.merged, k);
+    write_top(p.a, row, sh.scale, sh.merged);
 }
 
 // A workgroup takes a part of a row, its wavefronts every WAVES-th tile of it.
 template <typename T, int WAVES, bool TOP>
 __global__ __launch_bounds__(64 * WAVES) void k_logprobs(LogprobsArgs p, int *err) {
-    __shared__ Shared<TOP ? WAVES : 0> sh;
     __shared__ float group_largest[TOP ? kGroups : 1][64 * WAVES], part[WAVES][3];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const uint64_t row = blockIdx.x / p.parts;
@@ -399,37 +420,50 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(LogprobsArgs p, int *er
             part[wave][1] = w.s;
             part[wave][2] = w.t;
         }
-        __syncthreads();
-        w = Softmax{part[0][0], part[0][1], part[0][2]};
-#pragma unroll
-        for (int i = 1; i < WAVES; ++i) w = joined(w, Softmax{part[i][0], part[i][1], part[i][2]});
     }
+    __syncthreads();
+    auto joined_parts = [&] {
+        if constexpr (WAVES > 1) {
+            w = Softmax{part[0][0], part[0][1], part[0][2]};
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) w = joined(w, Softmax{part[i][0], part[i][1], part[i][2]});
+        }
+        return w;
+    };
     if (p.parts > 1) {
-        if (tid == 0) p.sums[blockIdx.x] = w;
+        if (tid == 0) p.sums[blockIdx.x] = joined_parts();
         return;
     }
     const Given given = given_of<T>(p.a, row);
+    auto sums = [&] { return write_sums(p.a, row, joined_parts(), given, err); };
     if constexpr (TOP) {
-        __syncthreads();
-        alternatives<T, WAVES, WAVES>(p, row, &group_largest[0][0], p.groups, sh);
+        __shared__ Shared<WAVES> sh;
+        alternatives<T, WAVES, WAVES>(p, row, &group_largest[0][0], p.groups, sh, sums);
+    } else {
+        if (wave == 0) sums();
     }
-    if (wave == 0) write_row(p.a, row, w, given, TOP ? sh.merged : nullptr, err);
 }
 
 // A workgroup finishes a row that was in parts.
 constexpr int kJoinWaves = 16;
 template <typename T, bool TOP>
 __global__ __launch_bounds__(TOP ? 64 * kJoinWaves : 64) void k_logprobs_join(LogprobsArgs p, int *err) {
-    __shared__ Shared<TOP ? kJoinWaves : 0> sh;
+    const uint32_t lane = threadIdx.x & 63;
     const uint64_t row = blockIdx.x;
     const Given given = given_of<T>(p.a, row);
     Softmax w{kNone, 0.0f, 0.0f};
-    if (threadIdx.x < p.parts) w = p.sums[row * p.parts + threadIdx.x];
-    if constexpr (TOP) alternatives<T, kJoinWaves, 4>(p, row, p.largest + row * p.parts * p.groups * 256, p.parts * p.groups, sh);
-    if (threadIdx.x >= 64) return;
+    if (lane < p.parts) w = p.sums[row * p.parts + lane];
+    auto sums = [&] {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) w = joined(w, Softmax{__shfl_xor(w.m, d), __shfl_xor(w.s, d), __shfl_xor(w.t, d)});
-    write_row(p.a, row, w, given, TOP ? sh.merged : nullptr, err);
+        for (int d = 1; d < 64; d *= 2) w = joined(w, Softmax{__shfl_xor(w.m, d), __shfl_xor(w.s, d), __shfl_xor(w.t, d)});
+        return write_sums(p.a, row, w, given, err);
+    };
+    if constexpr (TOP) {
+        __shared__ Shared<kJoinWaves> sh;
+        alternatives<T, kJoinWaves, 4>(p, row, p.largest + row * p.parts * p.groups * 256, p.parts * p.groups, sh, sums);
+    } else {
+        sums();
+    }
 }
 
 // How a call runs: wavefronts of a workgroup, parts of a row, and groups.
@@ -440,8 +474,10 @@ Plan plan_of(const prism_logprobs &a) {
     Plan p;
     p.waves = a.vocab <= 4 * kTile ? 1 : 4;
     const uint32_t tiles = (a.vocab + p.waves * kTile - 1) / (p.waves * kTile);
-    // Rows are split until some 1024 workgroups share the logits, a tile for each wavefront at least.
-    uint32_t parts = p.waves == 1 ? 1 : (1024 + a.tokens - 1) / a.tokens;
+    // Up to 256 rows are split until some 1024 workgroups share the logits, a tile for each wavefront at least; more keep the
+    // memory busy whole (rows of 151936 binary32 logits, 20 alternatives, whole / split: 200 rows 36 / 32 us, 256 42 / 38, 400
+    // 52 / 70, 900 106 / 145).
+    uint32_t parts = p.waves == 1 || a.tokens > 256 ? 1 : (1024 + a.tokens - 1) / a.tokens;
     if (parts > tiles) parts = tiles;
     if (parts > kMostParts) parts = kMostParts;
     uint32_t some = (tiles + parts - 1) / parts;

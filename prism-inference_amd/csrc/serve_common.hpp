@@ -54,6 +54,12 @@ __device__ __forceinline__ bool fits(f32x4 v) {
     return finite(r[0]) && finite(r[1]) && finite(r[2]) && finite(r[3]);
 }
 
+// What a wavefront's lanes wrote to LDS is there for the others.
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 constexpr int kInt8 = PRISM_CACHE_INT8, kE4m3 = PRISM_CACHE_E4M3;
 
 // The codes of four values, ties to even, magnitudes past the format's largest at it.  Not for NaN.

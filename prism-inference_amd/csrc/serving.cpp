@@ -228,9 +228,14 @@ int prism_hip_qkv_append_device(prism_hip_ctx *c, const prism_hip_rope *rope, co
     if (rc) return rc;
     OnDevice on(c);
     const uint64_t width = static_cast<uint64_t>(kv) * d;
+    const RopeRows q{a->q, a->q_out, a->q_stride, a->q_out_stride, a->heads, a->q_norm};
+    if (cache->format == PRISM_CACHE_E2M1 && rope->rot.dims % 8 == 0) {
+        const RopeRows k{a->k, nullptr, a->k_stride, 0, kv, a->k_norm};
+        return launch_result(c, launch_qkv_append4(*cache, a->dtype, rope->rot, q, k, a->v, a->v_stride, a->positions, a->slots, a->tokens, a->eps,
+                                                   c->err, s), "append launch");
+    }
     rc = ensure(c, c->rope, type_size(a->dtype) * width * a->tokens);
     if (rc) return rc;
-    const RopeRows q{a->q, a->q_out, a->q_stride, a->q_out_stride, a->heads, a->q_norm};
     const RopeRows k{a->k, c->rope.p, a->k_stride, width, kv, a->k_norm};
     rc = launch_result(c, launch_rope(a->dtype, rope->rot, q, k, a->positions, a->tokens, d, a->eps, c->err, s), "rotation launch");
     if (rc) return rc;

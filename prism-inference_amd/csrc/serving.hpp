@@ -37,6 +37,9 @@ int launch_kv_append(const prism_kv_cache &cache, int dtype, const void *k, uint
 // The same into a cache of 4 bits a value (kvcache4.hip).
 int launch_kv_append4(const prism_kv_cache &cache, int dtype, const void *k, uint64_t k_stride, const void *v,
                       uint64_t v_stride, const int32_t *slots, uint32_t tokens, int *err, hipStream_t s);
+// Rotated q into memory, rotated k and v into a cache of 4 bits a value, in one launch; dims multiples of 8.
+int launch_qkv_append4(const prism_kv_cache &cache, int dtype, const Rotation &rot, const RopeRows &q, const RopeRows &k, const void *v,
+                       uint64_t v_stride, const int32_t *positions, const int32_t *slots, uint32_t tokens, float eps, int *err, hipStream_t s);
 // Slots of a cache of any format as rows (k or v may be null).
 int launch_kv_read(const prism_kv_cache &cache, int dtype, const int32_t *slots, uint32_t tokens, void *k, uint64_t k_stride,
                    void *v, uint64_t v_stride, int *err, hipStream_t s);
