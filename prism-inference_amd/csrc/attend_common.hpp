@@ -200,6 +200,18 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
     const uint64_t row = uniform(blockIdx.x * (4 / WAVES) + wave / WAVES), all_rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
     if (row >= all_rows) return;
     const uint32_t token = static_cast<uint32_t>(row / p.a.heads), head = static_cast<uint32_t>(row % p.a.heads);
+    // The first four parts are loaded before it is known how many the row has.
+    float f[4], pl[4], v[4][E];
+    auto load = [&](uint32_t s0, uint32_t n) {
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            const uint64_t at = min(s0 + u, n - 1) * all_rows + row;
+            f[u] = p.part_ml[2 * at];
+            pl[u] = p.part_ml[2 * at + 1];
+            __builtin_memcpy(v[u], p.part + at * D + E * lane, sizeof v[u]);
+        }
+    };
+    load(4 * mine, p.splits);
     // The request of the token, 64 candidates at a time.
     uint32_t lo = 0, n = p.a.requests;
     while (n > 1) {
@@ -224,14 +236,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
     const float ref = top == kNone ? 0.0f : top;
     float l = 0.0f, acc[E] = {};
     for (uint32_t s0 = 4 * mine; s0 < parts; s0 += 4 * WAVES) {
-        float f[4], pl[4], v[4][E];
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) {
-            const uint64_t at = min(s0 + u, parts - 1) * all_rows + row;
-            f[u] = p.part_ml[2 * at];
-            pl[u] = p.part_ml[2 * at + 1];
-            __builtin_memcpy(v[u], p.part + at * D + E * lane, sizeof v[u]);
-        }
+        if (s0 != 4 * mine) load(s0, parts);
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
             const float w = s0 + u < parts ? __builtin_amdgcn_exp2f(f[u] - ref) : 0.0f;

@@ -16,6 +16,7 @@
 //      the B operand of the second product as they stand.
 //   V  lane (n, g) has the dimensions [n D/16, (n + 1) D/16) of the same 16 keys: its codes of two keys
 //      are converted two dimensions at a time and their halves swapped (two byte permutations for four values).
+#include <algorithm>
 #include <type_traits>
 
 #include "attend_common.hpp"
@@ -530,8 +531,10 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     if (p.shared) {
         // Some eight workgroups a CU were every request as long as max_length, so that long requests among
         // short ones do not finish last; eight blocks a part at least, two for each wavefront.
-        parts = (blocks + 7) / 8;
+        parts = (blocks + 3) / 4;
         if (parts > 8ull * cus / tiles) parts = 8ull * cus / tiles;
+        const uint64_t more = std::min<uint64_t>(12ull * cus / tiles, blocks * c.head_dim / 6144);
+        if (tiles >= cus && parts < more) parts = more;
     } else {
         parts = blocks / 24;
         if (parts > 8ull * cus / tiles) parts = 8ull * cus / tiles;
