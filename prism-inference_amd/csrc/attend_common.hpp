@@ -191,8 +191,9 @@ __device__ __forceinline__ void keep_bytes(u32x4 &v, int32_t keep) {
 }
 
 // Joins the parts of the rows that have more than one: WAVES wavefronts a row, which share its parts, a lane
-// with D / 64 dimensions; four parts in flight each.
-template <typename T, int D, int WAVES>
+// with D / 64 dimensions; four parts in flight each.  EARLY (single tokens, where most rows have parts and a load's latency
+// counts): the first four are loaded before it is known how many the row has.
+template <typename T, int D, int WAVES, bool EARLY = false>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, int *err) {
     constexpr int E = D / 64;
     __shared__ float join[WAVES > 1 ? 4 : 1][D + 1];
@@ -200,7 +201,6 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
     const uint64_t row = uniform(blockIdx.x * (4 / WAVES) + wave / WAVES), all_rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
     if (row >= all_rows) return;
     const uint32_t token = static_cast<uint32_t>(row / p.a.heads), head = static_cast<uint32_t>(row % p.a.heads);
-    // The first four parts are loaded before it is known how many the row has.
     float f[4], pl[4], v[4][E];
     auto load = [&](uint32_t s0, uint32_t n) {
 #pragma unroll
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
             __builtin_memcpy(v[u], p.part + at * D + E * lane, sizeof v[u]);
         }
     };
-    load(4 * mine, p.splits);
+    if constexpr (EARLY) load(4 * mine, p.splits);
     // The request of the token, 64 candidates at a time.
     uint32_t lo = 0, n = p.a.requests;
     while (n > 1) {
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs p, uint32_t M, i
     const float ref = top == kNone ? 0.0f : top;
     float l = 0.0f, acc[E] = {};
     for (uint32_t s0 = 4 * mine; s0 < parts; s0 += 4 * WAVES) {
-        if (s0 != 4 * mine) load(s0, parts);
+        if (!EARLY || s0 != 4 * mine) load(s0, parts);
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
             const float w = s0 + u < parts ? __builtin_amdgcn_exp2f(f[u] - ref) : 0.0f;

@@ -390,9 +390,10 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 // converted to binary16 once by the workgroup, a quarter of the keys by each wavefront, into LDS in the order of the
 // operands; the next block's codes come from memory meanwhile and are converted behind the products, so a
 // block costs one barrier.
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool WIDE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendArgs p, int *err) {
     typedef Rows4<T, D, NT> R;
+    typedef std::conditional_t<WIDE, uint64_t, uint32_t> Offset;
     constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT, KG = D == 256 ? 2 : 1;
     __shared__ f16x8 kf[2][4][KS][64];
     __shared__ f16x4 vf[2][DT][2][2][64];  // halves of an operand apart: writes of 8 bytes without bank conflicts
@@ -405,50 +406,65 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendAr
     rows.load(p, tile.q, min(tile.row0 + wave * 16 * NT, tile.last), tile.last, kvh);
     const bool idle = tile.row0 + wave * 16 * NT > tile.last;  // converts only
 
-    const uint32_t page_mask = p.c.page_size - 1;
+    const uint32_t page_mask = p.c.page_size - 1, page_log2 = p.page_log2;
     const int32_t *table = p.a.block_table + static_cast<uint64_t>(tile.r) * p.a.max_pages;
     const uint8_t *kc = static_cast<const uint8_t *>(p.c.k), *vc = static_cast<const uint8_t *>(p.c.v);
     const uint32_t kgroup = n / 4;
     bool missing = false;
 
-    // Codes of block b: this wavefront's key 4 i + wave of each 16 (i: the lane's n & 3 for K, all four for V).
+    // Codes of a block: this wavefront's key 4 i + wave of each 16 (i: the lane's n & 3 for K, all four for V).
     uint32_t kraw[D / 32], ke[KG];
     ValueCodes<D> vraw[4];
     u32x4 ve;
-    bool there_next = false;
+    Offset k_at = 0, ke_at = 0, v_at = 0, ve_at = 0;
+    bool there_found = false;
     int32_t id_k = 0, id_v = 0;
-    auto look = [&](uint32_t b) {  // the table's entries of block b
+    // Three steps of a block, each in another's shadow: its table entries, the addresses that follow from them, its codes.
+    auto look = [&](uint32_t b) {
         const int32_t base = static_cast<int32_t>(64 * b);
         id_k = entry_at(p, tile, table, base + 16 * static_cast<int32_t>(kgroup));
         id_v = entry_at(p, tile, table, base + 16 * static_cast<int32_t>(g));
     };
-    auto fetch = [&](uint32_t b) {  // its codes and scales, from the pages that look found
+    auto find = [&](uint32_t b) {
         const int32_t base = static_cast<int32_t>(64 * b);
         const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
-        there_next = is_page(p, tile, id_v, key_v);
-        missing |= !there_next && seen(tile, key_v);
-        const uint64_t unit_k = static_cast<uint64_t>(is_page(p, tile, id_k, key_k) ? id_k : 0) * p.c.kv_heads + kvh;
-        const uint64_t unit_v = static_cast<uint64_t>(there_next ? id_v : 0) * p.c.kv_heads + kvh;
-        const uint32_t place_k = (static_cast<uint32_t>(key_k) & page_mask) + 4 * (n & 3) + wave, place_v = static_cast<uint32_t>(key_v) & page_mask;
-#pragma unroll
-        for (int j = 0; j < KG; ++j) ke[j] = p.c.k_exponent[((unit_k * (D / 32) + (D == 64 ? g / 2 : KG * g + j)) << p.page_log2) + place_k];
-        ve = *reinterpret_cast<const u32x4 *>(p.c.v_exponent + ((unit_v * (D / 32) + n / (512 / D)) << p.page_log2) + place_v);
-        const uint8_t *kp = kc + ((unit_k << p.page_log2) + place_k) * (D / 2) + g * (D / 8);
-        __builtin_memcpy(kraw, __builtin_assume_aligned(kp, D == 64 ? 8 : 16), D / 8);
-        const uint8_t *vp = vc + ((unit_v << p.page_log2) + place_v + wave) * (D / 2) + n * (D / 32);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vraw[i].load(vp + 4 * i * (D / 2));
+        there_found = is_page(p, tile, id_v, key_v);
+        missing |= !there_found & seen(tile, key_v);
+        const uint32_t page_k = is_page(p, tile, id_k, key_k) ? id_k : 0, page_v = there_found ? id_v : 0;
+        // Below 2^32 bytes of codes there are fewer than 2^24 pages.
+        Offset unit_k, unit_v;
+        if constexpr (WIDE) {
+            unit_k = static_cast<Offset>(page_k) * p.c.kv_heads + kvh, unit_v = static_cast<Offset>(page_v) * p.c.kv_heads + kvh;
+        } else {
+            unit_k = __umul24(page_k, p.c.kv_heads) + kvh, unit_v = __umul24(page_v, p.c.kv_heads) + kvh;
+        }
+        unit_k <<= page_log2, unit_v <<= page_log2;
+        const uint32_t place_k = (static_cast<uint32_t>(key_k) & page_mask) + (4 * (n & 3) + wave), place_v = static_cast<uint32_t>(key_v) & page_mask;
+        ke_at = unit_k * (D / 32) + (place_k + (static_cast<uint32_t>(D == 64 ? g / 2 : KG * g) << page_log2));
+        ve_at = unit_v * (D / 32) + (place_v + (n / (512 / D) << page_log2));
+        k_at = (unit_k + place_k) * (D / 2) + g * (D / 8);
+        v_at = (unit_v + place_v) * (D / 2) + (wave * (D / 2) + n * (D / 32));
     };
-    auto convert = [&](uint32_t b) {  // into buffer b & 1
-        const uint32_t at = b & 1;
+    auto fetch = [&] {
+#pragma unroll
+        for (int j = 0; j < KG; ++j) ke[j] = p.c.k_exponent[ke_at + (static_cast<Offset>(j) << page_log2)];
+        ve = *reinterpret_cast<const u32x4 *>(p.c.v_exponent + ve_at);
+        __builtin_memcpy(kraw, __builtin_assume_aligned(kc + k_at, D == 64 ? 8 : 16), D / 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vraw[i].load(vc + v_at + 4 * i * (D / 2));
+    };
+    // Scales behind the keys, and of stand-ins, may be no numbers, which zero probabilities do not silence.
+    auto mend = [&](uint32_t b, bool there) {
+        const int32_t left = tile.seen_hi - static_cast<int32_t>(64 * b + 16 * g);
+        if (__ballot(!there || left < 16)) keep_bytes(ve, there ? left : 0);
+    };
+    const uint32_t pick = 0x000c0c0cu | wave << 24;  // byte `wave` of a word on top
+    auto convert = [&](uint32_t at) {                // into buffer `at`
 #pragma unroll
         for (int k = 0; k < KS; ++k) kf[at][wave][k][lane] = eight_of(kraw[k], scale_in<0>(ke[KG * k / KS]));
-        // Scales behind the keys, and of stand-ins, may be no numbers, which zero probabilities do not silence.
-        const int32_t left = tile.seen_hi - static_cast<int32_t>(64 * b + 16 * g);
-        if (__ballot(!there_next || left < 16)) keep_bytes(ve, there_next ? left : 0);
         float vs[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vs[i] = __uint_as_float((ve[i] >> (8 * wave) & 0xffu) << 23);
+        for (int i = 0; i < 4; ++i) vs[i] = __uint_as_float(perm(0u, ve[i], pick) >> 1);
 #pragma unroll
         for (int b2 = 0; b2 < DT / 2; ++b2) {
             f16x2 x[4];
@@ -459,22 +475,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendAr
         }
     };
 
+    // At the top of block b its codes are in LDS, those of b + 1 on their way to registers, the addresses of b + 2
+    // still to be found; past the last block the last one stands in.
+    bool there_now = false, there_next = false;
     if (tile.b0 < tile.b1) {
+        const uint32_t end = tile.b1 - 1;
         look(tile.b0);
-        fetch(tile.b0);
-        if (tile.b0 + 1 < tile.b1) look(tile.b0 + 1);
-        convert(tile.b0);
+        find(tile.b0);
+        fetch();
+        there_now = there_found;
+        mend(tile.b0, there_now);
+        convert(tile.b0 & 1);
+        look(min(tile.b0 + 1, end));
+        find(min(tile.b0 + 1, end));
+        fetch();
+        there_next = there_found;
+        look(min(tile.b0 + 2, end));
     }
     for (uint32_t b = tile.b0; b < tile.b1; ++b) {
+        const uint32_t end = tile.b1 - 1;
         __syncthreads();  // block b is in LDS, and every wavefront is done with block b - 1
-        const bool there = there_next;
-        if (b + 1 < tile.b1) {
-            fetch(b + 1);
-            if (b + 2 < tile.b1) look(b + 2);
-        }
         const int32_t base = static_cast<int32_t>(64 * b);
-        if (!idle && base < rows.any_hi && base > rows.any_lo - 64) {  // base + 64 may be 2^31
-            const bool edge = base < rows.all_lo || base > rows.all_hi - 64 || __ballot(there) != ~0ull;
+        const bool active = !idle && base < rows.any_hi && base > rows.any_lo - 64;  // base + 64 may be 2^31
+        if (active) {
+            const bool edge = base < rows.all_lo || base > rows.all_hi - 64 || __ballot(there_now) != ~0ull;
             // Products of one step of dimensions, four key tiles by NT row tiles, do not wait for each other.
             f32x4 s[NT][4];
 #pragma unroll
@@ -487,13 +511,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendAr
 #pragma unroll
                         for (int u = 0; u < NT; ++u) s[u][t] = mfma(kv, rows.qv[i][u][k], k || i ? s[u][t] : f32x4{0, 0, 0, 0});
                 }
+            find(min(b + 2, end));
             float off[NT];
-            rows.scores(s, there, edge, base + 16 * static_cast<int32_t>(g), off);
+            rows.scores(s, there_now, edge, base + 16 * static_cast<int32_t>(g), off);
+            mend(min(b + 1, end), there_next);
             f16x8 pv[2][LIMBS][NT];
             rows.template probabilities<0>(s, pv[0], off);
             rows.template probabilities<1>(s, pv[1], off);
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     const f16x8 vv = __builtin_shufflevector(vf[b & 1][d][c][0][lane], vf[b & 1][d][c][1][lane], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -502,8 +528,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendAr
 #pragma unroll
                         for (int u = 0; u < NT; ++u) rows.acc[u][d] = mfma(vv, pv[c][i][u], rows.acc[u][d]);
                 }
+            }
+            convert(~b & 1);
+        } else {
+            find(min(b + 2, end));
+            mend(min(b + 1, end), there_next);
+            convert(~b & 1);
         }
-        if (b + 1 < tile.b1) convert(b + 1);
+        fetch();
+        look(min(b + 3, end));
+        there_now = there_next;
+        there_next = there_found;
     }
     if (missing) raise_error(err, kErrIndex);
     if (idle) return;
@@ -530,12 +565,18 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     uint64_t parts;
     if (p.shared) {
         // Some eight workgroups a CU were every request as long as max_length, so that long requests among
-        // short ones do not finish last; eight blocks a part at least, two for each wavefront.
+        // short ones do not finish last; four blocks a part at least, one for each wavefront.  Where the tiles alone fill the
+        // chip, up to twelve, as long as a part has 48 blocks of 128 dimensions (64 requests of up to 16384 keys, heads of 128,
+        // with 8 / 12 / 16 workgroups a CU 138 / 130 / 132 us, heads of 64 81 / 87 / 83; eight of up to 131072, heads of 256,
+        // 157 / 164 / 173).
         parts = (blocks + 3) / 4;
         if (parts > 8ull * cus / tiles) parts = 8ull * cus / tiles;
         const uint64_t more = std::min<uint64_t>(12ull * cus / tiles, blocks * c.head_dim / 6144);
         if (tiles >= cus && parts < more) parts = more;
     } else {
+        // A part writes and reads its rows' sums, as long as some five blocks take, so parts have 24 blocks or more until the
+        // chip is full, and then up to eight workgroups a CU, eight blocks where the tiles leave CUs idle (33 blocks on 504
+        // tiles: 141 us whole, 166 in two parts).
         parts = blocks / 24;
         if (parts > 8ull * cus / tiles) parts = 8ull * cus / tiles;
         uint64_t fill = 2ull * cus / tiles;
@@ -553,7 +594,8 @@ int attend_launch(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s
     const dim3 grid(p.slots * p.c.kv_heads, 1, p.splits);
     constexpr int most = D == 256 ? 1 : 2;  // row tiles of the kernel for few rows
     const bool wide = static_cast<uint64_t>(p.c.pages) * p.c.page_size * p.c.kv_heads * (D / 2) > 0xffffffffull;
-    if (!plan.shared) k_attend4_tile<T, D, 2><<<grid, 256, 0, s>>>(p, err);
+    if (!plan.shared && wide) k_attend4_tile<T, D, 2, true><<<grid, 256, 0, s>>>(p, err);
+    else if (!plan.shared) k_attend4_tile<T, D, 2, false><<<grid, 256, 0, s>>>(p, err);
     else if (wide && plan.nt == 1) k_attend4_rows<T, D, 1, true><<<grid, 256, 0, s>>>(p, err);
     else if (wide) k_attend4_rows<T, D, most, true><<<grid, 256, 0, s>>>(p, err);
     else if (plan.nt == 1) k_attend4_rows<T, D, 1, false><<<grid, 256, 0, s>>>(p, err);
@@ -561,8 +603,11 @@ int attend_launch(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s
     int rc = launch_status();
     if (rc || p.splits == 1) return rc;
     const uint64_t rows = static_cast<uint64_t>(p.a.tokens) * p.a.heads;
-    if (p.splits > 8) k_attend_join<T, D, 4><<<static_cast<uint32_t>(rows), 256, 0, s>>>(p, plan.M, err);
-    else k_attend_join<T, D, 1><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, s>>>(p, plan.M, err);
+    const uint32_t many = static_cast<uint32_t>(rows), quarter = static_cast<uint32_t>((rows + 3) / 4);
+    if (p.splits > 8 && plan.shared) k_attend_join<T, D, 4, true><<<many, 256, 0, s>>>(p, plan.M, err);
+    else if (p.splits > 8) k_attend_join<T, D, 4><<<many, 256, 0, s>>>(p, plan.M, err);
+    else if (plan.shared) k_attend_join<T, D, 1, true><<<quarter, 256, 0, s>>>(p, plan.M, err);
+    else k_attend_join<T, D, 1><<<quarter, 256, 0, s>>>(p, plan.M, err);
     return launch_status();
 }
 template <typename T>
