@@ -475,7 +475,8 @@ int prism_hip_qkv_append_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, 
                                 const prism_qkv_append *step, void *stream);
 
 /* Reads slots of a cache of any format back: k, v [tokens][kv_heads][head_dim] of type dtype, a value its code times
- * its scale, rounded once.  A slot of -1 leaves its token's rows as they were; so does one outside the cache, with
+ * its scale in binary32, rounded from there to the type (exact where the scale is a power of two and the type binary32;
+ * always so with PRISM_CACHE_E2M1, whatever the type).  A slot of -1 leaves its token's rows as they were; so does one outside the cache, with
  * PRISM_ERR_INVALID_INPUT at sync.  Any order of slots, the same one any number of times.  A value that is not
  * finite in the type is PRISM_ERR_NONFINITE.  k or v may be NULL (not read).  Strides as for the append. */
 int prism_hip_kv_read_device(prism_hip_ctx *ctx, const prism_kv_cache *cache, int dtype, const int32_t *slots,
