@@ -59,6 +59,17 @@ __device__ __forceinline__ uint32_t seconds(f16x2 a, f16x2 b) {
     return perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
 }
 
+// Scales of positions that no row sees, before a window, behind the keys or of a stand-in, may be no numbers, which zero
+// probabilities do not silence: of 16 bytes those from `from` to `to` stay.
+__device__ __forceinline__ void keep_scales(u32x4 &v, bool there, int32_t from, int32_t to) {
+    keep_bytes(v, there ? to : 0);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int32_t gone = from - 4 * w;
+        v[w] &= gone >= 4 ? 0u : gone <= 0 ? ~0u : ~0u << (8 * gone);
+    }
+}
+
 // What both kernels below share: a wavefront's 16 * NT rows, their queries, statistics and sums.
 // T: type of q and out; LIMBS: binary16 parts of q and of the probabilities (2 for binary32).
 template <typename T, int D, int NT>
@@ -315,8 +326,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
         rows.scores(s, there, edge, key, off);
         rows.template probabilities<0>(s, pv[0], off);
         rows.template probabilities<1>(s, pv[1], off);
-        // Scales behind the keys, and of stand-ins, may be no numbers, which zero probabilities do not silence.
-        if (edge) keep_bytes(ve, there ? tile.seen_hi - key : 0);
+        if (edge) keep_scales(ve, there, tile.seen_lo - key, tile.seen_hi - key);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             // Element j of the operand is the key 4 (j % 4) + 2 c + j / 4.
@@ -453,10 +463,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendAr
 #pragma unroll
         for (int i = 0; i < 4; ++i) vraw[i].load(vc + v_at + 4 * i * (D / 2));
     };
-    // Scales behind the keys, and of stand-ins, may be no numbers, which zero probabilities do not silence.
     auto mend = [&](uint32_t b, bool there) {
-        const int32_t left = tile.seen_hi - static_cast<int32_t>(64 * b + 16 * g);
-        if (__ballot(!there || left < 16)) keep_bytes(ve, there ? left : 0);
+        const int32_t key = static_cast<int32_t>(64 * b + 16 * g);
+        if (__ballot(!there || key < tile.seen_lo || key > tile.seen_hi - 16)) keep_scales(ve, there, tile.seen_lo - key, tile.seen_hi - key);
     };
     const uint32_t pick = 0x000c0c0cu | wave << 24;  // byte `wave` of a word on top
     auto convert = [&](uint32_t at) {                // into buffer `at`

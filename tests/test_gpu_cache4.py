@@ -391,6 +391,30 @@ def test_gpu_attention4_masked_places_hold_anything(ctx, added, d):
     check(out.read(), want, tol)
 
 
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 64), (256, 256)])
+@pytest.mark.parametrize("added", [1, 30])
+def test_gpu_attention4_places_before_a_window_hold_anything(ctx, added, d, page):
+    """Scales that are no numbers in front of the first token's window, in the page where the window begins, at every place of
+    16 neighbours it may begin at."""
+    rng = np.random.default_rng(21)
+    heads, kv, n = 8, 2, 203
+    lengths, offsets = [n], [0, added]
+    table, pages = make_table(rng, lengths, page)
+    cache = make_cache(rng, pages, kv, page, d)
+    q = Rows(rng.standard_normal((added, heads, d)), "f16")
+    at, place = np.divmod(np.arange(n), page)
+    for window in [*range(37, 55), 1, 2, 100]:
+        first = n - added + 1 - window
+        dirty = {m: a.copy() if isinstance(a, np.ndarray) else a for m, a in cache.items()}
+        for m in ("k", "v"):
+            dirty[m + "_scale"][table[0, at[:first]], :, :, place[:first]] = 255
+            dirty[m][table[0, at[:first]], :, place[:first]] = 0x7F
+        call, out = attend(ctx, Device(dirty, page), q, offsets, lengths, table, d ** -0.5, True, window)
+        assert ctx.sync() == 0, window
+        want, tol = co.attention(cache, q.x, offsets, lengths, table, page, d ** -0.5, True, window, "f16")
+        check(out.read(), want, tol)
+
+
 @pytest.mark.parametrize("added", [1, 40])
 def test_gpu_attention4_leaves_out_pages_that_are_none(ctx, added):
     rng = np.random.default_rng(11)
@@ -571,6 +595,38 @@ def test_gpu_cache4_graphs_share_scratch(ctx):
         assert ctx.sync() == 0
         flat = steps[i][3].buf.to_numpy(np.float32)[steps[i][3].where].reshape(steps[i][4].shape)
         check(flat, steps[i][4], steps[i][5])
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "int8", "e4m3"])
+def test_gpu_append_and_read_replayed(ctx, fmt):
+    """A captured append and read, replayed with other tokens, slots and eager calls between, gives what eager calls give."""
+    rng = np.random.default_rng(20)
+    page, d, kv, tokens = 16, 64, 3, 21
+    (_, held), (_, eager) = (held_cache(np.random.default_rng(1), fmt, 8, kv, page, d) for _ in range(2))
+    order = i32(np.arange(tokens))
+    k, v = (Rows(np.zeros((tokens, kv, d)), "bf16") for _ in range(2))
+    k2, v2 = (Rows(np.zeros((tokens, kv, d)), "f32") for _ in range(2))
+
+    def run(cache):
+        ctx.kv_append_device(cache.desc, ph.DTYPE_BF16, k, k.stride, v, v.stride, order, tokens)
+        ctx.kv_read_device(cache.desc, ph.DTYPE_F32, order, tokens, k2, k2.stride, v2, v2.stride)
+
+    run(held), run(eager)
+    assert ctx.sync() == 0
+    graph = Graph(ctx.stream(), lambda: run(held))
+    for start in (0, 21, 42, 63):
+        order.upload(np.arange(start, start + tokens, dtype=np.int32))
+        for x in (k, v):
+            x.buf.upload(so.to_device(rng.standard_normal(x.buf.nbytes // 2), "bf16"))
+        run(eager)
+        assert ctx.sync() == 0
+        want = k2.read(), v2.read()
+        assert np.abs(want[0]).max() > 0
+        for x in (k2, v2):
+            x.buf.upload(x.before)
+        graph.launch()
+        assert ctx.sync() == 0
+        assert np.array_equal(k2.read(), want[0]) and np.array_equal(v2.read(), want[1])
 
 
 def test_gpu_serving_step_with_the_4_bit_cache_and_log_probabilities(ctx):
