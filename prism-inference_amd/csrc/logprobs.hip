@@ -25,6 +25,8 @@ struct Softmax {
     float m, s, t;
 };
 __device__ __forceinline__ float exp_of(float y) { return __builtin_amdgcn_exp2f(y * kLog2e); }
+// a - b for a smaller a, no lower than where its exponential is 0 long since: the other factor of a 0 stays finite.
+__device__ __forceinline__ float difference(float a, float b) { return fmaxf(a - b, -200.0f); }
 __device__ __forceinline__ Softmax joined(Softmax a, Softmax b) {
     if (b.m > a.m) {
         const Softmax c = a;
@@ -32,7 +34,7 @@ __device__ __forceinline__ Softmax joined(Softmax a, Softmax b) {
         b = c;
     }
     // The second's largest counts as a word of weight exp(d) now.
-    const float d = b.m - a.m, e = exp_of(d);
+    const float d = difference(b.m, a.m), e = exp_of(d);
     const bool none = b.m == kNone;
     a.t += none ? b.t : e * (b.t + d * (b.s + 1.0f));
     a.s += none ? b.s : e * (b.s + 1.0f);  // a NaN of a part without a finite logit goes on
@@ -377,7 +379,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(LogprobsArgs p, int *er
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
             if (w.m != kNone) {  // the former largest counts as another word, of lane 0
-                const float d = w.m - m, e = exp_of(d);
+                const float d = difference(w.m, m), e = exp_of(d);
                 w.t = e * (w.t + d * w.s);
                 w.s *= e;
                 if (lane == 0) {

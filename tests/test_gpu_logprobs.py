@@ -161,6 +161,74 @@ def test_gpu_logprobs_flags(ctx, dtype, vocab):
         c.check([0, 2])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [4, 260])
+def test_gpu_logprobs_few_words_of_many(ctx, dtype, tokens):
+    """Rows of a long vocabulary, whole and in parts, where fewer words than asked for are not masked by a large negative logit,
+    and rows of one value."""
+    rng = np.random.default_rng(6)
+    vocab = 70001
+    x = np.empty((tokens, vocab))
+    for t in range(tokens):
+        x[t] = (-1e9, 0.0, -3e38, -65504.0)[t % 4]
+        some = rng.choice(vocab, 3 + t % 30, replace=False)
+        x[t, some] = rng.standard_normal(len(some))
+    for top in (5, 64):
+        c = Call(x, rng.integers(0, vocab, tokens), top, dtype)
+        ctx.logprobs_device(c.call)
+        assert ctx.sync() == 0
+        c.check()
+
+
+@pytest.mark.parametrize("tokens,vocab", [(260, 70001), (300, 131072), (1, (1 << 20) + 5), (2, (1 << 24) - 3), (1, 1 << 24)])
+def test_gpu_logprobs_of_long_rows(ctx, tokens, vocab):
+    """Groups of several tiles."""
+    rng = np.random.default_rng(vocab)
+    c = Call(logits(rng, tokens, vocab, 0.1), rng.integers(0, vocab, tokens), 20, "f16", 1, 1)
+    ctx.logprobs_device(c.call)
+    assert ctx.sync() == 0
+    c.check()
+
+
+def test_gpu_logprobs_of_many_long_rows(ctx):
+    """More than 256 rows past 2^20 words: parts of the largest groups.  Every row is the same."""
+    from hiprt import DeviceBuffer
+    rng = np.random.default_rng(7)
+    tokens, vocab, top = 257, (1 << 20) + 70, 9
+    row = so.to_device(logits(rng, 1, vocab, 0.1), "f16")
+    big = DeviceBuffer(2 * tokens * vocab)
+    for t in range(tokens):
+        big.upload(row, 2 * t * vocab)
+    c = Call(so.from_device(row, "f16"), [vocab - 5], top, "f16")
+    out = {m: dev(np.zeros(tokens * k, np.float32)) for m, k in (("logprobs", 1), ("entropy", 1), ("top_logprobs", top))}
+    ids = i32(np.zeros(tokens * top))
+    ctx.logprobs_device(ph.Logprobs(dtype=DTYPE["f16"], tokens=tokens, vocab=vocab, top=top, logits=big, stride=vocab, targets=i32([vocab - 5] * tokens),
+                                    top_ids=ids, **out))
+    assert ctx.sync() == 0
+    want = co.logprobs(c.x, [vocab - 5], top)
+    assert (ids.to_numpy(np.int32).reshape(tokens, top) == want["top_ids"][0]).all()
+    for m, b in out.items():
+        w, tol = want[m]
+        got = b.to_numpy(np.float32).reshape(tokens, -1)
+        check(got, np.broadcast_to(w.reshape(1, -1), got.shape), np.broadcast_to(np.reshape(tol, (1, -1)), got.shape))
+
+
+@pytest.mark.parametrize("vocab", [90, 40000])
+def test_gpu_logprobs_of_the_whole_range(ctx, vocab):
+    """Logits whose differences pass binary32's range."""
+    i = np.arange(vocab)
+    x = np.array([np.where(i % 7 == 0, 3e38, -3e38), np.where(i == vocab - 1, 3e38, -3e38), np.where(i == 0, 3.4e38, -3.4e38)])
+    c = Call(x, [0, vocab - 1, 0], 5)
+    ctx.logprobs_device(c.call)
+    assert ctx.sync() == 0
+    want = co.logprobs(c.x, [0, vocab - 1, 0], 1)
+    for m in ("logprobs", "entropy"):
+        check(c.get(m), *want[m])
+    best = c.get("top_logprobs")
+    check(best[:, :1], *want["top_logprobs"])
+    assert np.isneginf(best[1:, 1:]).all() and c.get("top_ids").tolist()[1:] == [[vocab - 1, 0, 1, 2, 3], [0, 1, 2, 3, 4]]
+
+
 def test_gpu_logprobs_of_what_is_asked(ctx):
     rng = np.random.default_rng(3)
     for vocab in (90, 50000):
