@@ -396,22 +396,24 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
     rows.write(p, tile.parts, blockIdx.z, err);
 }
 
-// Many rows (prompts, chunks): each wavefront has 16 * NT rows of its own and all keys.  A block's codes are
-// converted to binary16 once by the workgroup, a quarter of the keys by each wavefront, into LDS in the order of the
-// operands; the next block's codes come from memory meanwhile and are converted behind the products, so a
+// Many rows (prompts, chunks): each of WAVES wavefronts has 16 * NT rows of its own and all keys.  A block's codes are
+// converted to binary16 once by the workgroup, a quarter of the keys (or of eight wavefronts half the dimensions of one) by each
+// wavefront, into LDS in the order of the operands; the next block's codes come from memory meanwhile and are converted behind the products, so a
 // block costs one barrier.
-template <typename T, int D, int NT, bool WIDE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendArgs p, int *err) {
+template <typename T, int D, int NT, int WAVES, bool WIDE>
+__global__ __launch_bounds__(64 * WAVES, D == 256 && WAVES == 4 ? 1 : 2) void k_attend4_tile(AttendArgs p, int *err) {
     typedef Rows4<T, D, NT> R;
     typedef std::conditional_t<WIDE, uint64_t, uint32_t> Offset;
-    constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT, KG = D == 256 ? 2 : 1;
+    constexpr int LIMBS = R::LIMBS, KS = R::KS, DT = R::DT;
+    constexpr int H = WAVES / 4, HK = KS / H, HG = D == 256 ? 2 / H : 1, HB = DT / 2 / H;  // of one wavefront: its steps, scales and bytes
+    static_assert(H == 1 || (H == 2 && D == 256));
     __shared__ f16x8 kf[2][4][KS][64];
     __shared__ f16x4 vf[2][DT][2][2][64];  // halves of an operand apart: writes of 8 bytes without bank conflicts
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = lane & 15, g = lane / 16;
     Tile tile;
-    if (!tile_of(p, 64 * NT, blockIdx.z, err, &tile)) return;
-    const uint32_t kvh = tile.kvh;
+    if (!tile_of(p, 16 * NT * WAVES, blockIdx.z, err, &tile)) return;
+    const uint32_t kvh = tile.kvh, part = wave % 4, half = wave / 4;
     R rows;
     rows.load(p, tile.q, min(tile.row0 + wave * 16 * NT, tile.last), tile.last, kvh);
     const bool idle = tile.row0 + wave * 16 * NT > tile.last;  // converts only
@@ -422,9 +424,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendAr
     const uint32_t kgroup = n / 4;
     bool missing = false;
 
-    // Codes of a block: this wavefront's key 4 i + wave of each 16 (i: the lane's n & 3 for K, all four for V).
-    uint32_t kraw[D / 32], ke[KG];
-    ValueCodes<D> vraw[4];
+    // Codes of a block: this wavefront's key 4 i + part of each 16 (i: the lane's n & 3 for K, all four for V).
+    uint32_t kraw[HK], ke[HG];
+    ValueCodes<D / H> vraw[4];
     u32x4 ve;
     Offset k_at = 0, ke_at = 0, v_at = 0, ve_at = 0;
     bool there_found = false;
@@ -449,17 +451,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendAr
             unit_k = __umul24(page_k, p.c.kv_heads) + kvh, unit_v = __umul24(page_v, p.c.kv_heads) + kvh;
         }
         unit_k <<= page_log2, unit_v <<= page_log2;
-        const uint32_t place_k = (static_cast<uint32_t>(key_k) & page_mask) + (4 * (n & 3) + wave), place_v = static_cast<uint32_t>(key_v) & page_mask;
-        ke_at = unit_k * (D / 32) + (place_k + (static_cast<uint32_t>(D == 64 ? g / 2 : KG * g) << page_log2));
+        const uint32_t place_k = (static_cast<uint32_t>(key_k) & page_mask) + (4 * (n & 3) + part), place_v = static_cast<uint32_t>(key_v) & page_mask;
+        ke_at = unit_k * (D / 32) + (place_k + (static_cast<uint32_t>(D == 64 ? g / 2 : D == 128 ? g : 2 * g + HG * half) << page_log2));
         ve_at = unit_v * (D / 32) + (place_v + (n / (512 / D) << page_log2));
-        k_at = (unit_k + place_k) * (D / 2) + g * (D / 8);
-        v_at = (unit_v + place_v) * (D / 2) + (wave * (D / 2) + n * (D / 32));
+        k_at = (unit_k + place_k) * (D / 2) + (g * (D / 8) + half * (4 * HK));
+        v_at = (unit_v + place_v) * (D / 2) + (part * (D / 2) + n * (D / 32) + half * HB);
     };
     auto fetch = [&] {
 #pragma unroll
-        for (int j = 0; j < KG; ++j) ke[j] = p.c.k_exponent[ke_at + (static_cast<Offset>(j) << page_log2)];
+        for (int j = 0; j < HG; ++j) ke[j] = p.c.k_exponent[ke_at + (static_cast<Offset>(j) << page_log2)];
         ve = *reinterpret_cast<const u32x4 *>(p.c.v_exponent + ve_at);
-        __builtin_memcpy(kraw, __builtin_assume_aligned(kc + k_at, D == 64 ? 8 : 16), D / 8);
+        __builtin_memcpy(kraw, __builtin_assume_aligned(kc + k_at, D == 64 ? 8 : 16), 4 * HK);
 #pragma unroll
         for (int i = 0; i < 4; ++i) vraw[i].load(vc + v_at + 4 * i * (D / 2));
     };
@@ -467,20 +469,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attend4_tile(AttendAr
         const int32_t key = static_cast<int32_t>(64 * b + 16 * g);
         if (__ballot(!there || key < tile.seen_lo || key > tile.seen_hi - 16)) keep_scales(ve, there, tile.seen_lo - key, tile.seen_hi - key);
     };
-    const uint32_t pick = 0x000c0c0cu | wave << 24;  // byte `wave` of a word on top
+    const uint32_t pick = 0x000c0c0cu | part << 24;  // byte `part` of a word on top
     auto convert = [&](uint32_t at) {                // into buffer `at`
 #pragma unroll
-        for (int k = 0; k < KS; ++k) kf[at][wave][k][lane] = eight_of(kraw[k], scale_in<0>(ke[KG * k / KS]));
+        for (int k = 0; k < HK; ++k) kf[at][part][HK * half + k][lane] = eight_of(kraw[k], scale_in<0>(ke[HG * k / HK]));
         float vs[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) vs[i] = __uint_as_float(perm(0u, ve[i], pick) >> 1);
 #pragma unroll
-        for (int b2 = 0; b2 < DT / 2; ++b2) {
+        for (int b2 = 0; b2 < HB; ++b2) {
+            const uint32_t d = 2 * (HB * half + b2);
             f16x2 x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = pair_of(vraw[i].w[b2 / 4], vs[i], b2 % 4);
-            vf[at][2 * b2][wave / 2][wave % 2][lane] = __builtin_bit_cast(f16x4, u32x2{firsts(x[0], x[1]), firsts(x[2], x[3])});
-            vf[at][2 * b2 + 1][wave / 2][wave % 2][lane] = __builtin_bit_cast(f16x4, u32x2{seconds(x[0], x[1]), seconds(x[2], x[3])});
+            vf[at][d][part / 2][part % 2][lane] = __builtin_bit_cast(f16x4, u32x2{firsts(x[0], x[1]), firsts(x[2], x[3])});
+            vf[at][d + 1][part / 2][part % 2][lane] = __builtin_bit_cast(f16x4, u32x2{seconds(x[0], x[1]), seconds(x[2], x[3])});
         }
     };
 
@@ -565,9 +568,23 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     const uint64_t typical = (static_cast<uint64_t>(a.tokens) * group + a.requests - 1) / a.requests;  // rows of a request
     Plan p;
     p.shared = typical <= 32;
-    p.nt = p.shared && (c.head_dim == 256 || typical <= 16) ? 1 : 2;
+    auto slots_of = [&](uint32_t M) { return static_cast<uint32_t>(static_cast<uint64_t>(a.tokens) * group / M) + a.requests; };
+    if (p.shared) {
+        p.nt = c.head_dim == 256 || typical <= 16 ? 1 : 2;
+    } else {
+        // 128 rows a workgroup take fewer conversions and loads from LDS a row (a prompt of 8192 tokens, bf16, 620 us, with 64 rows
+        // 860), 64 fill the chip from fewer rows and waste less of a short request's tile: taken for short keys on up to two tiles of 128
+        // a CU (1000 tokens by themselves, bf16 49 -> 29 us, f32 62 -> 37), for requests of few rows (64 of one to 512 tokens, bf16, 166
+        // -> 141), and in binary32, whose products outweigh the conversions, on up to four a CU.  Heads of 256, where 64 rows leave one
+        // wavefront a SIMD, take them on up to one tile of 128 a CU (600 tokens by themselves, bf16, 35 -> 30; 1500 tokens 75 with 128
+        // rows, 107 with 64).  Over 219 batches of 1 to 32 requests, heads of 64 and 128, the rule is 1 % behind the better of the two each
+        // time, always 128 rows 15 %, always 64 4 %; over 156 with heads of 256 2 %, 9 % and 14 %.
+        const uint64_t tiles = static_cast<uint64_t>(slots_of(128)) * c.kv_heads, keys = a.window ? std::min(a.window, a.max_length) : a.max_length;
+        if (c.head_dim == 256) p.nt = tiles <= cus && keys < 1600 ? 1 : 2;
+        else p.nt = typical <= 256 || (tiles <= 2ull * cus && keys < 1600) || (tiles <= 4ull * cus && a.dtype == PRISM_DTYPE_F32) ? 1 : 2;
+    }
     p.M = p.shared ? 16 * p.nt : 64 * p.nt;
-    p.slots = static_cast<uint32_t>(static_cast<uint64_t>(a.tokens) * group / p.M) + a.requests;
+    p.slots = slots_of(p.M);
     uint64_t longest = a.max_length;
     if (a.window && longest > a.window + p.M / group) longest = a.window + p.M / group;  // what a tile sees of it
     const uint64_t tiles = static_cast<uint64_t>(p.slots) * c.kv_heads, blocks = longest / 64 + 1;
@@ -603,9 +620,18 @@ int attend_launch(const AttendArgs &p, const Plan &plan, int *err, hipStream_t s
     const dim3 grid(p.slots * p.c.kv_heads, 1, p.splits);
     constexpr int most = D == 256 ? 1 : 2;  // row tiles of the kernel for few rows
     const bool wide = static_cast<uint64_t>(p.c.pages) * p.c.page_size * p.c.kv_heads * (D / 2) > 0xffffffffull;
-    if (!plan.shared && wide) k_attend4_tile<T, D, 2, true><<<grid, 256, 0, s>>>(p, err);
-    else if (!plan.shared) k_attend4_tile<T, D, 2, false><<<grid, 256, 0, s>>>(p, err);
-    else if (wide && plan.nt == 1) k_attend4_rows<T, D, 1, true><<<grid, 256, 0, s>>>(p, err);
+    if (!plan.shared) {
+        // 64 rows are four wavefronts' with 16 each; 128 are four with 32, or with heads of 256 eight with 16, whose registers
+        // leave two on a SIMD (a prompt of 8192 tokens, 32 heads of 256, bf16, 2000 -> 1425 us, f32 2620 -> 1840).
+        constexpr int nt = D == 256 ? 1 : 2, waves = D == 256 ? 8 : 4;
+        if (plan.M == 64) {
+            if (wide) k_attend4_tile<T, D, 1, 4, true><<<grid, 256, 0, s>>>(p, err);
+            else k_attend4_tile<T, D, 1, 4, false><<<grid, 256, 0, s>>>(p, err);
+        } else {
+            if (wide) k_attend4_tile<T, D, nt, waves, true><<<grid, 64 * waves, 0, s>>>(p, err);
+            else k_attend4_tile<T, D, nt, waves, false><<<grid, 64 * waves, 0, s>>>(p, err);
+        }
+    } else if (wide && plan.nt == 1) k_attend4_rows<T, D, 1, true><<<grid, 256, 0, s>>>(p, err);
     else if (wide) k_attend4_rows<T, D, most, true><<<grid, 256, 0, s>>>(p, err);
     else if (plan.nt == 1) k_attend4_rows<T, D, 1, false><<<grid, 256, 0, s>>>(p, err);
     else k_attend4_rows<T, D, most, false><<<grid, 256, 0, s>>>(p, err);

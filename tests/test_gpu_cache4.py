@@ -317,6 +317,29 @@ def test_gpu_attention4(ctx, batch, d, heads, kv, page, dtype):
         check(out.read(), want, tol)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("batch", [[(200, 200)], [(90, 150), (1, 1), (400, 433)], [(300, 1900)]])
+def test_gpu_attention4_of_many_rows(ctx, batch, d, dtype):
+    """Workgroups of 128 rows: taken for long keys, in binary32 for many tiles (heads of 64 and 128)."""
+    rng = np.random.default_rng(len(batch) + d)
+    page = 32
+    heads, kv = (512, 256) if dtype == "f32" and d < 256 and len(batch) < 2 and batch[0][1] == 200 else (8, 2)
+    added, lengths = (list(x) for x in zip(*batch))
+    if heads == 512:
+        added, lengths = [330], [330]
+    offsets = np.concatenate([[0], np.cumsum(added)])
+    table, pages = make_table(rng, lengths, page)
+    cache = make_cache(rng, pages, kv, page, d)
+    held = Device(cache, page)
+    q = Rows(rng.standard_normal((offsets[-1], heads, d)) * 2, dtype, pad=7, shift=1)
+    for causal, window in ((True, 0), (True, 40), (False, 0)):
+        call, out = attend(ctx, held, q, offsets, lengths, table, d ** -0.5, causal, window, max_length=2000)
+        assert ctx.sync() == 0
+        want, tol = co.attention(cache, q.x, offsets, lengths, table, page, d ** -0.5, causal, window, dtype)
+        check(out.read(), want, tol)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("max_length", [0, 3000, 1 << 20])
 def test_gpu_attention4_splits_long_caches(ctx, dtype, max_length):
@@ -357,7 +380,7 @@ def test_gpu_attention4_rows_without_keys(ctx, added):
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("added", [1, 30])
+@pytest.mark.parametrize("added", [1, 30, 100])
 def test_gpu_attention4_masked_places_hold_anything(ctx, added, d):
     """Scales that are no numbers behind the keys, in pages no row sees, and missing pages before a window."""
     rng = np.random.default_rng(10)
@@ -374,7 +397,7 @@ def test_gpu_attention4_masked_places_hold_anything(ctx, added, d):
         dirty[m + "_scale"][unused] = 255
     held = Device(dirty, page)
     q = Rows(rng.standard_normal((added, heads, d)), "f16")
-    call, out = attend(ctx, held, q, offsets, lengths, table, d ** -0.5)
+    call, out = attend(ctx, held, q, offsets, lengths, table, d ** -0.5, max_length=2000)
     assert ctx.sync() == 0
     want, tol = co.attention(cache, q.x, offsets, lengths, table, page, d ** -0.5, True, 0, "f16")
     check(out.read(), want, tol)
@@ -385,31 +408,32 @@ def test_gpu_attention4_masked_places_hold_anything(ctx, added, d):
     for m in ("k", "v"):
         dirty[m + "_scale"][used[:first]] = 255
     held = Device(dirty, page)
-    call, out = attend(ctx, held, q, offsets, lengths, gone, d ** -0.5, True, 50)
+    call, out = attend(ctx, held, q, offsets, lengths, gone, d ** -0.5, True, 50, max_length=2000)
     assert ctx.sync() == 0
     want, tol = co.attention(cache, q.x, offsets, lengths, table, page, d ** -0.5, True, 50, "f16")
     check(out.read(), want, tol)
 
 
 @pytest.mark.parametrize("d,page", [(64, 16), (128, 64), (256, 256)])
-@pytest.mark.parametrize("added", [1, 30])
+@pytest.mark.parametrize("added", [1, 30, 100])
 def test_gpu_attention4_places_before_a_window_hold_anything(ctx, added, d, page):
     """Scales that are no numbers in front of the first token's window, in the page where the window begins, at every place of
     16 neighbours it may begin at."""
     rng = np.random.default_rng(21)
-    heads, kv, n = 8, 2, 203
+    heads, kv = 8, 2
+    n, windows = (203, [*range(37, 55), 1, 2, 100]) if added < 100 else (1830, range(1601, 1618))  # workgroups of 64 and 128 rows
     lengths, offsets = [n], [0, added]
     table, pages = make_table(rng, lengths, page)
     cache = make_cache(rng, pages, kv, page, d)
     q = Rows(rng.standard_normal((added, heads, d)), "f16")
     at, place = np.divmod(np.arange(n), page)
-    for window in [*range(37, 55), 1, 2, 100]:
+    for window in windows:
         first = n - added + 1 - window
         dirty = {m: a.copy() if isinstance(a, np.ndarray) else a for m, a in cache.items()}
         for m in ("k", "v"):
             dirty[m + "_scale"][table[0, at[:first]], :, :, place[:first]] = 255
             dirty[m][table[0, at[:first]], :, place[:first]] = 0x7F
-        call, out = attend(ctx, Device(dirty, page), q, offsets, lengths, table, d ** -0.5, True, window)
+        call, out = attend(ctx, Device(dirty, page), q, offsets, lengths, table, d ** -0.5, True, window, max_length=2000)
         assert ctx.sync() == 0, window
         want, tol = co.attention(cache, q.x, offsets, lengths, table, page, d ** -0.5, True, window, "f16")
         check(out.read(), want, tol)
@@ -521,8 +545,8 @@ def test_gpu_attention4_of_many_requests(ctx, requests):
     check(out.read(), want, tol)
 
 
-@pytest.mark.parametrize("added", [1, 6, 70])
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("added", [1, 6, 70, 300])
+@pytest.mark.parametrize("d", [64, 128, 256])
 def test_gpu_cache4_past_32_bits(ctx, added, d):
     """Pages whose codes stand past 4 GB: appended to, read back and attended over."""
     page, kv, heads = 256, 8, 8
@@ -546,7 +570,7 @@ def test_gpu_cache4_past_32_bits(ctx, added, d):
     small = co.append(small, x["k"], x["v"], np.arange(n), page)
     q = Rows(rng.standard_normal((added, heads, d)), "f16")
     held = type("Held", (), {"desc": desc})
-    call, out = attend(ctx, held, q, [0, added], [n], np.array([use]), 0.1)
+    call, out = attend(ctx, held, q, [0, added], [n], np.array([use]), 0.1, max_length=2000)
     assert ctx.sync() == 0
     for got, m in ((k2, "k"), (v2, "v")):
         assert np.array_equal(got.read(), co.values(small, m).swapaxes(1, 2).reshape(-1, kv, d)[:n])
