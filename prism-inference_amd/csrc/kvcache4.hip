@@ -9,7 +9,8 @@ namespace prism {
 
 namespace {
 
-// A lane has eight consecutive dimensions of one token and head, four lanes a scale.
+// A lane has eight consecutive dimensions of one token and head, four lanes a scale; one instruction makes two codes, so memory
+// bounds it: 7314 tokens of 48 requests, 4 heads of 256 in binary16, take 10.4 us, 3.7 TB/s.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_append4(Append4Args a, int *err) {
     constexpr uint32_t kLanes = D / 8, kRows = 256 / kLanes;
@@ -186,6 +187,10 @@ int append4_typed(const Append4Args &a, int *err, hipStream_t s) {
     return launch_status();
 }
 
+// A step's rotation and both appends in one launch: rotated keys go into codes without a pass through memory, and a step of 32
+// requests takes 4.4 us (two launches 8.1).  6030 tokens of 32 + 2 x 8 heads of 128, bf16, take 37 us for 130 MB, 3.5 TB/s, and
+// without norms 30, 4.3 TB/s: between them stand the norms' sums and products in binary64.  In binary32 54 us, 4.8 TB/s.
+// More workgroups to a token's heads are slower (twice as many 45 us: each makes the cosines again).
 template <typename T, int D>
 int qkv4_typed(const Rotation &rot, const RopeRows &q, const RopeRows &k, const int32_t *positions, float eps, const Append4Args &a, int *err,
                hipStream_t s) {

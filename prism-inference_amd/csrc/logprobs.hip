@@ -343,7 +343,9 @@ __device__ __forceinline__ void alternatives(const LogprobsArgs &p, uint64_t row
     write_top(p.a, row, sh.scale, sh.merged);
 }
 
-// A workgroup takes a part of a row, its wavefronts every WAVES-th tile of it.
+// A workgroup takes a part of a row, its wavefronts every WAVES-th tile of it, the next tile's loads in flight.  Memory bounds it:
+// 1024 rows of 151936 binary32 logits, 20 alternatives, take 116 us, 5.4 TB/s (none 107, 64 of them 128; bf16 72), 4096 of 32000
+// 100.  One row of 151936 takes 4.5 us in 38 parts, and its join 6.4.
 template <typename T, int WAVES, bool TOP>
 __global__ __launch_bounds__(64 * WAVES) void k_logprobs(LogprobsArgs p, int *err) {
     __shared__ float group_largest[TOP ? kGroups : 1][64 * WAVES], part[WAVES][3];
@@ -446,7 +448,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_logprobs(LogprobsArgs p, int *er
     }
 }
 
-// A workgroup finishes a row that was in parts.
+// A workgroup finishes a row that was in parts, with sixteen wavefronts, since what it waits for is the chain from the groups'
+// largest to the logits read again: 6.4 us for one row.
 constexpr int kJoinWaves = 16;
 template <typename T, bool TOP>
 __global__ __launch_bounds__(TOP ? 64 * kJoinWaves : 64) void k_logprobs_join(LogprobsArgs p, int *err) {

@@ -249,7 +249,11 @@ struct ValueCodes {
 };
 
 // Few rows (single tokens, drafts): the workgroup's four wavefronts share 16 * NT rows and split the
-// keys.  Every code is used once, so they go from memory to registers.
+// keys.  Every code is used once, so they go from memory to registers, and memory is the bound: 64 requests of up to 16384 keys
+// (8 heads of 128, 570 MB) 128 us, 4.5 TB/s, of one length 115 us, 5.0; 8 of up to 131072 (4 of 256) 156 to 163 us, 4.2 to 4.4, where
+// conversions of 16 rows for the 6 of a group count too.  A single request's 1025 keys take 6.7 us and their join 3.7, a launch and
+// four dependent loads each.  Keys through LDS, with half the accesses to L1, take as long; so do the next block's codes
+// loaded ahead into registers (140 against 137), and a launch bound for four wavefronts a SIMD spills (130 against 116).
 // WIDE: byte offsets into the keys or values pass 32 bits; else a lane's address is one register
 // beside a scalar base.
 template <typename T, int D, int NT, bool WIDE>
@@ -399,7 +403,9 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 // Many rows (prompts, chunks): each of WAVES wavefronts has 16 * NT rows of its own and all keys.  A block's codes are
 // converted to binary16 once by the workgroup, a quarter of the keys (or of eight wavefronts half the dimensions of one) by each
 // wavefront, into LDS in the order of the operands; the next block's codes come from memory meanwhile and are converted behind the products, so a
-// block costs one barrier.
+// block costs one barrier.  Bounds: conversions, exponentials and their like fill 52 % of a SIMD's cycles and the matrix cores 37 %,
+// which add up, since two wavefronts a SIMD hardly ever issue both at once: a prompt of 8192 tokens, 32 heads of 128, takes 580 to 705 us
+// card by card, 780 to 950 TFLOP/s.
 template <typename T, int D, int NT, int WAVES, bool WIDE>
 __global__ __launch_bounds__(64 * WAVES, D == 256 && WAVES == 4 ? 1 : 2) void k_attend4_tile(AttendArgs p, int *err) {
     typedef Rows4<T, D, NT> R;
