@@ -282,21 +282,24 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
         id_k = entry_at(p, tile, table, base + 16 * static_cast<int32_t>(kgroup));
         id_v = entry_at(p, tile, table, base + 16 * static_cast<int32_t>(g));
     };
-    auto fetch = [&](uint32_t b) {
-        const int32_t base = static_cast<int32_t>(64 * b);
-        const int32_t key_k = base + 16 * static_cast<int32_t>(kgroup), key_v = base + 16 * static_cast<int32_t>(g);
-        there_next = is_page(p, tile, id_v, key_v);
-        missing |= !there_next && seen(tile, key_v);
+    auto fetch_k = [&](uint32_t b) {
+        const int32_t key_k = static_cast<int32_t>(64 * b) + 16 * static_cast<int32_t>(kgroup);
         const Offset unit_k = static_cast<Offset>(is_page(p, tile, id_k, key_k) ? id_k : 0) * p.c.kv_heads + kvh;
-        const Offset unit_v = static_cast<Offset>(there_next ? id_v : 0) * p.c.kv_heads + kvh;
-        const uint32_t place_k = (static_cast<uint32_t>(key_k) & page_mask) + 4 * (n & 3), place_v = static_cast<uint32_t>(key_v) & page_mask;
+        const uint32_t place_k = (static_cast<uint32_t>(key_k) & page_mask) + 4 * (n & 3);
 #pragma unroll
         for (int j = 0; j < KG; ++j)
             ke[j] = *reinterpret_cast<const uint32_t *>(p.c.k_exponent + (((unit_k * (D / 32) + (D == 64 ? g / 2 : KG * g + j)) << p.page_log2) + place_k));
-        ve = *reinterpret_cast<const u32x4 *>(p.c.v_exponent + (((unit_v * (D / 32) + n / (512 / D)) << p.page_log2) + place_v));
         const Offset k_at = ((unit_k << p.page_log2) + place_k) * (D / 2) + g * (D / 8);
 #pragma unroll
         for (int t = 0; t < 4; ++t) __builtin_memcpy(kraw[t], __builtin_assume_aligned(kc + k_at + t * (D / 2), D == 64 ? 8 : 16), D / 8);
+    };
+    auto fetch_v = [&](uint32_t b) {
+        const int32_t key_v = static_cast<int32_t>(64 * b) + 16 * static_cast<int32_t>(g);
+        there_next = is_page(p, tile, id_v, key_v);
+        missing |= !there_next && seen(tile, key_v);
+        const Offset unit_v = static_cast<Offset>(there_next ? id_v : 0) * p.c.kv_heads + kvh;
+        const uint32_t place_v = static_cast<uint32_t>(key_v) & page_mask;
+        ve = *reinterpret_cast<const u32x4 *>(p.c.v_exponent + (((unit_v * (D / 32) + n / (512 / D)) << p.page_log2) + place_v));
         const Offset v_at = ((unit_v << p.page_log2) + place_v) * (D / 2) + n * (D / 32);
 #pragma unroll
         for (int r = 0; r < 16; ++r) vraw[r].load(vc + v_at + r * (D / 2));
@@ -305,9 +308,21 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
     if (first < tile.b1) look(first);
     R rows;
     rows.load(p, tile.q, tile.row0, tile.last, kvh);
+    // Heads of 256 leave two wavefronts a SIMD or one, so each product reloads the codes it used for its next block (8 requests of up
+    // to 131072 keys 163 -> 153 us); others load both at the top of the block (64 of up to 16384, heads of 128, 128 us either way,
+    // binary32 142 against 157, heads of 64 82 against 85).
+    constexpr bool kAhead = D == 256;
+    if (kAhead && first < tile.b1) {
+        fetch_k(first);
+        fetch_v(first);
+        if (first + 4 < tile.b1) look(first + 4);
+    }
     for (uint32_t b = first; b < tile.b1; b += 4) {
-        fetch(b);
-        if (b + 4 < tile.b1) look(b + 4);
+        if constexpr (!kAhead) {
+            fetch_k(b);
+            fetch_v(b);
+            if (b + 4 < tile.b1) look(b + 4);
+        }
         const int32_t base = static_cast<int32_t>(64 * b), key = base + 16 * static_cast<int32_t>(g);
         const bool there = there_next;
         const bool edge = base < rows.all_lo || base > rows.all_hi - 64 || __ballot(there) != ~0ull;
@@ -325,6 +340,7 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
                     for (int i = 0; i < LIMBS; ++i) s[u][t] = mfma(kv, rows.qv[i][u][k], s[u][t]);
             }
         }
+        if (kAhead && b + 4 < tile.b1) fetch_k(b + 4);
         f16x8 pv[2][LIMBS][NT];
         float off[NT];
         rows.scores(s, there, edge, key, off);
@@ -356,6 +372,10 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
                         rows.acc[u][2 * b2 + 1] = mfma(o.v, pv[c][i][u], rows.acc[u][2 * b2 + 1]);
                     }
             }
+        }
+        if (kAhead && b + 4 < tile.b1) {
+            fetch_v(b + 4);
+            if (b + 8 < tile.b1) look(b + 8);
         }
     }
     if (missing) raise_error(err, kErrIndex);
