@@ -616,13 +616,15 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     const uint64_t tiles = static_cast<uint64_t>(p.slots) * c.kv_heads, blocks = longest / 64 + 1;
     uint64_t parts;
     if (p.shared) {
-        // Some eight workgroups a CU were every request as long as max_length, so that long requests among
-        // short ones do not finish last; four blocks a part at least, one for each wavefront.  Where the tiles alone fill the
-        // chip, up to twelve, as long as a part has 48 blocks of 128 dimensions (64 requests of up to 16384 keys, heads of 128,
-        // with 8 / 12 / 16 workgroups a CU 138 / 130 / 132 us, heads of 64 81 / 87 / 83; eight of up to 131072, heads of 256,
-        // 157 / 164 / 173).
+        // Four workgroups a CU were every request as long as max_length where there are no more tiles than CUs (4 / 8 requests of up to 16384
+        // keys, 8 heads of 128, with 8 and 4 workgroups 22.7 -> 19.8 and 31 -> 26.4 us, 16 of 4000 26 -> 23.4; heads of 256, 3 requests of
+        // up to 131072 110 -> 92, 64 of up to 2000 35 -> 31, but 8 of up to 131072 152 -> 156), eight where they do not (64 requests of 8192
+        // keys 125 -> 115), so that long requests among short ones do not finish last; four blocks a part at least, one for each
+        // wavefront.  Where the tiles alone fill the chip, up to twelve, as long as a part has 48 blocks of 128 dimensions (64 requests
+        // of up to 16384 keys, heads of 128, with 8 / 12 / 16 workgroups a CU 138 / 130 / 132 us, heads of 64 81 / 87 / 83).
+        const uint64_t most = (tiles <= cus ? 4ull : 8ull) * cus / tiles;
         parts = (blocks + 3) / 4;
-        if (parts > 8ull * cus / tiles) parts = 8ull * cus / tiles;
+        if (parts > most) parts = most;
         const uint64_t more = std::min<uint64_t>(12ull * cus / tiles, blocks * c.head_dim / 6144);
         if (tiles >= cus && parts < more) parts = more;
     } else {
