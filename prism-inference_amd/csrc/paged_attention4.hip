@@ -250,10 +250,10 @@ struct ValueCodes {
 
 // Few rows (single tokens, drafts): the workgroup's four wavefronts share 16 * NT rows and split the
 // keys.  Every code is used once, so they go from memory to registers, and memory is the bound: 64 requests of up to 16384 keys
-// (8 heads of 128, 570 MB) 128 us, 4.5 TB/s, of one length 115 us, 5.0; 8 of up to 131072 (4 of 256) 156 to 163 us, 4.2 to 4.4, where
+// (8 heads of 128, 570 MB) 128 us, 4.5 TB/s, of one length 115 us, 5.0; 8 of up to 131072 (4 of 256) 156 us, 4.4, where
 // conversions of 16 rows for the 6 of a group count too.  A single request's 1025 keys take 6.7 us and their join 3.7, a launch and
-// four dependent loads each.  Keys through LDS, with half the accesses to L1, take as long; so do the next block's codes
-// loaded ahead into registers (140 against 137), and a launch bound for four wavefronts a SIMD spills (130 against 116).
+// four dependent loads each.  Keys through LDS, with half the accesses to L1, take as long; so do, but for heads
+// of 256, the next block's codes loaded ahead, and a launch bound for four wavefronts a SIMD spills (130 against 116).
 // WIDE: byte offsets into the keys or values pass 32 bits; else a lane's address is one register
 // beside a scalar base.
 template <typename T, int D, int NT, bool WIDE>
@@ -616,13 +616,14 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     const uint64_t tiles = static_cast<uint64_t>(p.slots) * c.kv_heads, blocks = longest / 64 + 1;
     uint64_t parts;
     if (p.shared) {
-        // Four workgroups a CU were every request as long as max_length where there are no more tiles than CUs (4 / 8 requests of up to 16384
-        // keys, 8 heads of 128, with 8 and 4 workgroups 22.7 -> 19.8 and 31 -> 26.4 us, 16 of 4000 26 -> 23.4; heads of 256, 3 requests of
-        // up to 131072 110 -> 92, 64 of up to 2000 35 -> 31, but 8 of up to 131072 152 -> 156), eight where they do not (64 requests of 8192
-        // keys 125 -> 115), so that long requests among short ones do not finish last; four blocks a part at least, one for each
-        // wavefront.  Where the tiles alone fill the chip, up to twelve, as long as a part has 48 blocks of 128 dimensions (64 requests
-        // of up to 16384 keys, heads of 128, with 8 / 12 / 16 workgroups a CU 138 / 130 / 132 us, heads of 64 81 / 87 / 83).
-        const uint64_t most = (tiles <= cus ? 4ull : 8ull) * cus / tiles;
+        // Four workgroups a CU were every request as long as max_length, so that long requests among short ones do not finish last,
+        // where there are no more tiles than CUs, and for heads of 256, of which two fit a CU (with 8 and 4 workgroups, 8 heads of
+        // 128: 4 requests of up to 16384 keys 22.7 -> 19.8 us, 8 31 -> 26.4, 16 of 4000 26 -> 23.4; 4 heads of 256: 3 requests of up to
+        // 131072 110 -> 92, 64 of up to 2000 35 -> 31, but 8 of up to 131072 152 -> 156); else eight (64 requests of 8192 keys 125 ->
+        // 115); four blocks a part at least, one for each wavefront.  Where the tiles alone fill the chip, up to twelve, as long as a
+        // part has 48 blocks of 128 dimensions (64 requests of up to 16384 keys, heads of 128, with 8 / 12 / 16 workgroups a CU 138 /
+        // 130 / 132 us, heads of 64 81 / 87 / 83).
+        const uint64_t most = (tiles <= cus || c.head_dim == 256 ? 4ull : 8ull) * cus / tiles;
         parts = (blocks + 3) / 4;
         if (parts > most) parts = most;
         const uint64_t more = std::min<uint64_t>(12ull * cus / tiles, blocks * c.head_dim / 6144);
