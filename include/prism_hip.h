@@ -29,6 +29,13 @@
 #include <stddef.h>
 #include <stdint.h>
 
+/* This header is C99 and C++.  C99 has no unnamed unions; GNU compilers take them there when they are marked. */
+#ifdef __GNUC__
+#define PRISM_HIP_EXTENSION __extension__
+#else
+#define PRISM_HIP_EXTENSION
+#endif
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -371,11 +378,11 @@ void *prism_hip_stream(prism_hip_ctx *ctx);
  * itself: its bytes are set when it is written, and no other's change. */
 typedef struct prism_kv_cache {
     void *k, *v;
-    union {
+    PRISM_HIP_EXTENSION union {
         float *k_scale;
         uint8_t *k_exponent;
     };
-    union {
+    PRISM_HIP_EXTENSION union {
         float *v_scale;
         uint8_t *v_exponent;
     };
