@@ -475,14 +475,14 @@ __global__ __launch_bounds__(TOP ? 64 * kJoinWaves : 64) void k_logprobs_join(Lo
 struct Plan {
     uint32_t waves, parts, each, tiles, groups;
 };
-Plan plan_of(const prism_logprobs &a) {
+Plan plan_of(const prism_logprobs &a, uint32_t cus) {
     Plan p;
     p.waves = a.vocab <= 4 * kTile ? 1 : 4;
     const uint32_t tiles = (a.vocab + p.waves * kTile - 1) / (p.waves * kTile);
-    // Up to 256 rows are split until some 1024 workgroups share the logits, a tile for each wavefront at least; more keep the
-    // memory busy whole (rows of 151936 binary32 logits, 20 alternatives, whole / split: 200 rows 36 / 32 us, 256 42 / 38, 400
-    // 52 / 70, 900 106 / 145).
-    uint32_t parts = p.waves == 1 || a.tokens > 256 ? 1 : (1024 + a.tokens - 1) / a.tokens;
+    // Up to a row a CU are split until some four workgroups a CU share the logits, a tile for each wavefront at least; more keep the
+    // memory busy whole (rows of 151936 binary32 logits, 20 alternatives, 256 CUs, whole / split: 200 rows 36 / 32 us, 256 42 / 38,
+    // 400 52 / 70, 900 106 / 145).
+    uint32_t parts = p.waves == 1 || a.tokens > cus ? 1 : (4 * cus + a.tokens - 1) / a.tokens;
     if (parts > tiles) parts = tiles;
     if (parts > kMostParts) parts = kMostParts;
     uint32_t some = (tiles + parts - 1) / parts;
@@ -511,13 +511,13 @@ int logprobs_typed(const LogprobsArgs &p, uint32_t waves, int *err, hipStream_t 
 
 }  // namespace
 
-size_t logprobs_scratch_bytes(const prism_logprobs &a, uint32_t) {
-    const Plan q = plan_of(a);
+size_t logprobs_scratch_bytes(const prism_logprobs &a, uint32_t cus) {
+    const Plan q = plan_of(a, cus);
     return q.parts == 1 ? 0 : static_cast<size_t>(a.tokens) * q.parts * (sizeof(Softmax) + (a.top ? 4ull * q.groups * 256 : 0));
 }
 
-int launch_logprobs(const prism_logprobs &a, void *scratch, uint32_t, int *err, hipStream_t s) {
-    const Plan q = plan_of(a);
+int launch_logprobs(const prism_logprobs &a, void *scratch, uint32_t cus, int *err, hipStream_t s) {
+    const Plan q = plan_of(a, cus);
     LogprobsArgs p{a, q.parts, q.each, q.tiles, q.groups, static_cast<float *>(scratch), nullptr};
     p.sums = reinterpret_cast<Softmax *>(p.largest + (a.top ? static_cast<size_t>(a.tokens) * q.parts * q.groups * 256 : 0));
     if (a.dtype == PRISM_DTYPE_F32) return logprobs_typed<float>(p, q.waves, err, s);

@@ -21,6 +21,7 @@ std::vector<std::string> g_log;
 std::string g_note;
 bool g_capturing = false;
 size_t g_largest = ~size_t(0);
+int g_cus = 256;
 uintptr_t g_handle = 0x1000;
 struct Config {
     dim3 grid, block;
@@ -68,6 +69,7 @@ extern "C" {
 
 // The test's side.
 void stub_capture(int on) { g_capturing = on != 0; }
+void stub_cus(int n) { g_cus = n; }  // of the contexts created from now on
 void stub_largest(size_t bytes) { g_largest = bytes; }
 int stub_alive(void *p) { return find(p) != nullptr; }
 size_t stub_allocations() { return g_ranges.size(); }
@@ -102,7 +104,7 @@ hipError_t hipGetDeviceCount(int *n) { return *n = 1, hipSuccess; }
 hipError_t hipSetDevice(int) { return hipSuccess; }
 hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600 *p, int) {
     std::memset(p, 0, sizeof *p);
-    p->multiProcessorCount = 256;
+    p->multiProcessorCount = g_cus;
     std::strcpy(p->gcnArchName, "gfx950");
     return hipSuccess;
 }

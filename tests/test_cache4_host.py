@@ -92,6 +92,28 @@ def test_a_call_made_once_uncaptured_can_be_captured(stub):  # noqa: F811
         """))
 
 
+def test_log_probabilities_are_split_by_the_devices_size(stub):  # noqa: F811
+    """Rows are split over workgroups up to a row a CU, until there are four workgroups a CU."""
+    stub(dedent("""
+        def grids(tokens, vocab=151936):
+            S.stub_log()
+            score(tokens=tokens, vocab=vocab, stride=vocab)
+            return [int(l.split(" grid ")[1].split()[0]) for l in S.stub_log().decode().splitlines() if l.startswith("launch")]
+        for cus in (256, 64, 32):
+            S.stub_cus(cus)
+            ctx = ph.Context(0)
+            for tokens in (1, 5, cus // 4, cus // 2, cus - 1, cus, cus + 1, 3 * cus):
+                got = grids(tokens)
+                if tokens > cus:
+                    assert got == [tokens], (cus, tokens, got)
+                    continue
+                # 38 tiles of four wavefronts, a part with a tile or more.
+                parts = min(-(-4 * cus // tokens), 38)
+                assert got == [tokens * -(-38 // -(-38 // parts)), tokens], (cus, tokens, got)
+            assert grids(5, 4096) == [5]
+        """))
+
+
 def test_oracle_codes_are_the_nearest():
     """Each code's own value, the borders between neighbours and points on both sides of them."""
     levels = co.LEVELS[:8]
