@@ -436,7 +436,8 @@ void prism_hip_rope_destroy(prism_hip_rope *rope);
 /* out[t][h] = the rotation of x[t][h] (head_dim 64, 128 or 256 values of type dtype) by
  * positions[t]; norm, if not NULL, first takes x to x / sqrt(mean(x^2) + eps) * norm[i]
  * (binary32 norm[head_dim]).  Computed in binary64, rounded once to binary32 and from
- * there to the type.  Strides are elements between tokens, at least heads * head_dim;
+ * there to the type; without a norm, values behind the rotation's dims come out as they are.
+ * Strides are elements between tokens, at least heads * head_dim;
  * out may be x with the same stride.  A non-finite x, or a result past the type's largest
  * value, is PRISM_ERR_NONFINITE at sync. */
 int prism_hip_rope_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, int dtype, const void *x, uint64_t x_stride,

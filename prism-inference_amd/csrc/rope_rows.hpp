@@ -164,13 +164,18 @@ __global__ __launch_bounds__(256) void k_rope(RopeRows a, RopeRows b, Rotation r
                     }
                 }
                 f32x4 o0, o1;
+                if (turns) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const double p = INTERLEAVED ? y[2 * j] : y[j], q = INTERLEAVED ? y[2 * j + 1] : y[4 + j];
-                    const float f = static_cast<float>(__builtin_fma(p, c[j], -(q * s[j])));
-                    const float g = static_cast<float>(__builtin_fma(q, c[j], p * s[j]));
-                    if constexpr (INTERLEAVED) (j < 2 ? o0 : o1)[2 * (j & 1)] = f, (j < 2 ? o0 : o1)[2 * (j & 1) + 1] = g;
-                    else o0[j] = f, o1[j] = g;
+                    for (int j = 0; j < 4; ++j) {
+                        const double p = INTERLEAVED ? y[2 * j] : y[j], q = INTERLEAVED ? y[2 * j + 1] : y[4 + j];
+                        const float f = static_cast<float>(__builtin_fma(p, c[j], -(q * s[j])));
+                        const float g = static_cast<float>(__builtin_fma(q, c[j], p * s[j]));
+                        if constexpr (INTERLEAVED) (j < 2 ? o0 : o1)[2 * (j & 1)] = f, (j < 2 ? o0 : o1)[2 * (j & 1) + 1] = g;
+                        else o0[j] = f, o1[j] = g;
+                    }
+                } else {  // as they are: a turn by nothing would lose a zero's sign, and an infinity's neighbours
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o0[j] = static_cast<float>(y[j]), o1[j] = static_cast<float>(y[4 + j]);
                 }
                 over |= !(most_of(o0, o1) < kPast<T>);
                 if constexpr (kAppends) {

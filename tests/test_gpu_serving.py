@@ -233,6 +233,42 @@ def test_gpu_rope_flags_a_nonfinite_row_and_keeps_the_others(ctx):
     rope.close()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,dims", [(64, 8), (64, 34), (128, 64), (128, 66), (256, 64), (256, 192)])
+def test_gpu_rope_leaves_what_stands_behind_the_rotated_dims(ctx, dtype, d, dims):
+    """Without a norm the values behind the rotated ones come out bit for bit: zeros of both signs, subnormals, and what stands next to an
+    infinity; with one, zeros keep their signs.  Several heads a wavefront and heads left over."""
+    rng = np.random.default_rng(d + dims)
+    tokens, heads = 5, 9
+    x = rng.standard_normal((tokens, heads, d))
+    x[:, :, dims::3] = -0.0
+    x[:, ::2, dims + 1::5] = 0.0
+    x[:, 1::3, dims + 5] = {"f32": 1e-42, "f16": 2.0 ** -24, "bf16": 2.0 ** -130}[dtype]
+    freq = ph.rope_frequencies(dims, 1e4)
+    bits = lambda v: np.ascontiguousarray(np.asarray(v, np.float64)).view(np.uint64)  # noqa: E731
+    for interleaved in (False, True):
+        rope = ph.Rope(ctx, dims, freq, interleaved=interleaved)
+        for infinite, normed in ((False, False), (True, False), (False, True)):
+            y = x.copy()
+            if infinite:
+                y[1, 2, dims + 6], y[3, 8, d - 1] = np.inf, -np.inf
+            rows, out = Rows(y, dtype, pad=3), Rows(np.ones_like(y), dtype)
+            norm = np.full(d, 1.5, np.float32)
+            ctx.rope_device(rope, DTYPE[dtype], rows, rows.stride, i32(np.arange(tokens) * 7), tokens, heads, d, out, out.stride,
+                            norm=dev(norm) if normed else None, eps=EPS)
+            assert ctx.sync() == (ph.ERR_NONFINITE if infinite else 0)
+            got = out.read()
+            if normed:
+                zero = rows.x[:, :, dims:] == 0
+                assert np.array_equal(bits(got[:, :, dims:])[zero], bits(rows.x[:, :, dims:])[zero])
+            else:
+                assert np.array_equal(bits(got[:, :, dims:]), bits(rows.x[:, :, dims:]))
+            want = so.rope(rows.x[:, :, :dims], np.arange(tokens) * 7, freq, dims, interleaved, 1.0)
+            if not normed:
+                assert (np.abs(got[:, :, :dims] - want) <= (so.HALF[dtype] + 2.0 ** -24) * np.abs(want) * 1.001 + so.TINY[dtype] + 1e-9).all()
+        rope.close()
+
+
 @pytest.mark.parametrize("dims", [64, 66])
 @pytest.mark.parametrize("dtype,most", [("f32", 3e38), ("f16", 6e4), ("bf16", 3.3e38)])
 def test_gpu_rope_flags_results_past_the_type(ctx, dtype, most, dims):
