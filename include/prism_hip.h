@@ -445,7 +445,7 @@ int prism_hip_rope_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, int dt
                           const float *norm, float eps, void *out, uint64_t out_stride, void *stream);
 
 /* Writes tokens of k and v [tokens][kv_heads][head_dim] to the cache's slots.  For every
- * page and head that receives tokens, M the largest magnitude among them:
+ * page and head that receives tokens, M the largest finite magnitude among them (0 if none is finite):
  *   s = max(the page's scale, or 0 where the page's first place is written now; 2^e),
  *       e the least integer >= -100 with M <= qmax * 2^e (qmax 127 or 448);
  *   tokens: code(x / s), ties to even; where s grew, the codes of the places before the
@@ -457,11 +457,12 @@ int prism_hip_rope_device(prism_hip_ctx *ctx, const prism_hip_rope *rope, int dt
  * consecutive slots.  A slot outside the cache, or a page's token that does not follow the
  * one before it and those that follow it, are not written and PRISM_ERR_INVALID_INPUT at sync; the same page in
  * two places of the batch is the caller's error and leaves that page undefined.  A NaN
- * is stored as 0, an infinity as the largest code, and either is PRISM_ERR_NONFINITE.
+ * is stored as 0, an infinity as the largest code under that scale, and either is PRISM_ERR_NONFINITE.
  * PRISM_CACHE_E2M1: slots in any order; every 32 dimensions of a token and head by themselves, M their
- * largest magnitude, e the least integer from -23 to 13 with M <= 6 * 2^e (13 if none): code(x / 2^e), ties to
- * the even code.  A magnitude past 49152 is stored as the largest code and is PRISM_ERR_NONFINITE, as a NaN (0)
- * and an infinity are.  The same slot twice in the batch is the caller's error and leaves that slot undefined. */
+ * largest finite magnitude (0 if none is finite), e the least integer from -23 to 13 with M <= 6 * 2^e (13 if
+ * there is none): code(x / 2^e), ties to the even code.  A magnitude past 49152 is stored as the largest code and is
+ * PRISM_ERR_NONFINITE.  So are a NaN, stored as 0, and an infinity, stored as the largest code: 6 * 2^e of the
+ * e that the finite values ask for, -23 beside zeros.  The same slot twice in the batch is the caller's error and leaves that slot undefined. */
 int prism_hip_kv_append_device(prism_hip_ctx *ctx, const prism_kv_cache *cache, int dtype, const void *k,
                                uint64_t k_stride, const void *v, uint64_t v_stride, const int32_t *slots,
                                uint32_t tokens, void *stream);

@@ -129,3 +129,16 @@ def test_oracle_codes_are_the_nearest():
     assert (e == 140).all() and (b == 0x77).all()
     b, e = co.quantized(np.concatenate([np.full(32, 6.0), np.full(32, 6.0001)])[None])
     assert e.tolist() == [[127, 128]]
+
+
+def test_oracle_scales_follow_the_finite_values():
+    """An infinity takes the largest code at the exponent that the finite values ask for; a NaN is 0."""
+    x = np.zeros((5, 32))
+    x[0, 3], x[1, 3], x[2, 3], x[3, :] = np.inf, -np.inf, np.nan, np.inf
+    x[4, 3], x[4, 9] = np.inf, 5.0
+    b, e = co.quantized(x)
+    values = co.values({"k": b[None, None], "k_scale": e.T[None, None], "format": "e2m1"}, "k")[0, 0]
+    least = 6 * 2.0 ** -23
+    assert e[:, 0].tolist() == [104, 104, 104, 104, 127]
+    assert values[0, 3] == least and values[1, 3] == -least and values[2, 3] == 0 and (values[3] == least).all()
+    assert values[4, 3] == 6 and values[4, 9] == 4  # 5 stands between 4 and 6, and 4 has the even code

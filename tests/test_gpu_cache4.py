@@ -151,6 +151,40 @@ def test_gpu_append4_flags_what_it_cannot_hold(ctx, dtype, past):
             held.check(co.append(cache, k.x, v.x, slots, page))
 
 
+@pytest.mark.parametrize("rotated", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_gpu_append4_scales_follow_the_finite_values(ctx, dtype, rotated):
+    """Infinities beside zeros, small values and nothing else, NaNs alone: each group by itself, its neighbours as ever."""
+    rng = np.random.default_rng(22)
+    d, page, kv, tokens = 64, 16, 2, 6
+    x = rng.standard_normal((tokens, kv, d)) * 2.0 ** -5
+    x[0, 0, :32], x[0, 0, 7] = 0.0, np.inf
+    x[1, 1, 40] = -np.inf
+    x[2, 0, 32:] = np.inf
+    x[3, 1, :32] = np.nan
+    x[4, 0, 5], x[4, 0, 6] = np.nan, np.inf
+    x[5, :, 33:40] = -0.0
+    k, v, q = Rows(x, dtype), Rows(x[::-1].copy(), dtype), Rows(np.zeros((tokens, 1, d)), dtype)
+    slots, held = rng.permutation(2 * page)[:tokens], None
+    cache = make_cache(rng, 2, kv, page, d)
+    if rotated:  # by nothing: positions of zero
+        held, rope = Device(cache, page), ph.Rope(ctx, 8, ph.rope_frequencies(8, 1e4))
+        ctx.qkv_append_device(rope, held.desc, ph.QkvAppend(dtype=DTYPE[dtype], tokens=tokens, heads=1, q=q, k=k, v=v, q_stride=q.stride, k_stride=k.stride,
+                                                            v_stride=v.stride, positions=i32(np.zeros(tokens)), slots=i32(slots), q_norm=None, k_norm=None,
+                                                            eps=EPS, q_out=q, q_out_stride=q.stride))
+        rc = ctx.sync()
+        rope.close()
+    else:
+        held, rc = run_append(ctx, cache, k, v, slots, page)
+    assert rc == ph.ERR_NONFINITE and ctx.sync() == 0
+    kx = k.x.copy()
+    if rotated:  # a pair's partner of an infinity, times a sine of 0, is NaN: of dimensions 0 to 3 and 4 to 7
+        with np.errstate(invalid="ignore"):
+            a, b = kx[..., :4].copy(), kx[..., 4:8].copy()
+            kx[..., :4], kx[..., 4:8] = a * 1.0 - b * 0.0, b * 1.0 + a * 0.0
+    held.check(co.append(cache, kx, v.x, slots, page))
+
+
 def test_gpu_append4_flags_slots_outside(ctx):
     rng = np.random.default_rng(4)
     d, page, kv = 128, 16, 2
