@@ -392,6 +392,32 @@ def test_gpu_attention4_splits_long_caches(ctx, dtype, max_length):
         check(out.read(), want, tol)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["single", "drafts", "many"])
+def test_gpu_attention4_parts_of_many_blocks(ctx, kind, d, dtype):
+    """Every kernel going through dozens of blocks a part (one part a tile, some, and as many as there may be, more than eight of
+    them joined), with a page that is none and the start of a window far behind the first blocks."""
+    rng = np.random.default_rng(d + len(kind))
+    page, kv = 16, 2
+    heads, added, lengths = {"single": (8, [1, 1, 1], [9000, 3000, 70]),       # 4 rows a request
+                             "drafts": (16, [3, 4, 2], [9000, 3000, 70]),      # 24: two row tiles, but for heads of 256
+                             "many": (2, [70, 90], [9000, 3000])}[kind]
+    offsets = np.concatenate([[0], np.cumsum(added)])
+    table, pages = make_table(rng, lengths, page)
+    cache = make_cache(rng, pages, kv, page, d)
+    held = Device(cache, page)
+    q = Rows(rng.standard_normal((offsets[-1], heads, d)), dtype, pad=4)
+    wrong = table.copy()
+    wrong[0, 8200 // page] = -1
+    for window in (0, 1500):
+        want, tol = co.attention(cache, q.x, offsets, lengths, table, page, d ** -0.5, True, window, dtype, drop=[(0, 8200 // page)])
+        for max_length in (0, 9000, 100000):
+            call, out = attend(ctx, held, q, offsets, lengths, wrong, d ** -0.5, True, window, max_length=max_length)
+            assert ctx.sync() == ph.ERR_INVALID_INPUT and ctx.sync() == 0
+            check(out.read(), want, tol)
+
+
 @pytest.mark.parametrize("added", [[1, 1, 1], [40, 3, 50]])
 def test_gpu_attention4_rows_without_keys(ctx, added):
     """Requests without keys, tokens before the first key: zeros, and the rows behind the last request stay as they were."""
@@ -504,6 +530,35 @@ def test_gpu_attention4_flags_lengths_and_offsets(ctx):
         assert ctx.sync() == ph.ERR_INVALID_INPUT and ctx.sync() == 0
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("added", [1, 9, 40])
+def test_gpu_attention4_writes_the_valid_requests_alone(ctx, added, dtype):
+    """Beside a request with a length that cannot be, the others are right; its rows, and whatever stands beside rows, stay as they were.
+    Offsets out of order write no other memory than rows."""
+    rng = np.random.default_rng(23)
+    page, d, heads, kv = 16, 64, 8, 2
+    good, offsets = [40, 33, 47], np.arange(4) * added
+    table, pages = make_table(rng, good, page)
+    cache = make_cache(rng, pages, kv, page, d)
+    held = Device(cache, page)
+    q = Rows(rng.standard_normal((3 * added + 2, heads, d)), dtype)
+    want, tol = co.attention(cache, q.x, offsets, good, table, page, 0.1, True, 0, dtype)
+    for wrong in range(3):
+        for n in (-1, 1000, 65, -(1 << 31), (1 << 31) - 1):  # the table has four columns of 16
+            lengths = [n if r == wrong else x for r, x in enumerate(good)]
+            call, out = attend(ctx, held, q, offsets, lengths, table, 0.1, max_length=64)
+            assert ctx.sync() == ph.ERR_INVALID_INPUT and ctx.sync() == 0
+            got, rows = out.read(), slice(added * wrong, added * wrong + added)
+            assert (got[rows] == 3.0).all() and (got[3 * added:] == 3.0).all()
+            others = np.r_[0:added * wrong, added * wrong + added:3 * added]
+            check(got, want, tol, others)
+    t = len(q.x)
+    for bad in ([0, 2, 1, 3], [0, 1, 2, t + 1], [-1, 1, 2, 3], [0, t, 0, t], [0, -5, 2, 3], [0, (1 << 31) - 1, 2, 3]):
+        call, out = attend(ctx, held, q, bad, good, table, 0.1, max_length=64)
+        assert ctx.sync() == ph.ERR_INVALID_INPUT and ctx.sync() == 0
+        out.read()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("added", [1, 40])
 def test_gpu_attention4_flags_nonfinite_rows(ctx, dtype, added):
@@ -610,6 +665,86 @@ def test_gpu_cache4_past_32_bits(ctx, added, d):
         assert np.array_equal(got.read(), co.values(small, m).swapaxes(1, 2).reshape(-1, kv, d)[:n])
     want, tol = co.attention(small, q.x, [0, added], [n], np.arange(4)[None], page, 0.1, True, 0, "f16")
     check(out.read(), want, tol)
+
+
+def far_cache4(d):
+    """A cache of 8 GB of codes each, and the pages that are used."""
+    page, kv = 256, 8
+    pages = (1 << 33) // (page * kv * d // 2) + 40
+    buf = {n: DeviceBuffer(pages * kv * page * d // 2) for n in ("k", "v")}
+    buf.update({n: DeviceBuffer(pages * kv * page * d // 32) for n in ("k_scale", "v_scale")})
+    return ph.KvCache(**buf, format=ph.CACHE_E2M1, pages=pages, page_size=page, kv_heads=kv, head_dim=d), buf, [pages - 1, 3, pages // 2 + 5, pages - 9]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("added", [1, 20, 70, 300])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_gpu_attention4_past_32_bits_in_every_form(ctx, added, d, dtype):
+    """Codes past 4 GB: one and two row tiles, 64 and 128 rows a workgroup, one part and several, binary32 and 16 bits."""
+    page, kv, n = 256, 8, 3 * 256 + 77
+    heads = 512 if added == 300 and dtype == "f32" and d < 256 else 8  # 128 rows a workgroup in binary32
+    desc, buf, use = far_cache4(d)
+    rng = np.random.default_rng(24)
+    small = make_cache(rng, 4, kv, page, d)
+    for m, b in buf.items():
+        for i, at in enumerate(use):
+            b.upload(small[m][i], at * small[m][i].nbytes)
+    q = Rows(rng.standard_normal((added, heads, d)), dtype)
+    held = type("Held", (), {"desc": desc})
+    want, tol = co.attention(small, q.x, [0, added], [n], np.arange(4)[None], page, 0.1, True, 0, dtype)
+    for max_length in (0, n, 2000):
+        call, out = attend(ctx, held, q, [0, added], [n], np.array([use]), 0.1, max_length=max_length)
+        assert ctx.sync() == 0
+        check(out.read(), want, tol)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("d", [64, 256])
+def test_gpu_read8_past_32_bits(ctx, fmt, d):
+    """Pages of an 8-bit cache whose codes stand past 4 GB, read back."""
+    page, kv = 64, 8
+    pages = (1 << 33) // (page * kv * d) + 40
+    rng = np.random.default_rng(25)
+    small = make_cache8(rng, 4, kv, page, d, fmt)
+    if fmt == "e4m3":
+        for n in ("k", "v"):
+            small[n] = np.where(small[n] & 127 == 127, 126, small[n]).astype(np.uint8)
+    buf = {n: DeviceBuffer(pages * kv * page * d) for n in ("k", "v")}
+    buf.update({n: DeviceBuffer(4 * pages * kv) for n in ("k_scale", "v_scale")})
+    desc = ph.KvCache(**buf, format={"int8": ph.CACHE_INT8, "e4m3": ph.CACHE_E4M3}[fmt], pages=pages, page_size=page, kv_heads=kv, head_dim=d)
+    use = np.array([pages - 1, 3, pages // 2 + 5, pages - 9])
+    for m, b in buf.items():
+        for i, at in enumerate(use):
+            b.upload(small[m][i], int(at) * small[m][i].nbytes)
+    x = {m: so.rounded(co.values(small, m).swapaxes(1, 2).reshape(-1, kv, d), "f32") for m in ("k", "v")}
+    for order in (np.arange(3, 4 * page - 5), rng.permutation(4 * page)):
+        slots = use[order // page] * page + order % page
+        k, v = (Rows(np.zeros((len(order), kv, d)), "f32") for _ in range(2))
+        ctx.kv_read_device(desc, ph.DTYPE_F32, i32(slots), len(order), k, k.stride, v, v.stride)
+        assert ctx.sync() == 0
+        assert np.array_equal(k.read(), x["k"][order]) and np.array_equal(v.read(), x["v"][order])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [128, 256])
+def test_gpu_attention4_same_result_each_time_in_16_bits(ctx, d, dtype):
+    """Single tokens over many parts and chunks, other calls between: every repeat gives the same bits."""
+    rng = np.random.default_rng(26)
+    page, heads, kv, lengths = 16, 16, 4, [5000, 900, 17]
+    table, pages = make_table(rng, lengths, page)
+    held = Device(make_cache(rng, pages, kv, page, d), page)
+    other = Rows(rng.standard_normal((3, heads, d)), "f32")
+    for added in ([1, 1, 1], [150, 90, 17]):
+        offsets = np.concatenate([[0], np.cumsum(added)])
+        q = Rows(rng.standard_normal((offsets[-1], heads, d)), dtype)
+        first = None
+        for _ in range(5):
+            attend(ctx, held, other, [0, 1, 2, 3], lengths, table, 0.1)
+            call, out = attend(ctx, held, q, offsets, lengths, table, 0.1)
+            assert ctx.sync() == 0
+            got = out.read()
+            assert first is None or np.array_equal(first, got)
+            first = got
 
 
 def test_gpu_attention4_same_result_each_time(ctx):
