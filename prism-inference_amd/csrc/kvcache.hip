@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256) void k_plan_fill(prism_kv_plan p, PlanScratch 
 // Dims that are multiples of 8 take k_rope (rope_rows.hpp).
 
 // Any dims: a lane has four consecutive elements and looks their partners up, one row in flight (4099 tokens x 24 heads of
-// 256 bf16 with 66 dims take 45 us where k_rope takes 20 with 64).
+// 256 bf16 with 66 dims take 64 us where k_rope takes 26 with 64; 6030 x 40 of 128 with norms 181 where it takes 33).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_rope_any(RopeRows a, RopeRows b, Rotation rot, const int32_t *positions, uint32_t tokens,
                                                   uint32_t heads_each, double eps, int *err) {
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256) void k_rope_any(RopeRows a, RopeRows b, Rotati
 // scale and codes have one writer and no result depends on timing.  Runs that a wavefront's
 // registers hold (single tokens above all) go to one wavefront each, longer ones to all four, which
 // exchange their magnitudes.  Earlier codes of the page are rewritten only where the scale grew.
-// 8192 bf16 tokens of 8 heads of 128 into e4m3 pages of 64 take 17 us (50 MB, 2.9 TB/s), 48 ragged f16 chunks of 4 heads of
+// 6030 bf16 tokens of 8 heads of 128 into e4m3 pages of 64 take 17.5 us (37 MB, 2.1 TB/s), 48 ragged f16 chunks of 4 heads of
 // 256 20 us, 32 single f32 tokens 4 us: a few chains of loads per wavefront and its VALU work, not yet memory.
 
 template <int FMT>

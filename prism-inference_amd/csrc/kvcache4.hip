@@ -92,7 +92,7 @@ __device__ __forceinline__ void read_keys(const ReadArgs &a, uint32_t block, uin
 }
 // 8 bits, values, which a page holds by dimension: D / 4 lanes take eight tokens, a lane four dimensions.  Tokens that follow each
 // other stand in one or two runs of sixteen places, which a lane loads whole, sixteen bytes a dimension, before it writes
-// any token; others load a byte a value.  The values of 8192 tokens of 8 heads of 128 take 10.9 us this way, a byte a value 19.5, runs
+// any token; others load a byte a value.  Each run is loaded by both windows of its sixteen places, and a window within one run loads it twice.  The values of 8192 tokens of 8 heads of 128 take 10.9 us this way, a byte a value 19.5, runs
 // loaded in the loop over the tokens 22 (a load's wait is one for every store before it too); windows of 16 tokens are as fast
 // there and slower where requests end inside them (40 of 1 to 333 tokens: 11.7 and 7.9), windows of 4 take 13.8 and 7.3.
 constexpr uint32_t kWindow = 8;
@@ -188,8 +188,9 @@ int append4_typed(const Append4Args &a, int *err, hipStream_t s) {
 }
 
 // A step's rotation and both appends in one launch: rotated keys go into codes without a pass through memory, and a step of 32
-// requests takes 4.4 us (two launches 8.1).  6030 tokens of 32 + 2 x 8 heads of 128, bf16, take 37 us for 130 MB, 3.5 TB/s, and
-// without norms 30, 4.3 TB/s: between them stand the norms' sums and products in binary64.  In binary32 54 us, 4.8 TB/s.
+// requests takes 4.4 us (two launches 8.1).  6030 tokens of 32 + 2 x 8 heads of 128, bf16, take 42 us from and to HBM, 130 MB, 3.1 TB/s (33
+// where the last-level cache has them), and without norms 36 (27): between them stand the norms' sums and products in binary64, whose issue
+// is the bound.  In binary32 55 us, 4.6 TB/s.
 // More workgroups to a token's heads are slower (twice as many 45 us: each makes the cosines again).
 template <typename T, int D>
 int qkv4_typed(const Rotation &rot, const RopeRows &q, const RopeRows &k, const int32_t *positions, float eps, const Append4Args &a, int *err,

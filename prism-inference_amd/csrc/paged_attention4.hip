@@ -422,10 +422,11 @@ __global__ __launch_bounds__(256, D == 256 && sizeof(T) == 4 ? 1 : 2) void k_att
 
 // Many rows (prompts, chunks): each of WAVES wavefronts has 16 * NT rows of its own and all keys.  A block's codes are
 // converted to binary16 once by the workgroup, a quarter of the keys (or of eight wavefronts half the dimensions of one) by each
-// wavefront, into LDS in the order of the operands; the next block's codes come from memory meanwhile and are converted behind the products, so a
-// block costs one barrier.  Bounds: conversions, exponentials and their like fill 52 % of a SIMD's cycles and the matrix cores 37 %,
-// which add up, since two wavefronts a SIMD hardly ever issue both at once: a prompt of 8192 tokens, 32 heads of 128, takes 580 to 705 us
-// card by card, 780 to 950 TFLOP/s.
+// wavefront, into LDS in the order of the operands; the next block's codes come from memory meanwhile and are converted after the products, so a
+// block costs one barrier.  Bounds: conversions, exponentials and their like, at four cycles an instruction, fill 51 % of a SIMD's cycles and
+// the matrix cores 39 %.  They add up: the conversions stand behind a block's last product (both ends of the branch below compile to one), where
+// only the SIMD's other wavefront has products to issue beside them.  A prompt of 8192 tokens, 32 heads of 128, takes 580 to 705 us card by
+// card, 780 to 950 TFLOP/s.
 template <typename T, int D, int NT, int WAVES, bool WIDE>
 __global__ __launch_bounds__(64 * WAVES, D == 256 && WAVES == 4 ? 1 : 2) void k_attend4_tile(AttendArgs p, int *err) {
     typedef Rows4<T, D, NT> R;
@@ -593,6 +594,8 @@ Plan attend_plan(const prism_kv_cache &c, const prism_attention &a, uint32_t cus
     const uint32_t group = a.heads / c.kv_heads;
     const uint64_t typical = (static_cast<uint64_t>(a.tokens) * group + a.requests - 1) / a.requests;  // rows of a request
     Plan p;
+    // Drafts of 17 to 32 rows a request are faster here than on tiles of 64 rows, most of which they leave empty (64 requests of up to 16384 keys,
+    // 8 heads of 128, 24 / 32 rows each, bf16 168 / 254 us against 306 / 348, binary32 215 / 339 against 416 / 461; heads of 64 and 256 alike).
     p.shared = typical <= 32;
     auto slots_of = [&](uint32_t M) { return static_cast<uint32_t>(static_cast<uint64_t>(a.tokens) * group / M) + a.requests; };
     if (p.shared) {

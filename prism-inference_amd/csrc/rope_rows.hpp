@@ -12,9 +12,10 @@ namespace {
 // A workgroup rotates kRopeTokens tokens of some heads, a wavefront one token: the workgroup makes
 // their cosines and sines in binary64 first (one pair of them serves every head), then each lane
 // keeps those of its four pairs and takes the heads, several rows in flight.  binary64 FMAs
-// run at the binary32 rate here, so the exact rotation costs no more than a rounded one; memory
-// bounds it: 4099 tokens x 24 heads of 256 bf16 take 24 us, 4.2 TB/s, 8192 x 40 of 128 35 us, 4.8 TB/s
-// (a lane with four elements that looked their partners up, one row in flight: 56 and 137).
+// run at the binary32 rate here, so the exact rotation costs no more than a rounded one.  Memory
+// bounds it without norms: from and to HBM 4099 tokens x 24 heads of 256 bf16, interleaved, take 26 us, 3.9 TB/s, 8192 x 40 of
+// 128 37 us, 4.5 TB/s (a lane with four elements that looked their partners up, one row in flight: 56 and 137).  Norms, whose
+// sums, roots and products are binary64 too, make them 29 and 41 us.
 
 constexpr uint32_t kRopeTokens = 4;
 

@@ -31,7 +31,7 @@ struct OnDevice {
     OnDevice &operator=(const OnDevice &) = delete;
 };
 
-// Bounds that keep every grid below 2^32 work-items.
+// Bounds that keep every dimension of a grid below 2^32 work-items.
 constexpr uint64_t kMostTokens = 1u << 23, kMostHeads = 1u << 12, kMostRows = 1u << 26, kMostWords = 1u << 24;
 
 bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
